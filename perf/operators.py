@@ -209,9 +209,9 @@ def _prepare_own(case, s):
                  out=_empty(n * case["k"], case["rows"], dtype=case["out"]))
     else:
         s.update(out=_empty(n, case["cols"], dtype=case["out"]))
-    if kind == "quantize" or case.get("x") == "mxfp4":  # the rows' codes and scales
-        m, cols = len(s["x"]), case["cols"]
-        s.update(codes=_empty(m, cols // 2, dtype=torch.uint8), scales=_empty(m, cols // 32, dtype=torch.uint8))
+    if kind == "quantize" or case.get("x") == "mxfp4":  # the rows' codes and scales, rows padded to 128 values
+        m, units = len(s["x"]), -(-case["cols"] // 128)
+        s.update(codes=_empty(m, 64 * units, dtype=torch.uint8), scales=_empty(m, 4 * units, dtype=torch.uint8))
 
 
 # ------------------------------------------------------------ one pass
