@@ -40,6 +40,12 @@ extern "C" {
 #define TINYOAI_Q5_K 13
 #define TINYOAI_Q6_K 14
 #define TINYOAI_BF16 30
+/* Microscaled 4-bit floating point: the type of single weights and experts
+ * only (below), no counterpart in the reference. Blocks {e8m0 scale s,
+ * 16 bytes} of 32 values, byte j holding the codes of values j (low half) and
+ * j + 16; a code is sign, two exponent bits and a fraction bit (0, 0.5, 1, 1.5,
+ * 2, 3, 4, 6), its value code * 2^(s - 127); s = 255 makes the block NaN. */
+#define TINYOAI_MXFP4 39
 
 typedef struct tinyoai_model tinyoai_model;
 typedef struct tinyoai_weight tinyoai_weight;
@@ -307,6 +313,76 @@ int tinyoai_weight_mul_device(tinyoai_weight *w, const float *x_dev, int32_t n, 
  * array. */
 int tinyoai_weight_mul_device_noalloc(tinyoai_weight *w, const float *x_dev, int32_t n, float *out_dev, void *stream);
 int tinyoai_weight_free(tinyoai_weight *w);
+
+/* ---------------- mixture-of-experts operators (no counterpart in the reference) ----------------
+ *
+ * Device buffers throughout; every call enqueues on `stream` (a hipStream_t)
+ * without synchronizing. NULL is the handle's own stream where the call takes
+ * a handle, else the current device's default stream. All may be captured;
+ * none allocates but the products (their scratch as tinyoai_weight_mul_device's).
+ * Types are TINYOAI_F32, TINYOAI_F16 and TINYOAI_BF16; rows of a buffer are
+ * `ld` values apart.
+ *
+ * MXFP4 rows: for each row 64 bytes of codes (two a byte, the earlier value in
+ * the low half) and 4 scale bytes per 128 columns, ceil(cols / 128) of them;
+ * columns past `cols` hold zeros, as tinyoai_mxfp4_quantize_device writes them.
+ * Codes lie on a 16-byte boundary, scales on a 4-byte one. */
+
+/* n rows of `cols` values (a multiple of 32) to MXFP4: a block's scale is
+ * 2^(floor(log2 m) - 2), m its largest magnitude, within 2^-127 .. 2^127; values
+ * over the scale go to the nearest code, halfway ones to the even code, those
+ * past 6 to 6. A block with an infinity or NaN becomes NaN (scale 255). */
+int tinyoai_mxfp4_quantize_device(int32_t dtype, const void *x_dev, int64_t ldx, int64_t n, int64_t cols,
+                                  uint8_t *codes_dev, uint8_t *scales_dev, void *stream);
+/* The values of MXFP4 rows (exact in fp32 and bf16 but for overflow to
+ * infinity; to fp16 rounded to the nearest). */
+int tinyoai_mxfp4_dequantize_device(const uint8_t *codes_dev, const uint8_t *scales_dev, int64_t n, int64_t cols,
+                                    int32_t dtype, void *out_dev, int64_t ldo, void *stream);
+/* out[n][rows] = x * W^T in fp32 for MXFP4 rows x and an MXFP4 weight
+ * (tinyoai_weight_upload): the 4-bit products are exact, their sums fp32. For
+ * fp32 rows, tinyoai_weight_mul and its device forms take MXFP4 weights as any
+ * other, at fp32 accuracy. The current device must be the weight's. */
+int tinyoai_weight_mul_mxfp4_device(tinyoai_weight *w, const uint8_t *codes_dev, const uint8_t *scales_dev, int32_t n,
+                                    float *out_dev, void *stream);
+
+/* Routing: the k best experts of each of n tokens by their logits [n][experts]
+ * (1 <= k <= 32, experts <= 1024, n * k <= 2^30), best first, ties to the lower
+ * expert, -0 equal to +0. Logits of -inf and NaN are never chosen: a token with
+ * fewer than k others gets id -1 and weight 0 in what is left. Weights are the
+ * softmax over the token's chosen logits, or with over_all nonzero over all of
+ * them (+inf: those experts share the weight evenly).
+ *   ids, weights [n][k]; the chosen (token, choice) pairs sorted by expert, by
+ *   token within one: expert e has rows offsets[e] .. offsets[e + 1] - 1
+ *   (offsets [experts + 1]); tokens [n * k] the token of each row, -1 past the
+ *   last; positions [n][k] each choice's row, or -1. */
+int tinyoai_route_device(int32_t dtype, const void *logits_dev, int64_t ld, int32_t n, int32_t experts, int32_t k,
+                         int32_t over_all, int32_t *ids_dev, float *weights_dev, int32_t *offsets_dev,
+                         int32_t *tokens_dev, int32_t *positions_dev, void *stream);
+/* out[t] = sum over j of weights[t][j] * y[positions[t][j]] for n tokens of k
+ * choices, in fp32 and in the order of j, rounded once; positions outside
+ * [0, y_rows) add nothing. */
+int tinyoai_combine_device(int32_t dtype, const void *y_dev, int64_t ldy, int32_t y_rows, const int32_t *positions_dev,
+                           const float *weights_dev, int32_t n, int32_t k, int64_t cols, int32_t out_dtype, void *out_dev,
+                           int64_t ldo, void *stream);
+
+/* `experts` matrices [rows][cols] of type MXFP4 or BF16, one after another in
+ * `data` (`nbytes` in all). With `up` (as `data`), each expert is a (gate, up)
+ * pair and its products are silu(gate) * up (stablelm.go:371-373). */
+typedef struct tinyoai_experts tinyoai_experts;
+int tinyoai_experts_upload(int32_t dtype, int32_t experts, int64_t rows, int64_t cols, const void *data, const void *up,
+                           uint64_t nbytes, tinyoai_experts **out);
+/* Products grouped by expert: out[r] = x[index[r]] * W_e^T (silu(gate) * up of
+ * pairs) for the rows r of expert e, offsets[e] <= r < offsets[e + 1] <= n, as
+ * tinyoai_route_device lists them; index NULL: x[r]. Other rows of out stay as
+ * they are. x: F32, F16 or BF16 [x_rows][ldx], or MXFP4 rows (x_scales_dev their
+ * scales, ldx = cols; MXFP4 experts). Sums are fp32: F32 and F16 rows count
+ * with all their bits. An index outside [0, x_rows) gives a row of zeros;
+ * offsets outside [0, n] or falling count as the nearest that are not. The
+ * current device must be the handle's. */
+int tinyoai_experts_mul_device(tinyoai_experts *e, int32_t x_dtype, const void *x_dev, const uint8_t *x_scales_dev,
+                               int64_t ldx, int32_t x_rows, const int32_t *offsets_dev, const int32_t *index_dev,
+                               int32_t n, int32_t out_dtype, void *out_dev, int64_t ldo, void *stream);
+int tinyoai_experts_free(tinyoai_experts *e);
 
 #ifdef __cplusplus
 }

@@ -20,9 +20,10 @@
 #include <utility>
 #include <vector>
 
+#include "experts.h"
 #include "kernels.h"
 #include "model.h"
-#include "scratch.h"
+#include "stream_scratch.h"
 
 LaunchTiming &launch_timing() {
   thread_local LaunchTiming t;
@@ -1910,21 +1911,16 @@ using namespace tinyoai;
 
 struct tinyoai_weight {
   DevMatrix m;
-  int device = 0;  // the device the weight lives on
+  ExpertMatrix mx;  // MXFP4: one matrix (m stays empty)
+  int device = 0;   // the device the weight lives on
   hipStream_t stream = nullptr;
-  // Operand planes and K-split partials of tinyoai_weight_mul_device: a
-  // buffer per stream (calls on one stream run in order; `mu` keeps one
-  // call's launches together), one that further streams share in turn
-  // (`shared_done`: after its last call), and buffers that captured graphs
-  // own.
-  std::mutex mu;
-  ScratchPool scratch;
-  hipEvent_t shared_done = nullptr;
+  // Operand planes and K-split partials of tinyoai_weight_mul_device.
+  StreamScratch scratch;
   ~tinyoai_weight() {
-    scratch.clear([](void *p) { hipFree(p); });
-    if (shared_done) hipEventDestroy(shared_done);
     if (stream) hipStreamDestroy(stream);
   }
+  int64_t rows() const { return mx.d.codes ? mx.d.rows : m.desc.rows; }
+  int64_t cols() const { return mx.d.codes ? mx.d.cols : m.desc.cols; }
 };
 
 extern "C" {
@@ -2329,7 +2325,8 @@ int tinyoai_weight_upload(int32_t dtype, int64_t rows, int64_t cols, const void 
   if (e != hipSuccess) return hip_fail(e, "hipGetDevice");
   e = hipStreamCreateWithFlags(&w->stream, hipStreamNonBlocking);
   if (e != hipSuccess) return hip_fail(e, "hipStreamCreate");
-  int rc = w->m.upload(dtype, rows, cols, data, nbytes, w->stream);
+  int rc = dtype == FMT_MXFP4 ? w->mx.upload(dtype, 1, rows, cols, data, nullptr, nbytes, w->stream)
+                              : w->m.upload(dtype, rows, cols, data, nbytes, w->stream);
   if (rc) return rc;
   e = hipStreamSynchronize(w->stream);
   if (e != hipSuccess) return hip_fail(e, "weight upload");
@@ -2338,13 +2335,14 @@ int tinyoai_weight_upload(int32_t dtype, int64_t rows, int64_t cols, const void 
 }
 
 int tinyoai_weight_read_values(tinyoai_weight *w, int64_t offset, int64_t n, float *out) {
-  if (!w || !out || offset < 0 || n < 0 || offset + n > (int64_t)w->m.desc.rows * w->m.desc.cols)
+  if (!w || !out || offset < 0 || n < 0 || offset + n > w->rows() * w->cols())
     return fail(TINYOAI_EINVAL, "invalid readValues span");
   if (n == 0) return TINYOAI_OK;
   float *dev;
   hipError_t e = device_alloc(&dev, (size_t)n * 4);
   if (e != hipSuccess) return fail(TINYOAI_ENOMEM, "hipMalloc: %s", hipGetErrorString(e));
-  e = launch_read_values(w->m.desc, offset, n, dev, w->stream);
+  e = w->mx.d.codes ? launch_mx_read(w->mx.d, offset, n, dev, w->stream)
+                    : launch_read_values(w->m.desc, offset, n, dev, w->stream);
   if (e == hipSuccess) e = hipMemcpyAsync(out, dev, (size_t)n * 4, hipMemcpyDeviceToHost, w->stream);
   if (e == hipSuccess) e = hipStreamSynchronize(w->stream);
   hipFree(dev);
@@ -2448,88 +2446,44 @@ static hipError_t product_launch(const Product &p, const Matrix &m, const float 
   return e;
 }
 
-namespace {
-// Allowing this thread's allocations while a stream is captured.
-struct RelaxedCapture {
-  hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
-  bool set = hipThreadExchangeStreamCaptureMode(&mode) == hipSuccess;
-  ~RelaxedCapture() {
-    if (set) hipThreadExchangeStreamCaptureMode(&mode);
-  }
-};
-// This thread's number, no other's before or after.
-uint64_t thread_number() {
-  static std::atomic<uint64_t> next{1};
-  thread_local const uint64_t number = next++;
-  return number;
+// The product of fp32 rows with an MXFP4 weight.
+static MxProduct mx_weight_product(const tinyoai_weight *w, const float *x, int n, float *out) {
+  return MxProduct{w->mx.d, FMT_F32, x, nullptr, w->mx.d.cols, n, nullptr, nullptr, n, FMT_F32, out, w->mx.d.rows};
 }
-}  // namespace
 
 extern "C" {
 
 int tinyoai_weight_mul_device(tinyoai_weight *w, const float *x_dev, int32_t n, float *out_dev, void *stream) try {
   if (!w || !x_dev || !out_dev || n <= 0) return fail(TINYOAI_EINVAL, "invalid product arguments");
   hipStream_t st = stream ? (hipStream_t)stream : w->stream;
+  if (w->mx.d.codes) {
+    const MxProduct p = mx_weight_product(w, x_dev, n, out_dev);
+    return w->scratch.run(st, mx_scratch(p), [&](void *scratch) { return launch_mx_product(p, scratch, st); });
+  }
   const Matrix &m = w->m.desc;
-  hipError_t e = hipSuccess;
   if (n == 1) {  // a few microseconds: no more host work than the launch
-    e = product_launch(Product{Route::row}, m, x_dev, n, out_dev, nullptr, st);
+    const hipError_t e = product_launch(Product{Route::row}, m, x_dev, n, out_dev, nullptr, st);
     return e == hipSuccess ? TINYOAI_OK : hip_fail(e, "product launch");
   }
   const Product p = plan_product(m, x_dev, n);
-  if (!p.bytes()) {
-    e = product_launch(p, m, x_dev, n, out_dev, nullptr, st);
-    return e == hipSuccess ? TINYOAI_OK : hip_fail(e, "product launch");
-  }
-  hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
-  unsigned long long id = 0;
-  hipGraph_t graph = nullptr;
-  if ((e = hipStreamGetCaptureInfo_v2(st, &cap, &id, &graph, nullptr, nullptr)) != hipSuccess)
-    return hip_fail(e, "hipStreamGetCaptureInfo");
-  // (under capture nothing is given back to make room: hipFree waits for the device)
-  const bool capturing = cap != hipStreamCaptureStatusNone;
-  auto alloc = [capturing](size_t bytes) {
-    RelaxedCapture relaxed;
-    void *ptr = nullptr;
-    if ((capturing ? hipMalloc(&ptr, bytes) : device_alloc(&ptr, bytes)) == hipSuccess) return ptr;
-    (void)hipGetLastError();
-    return static_cast<void *>(nullptr);
-  };
-  std::lock_guard<std::mutex> lock(w->mu);
-  ScratchPool::Lease lease;
-  if (capturing) {
-    ScratchPool::Record *made = nullptr;
-    lease.ptr = w->scratch.captured(id, st, p.bytes(), alloc, &made);
-    hipUserObject_t owner = nullptr;
-    if (made) {  // the graph's, and that of every executable graph made from it
-      e = hipUserObjectCreate(&owner, made, ScratchPool::release, 1, hipUserObjectNoDestructorSync);
-      if (e != hipSuccess) {
-        ScratchPool::release(made);
-        return hip_fail(e, "product scratch");
-      }
-      if ((e = hipGraphRetainUserObject(graph, owner, 1, hipGraphUserObjectMove)) != hipSuccess) {
-        hipUserObjectRelease(owner, 1);
-        return hip_fail(e, "product scratch");
-      }
-    }
-  } else {
-    lease = w->scratch.eager(st, st == hipStreamPerThread ? thread_number() : 0, p.bytes(), alloc);
-  }
-  if (!lease.ptr) return fail(TINYOAI_ENOMEM, "product scratch of %zu bytes", p.bytes());
-  if (lease.shared) {
-    RelaxedCapture relaxed;
-    if (!w->shared_done)
-      e = hipEventCreateWithFlags(&w->shared_done, hipEventDisableTiming);
-    else
-      e = hipStreamWaitEvent(st, w->shared_done, 0);
-    if (e != hipSuccess) return hip_fail(e, "product scratch");
-  }
-  e = product_launch(p, m, x_dev, n, out_dev, lease.ptr, st);
-  if (lease.shared) {  // also after a launch that failed: an earlier one of the call may run
-    const hipError_t r = hipEventRecord(w->shared_done, st);
-    if (e == hipSuccess) e = r;
-  }
-  return e == hipSuccess ? TINYOAI_OK : hip_fail(e, "product launch");
+  return w->scratch.run(st, p.bytes(),
+                        [&](void *scratch) { return product_launch(p, m, x_dev, n, out_dev, scratch, st); });
+} catch (const std::exception &e) {
+  return fail(TINYOAI_ENOMEM, "product: %s", e.what());
+}
+
+int tinyoai_weight_mul_mxfp4_device(tinyoai_weight *w, const uint8_t *codes_dev, const uint8_t *scales_dev, int32_t n,
+                                    float *out_dev, void *stream) try {
+  if (!w || !codes_dev || !scales_dev || !out_dev || n <= 0) return fail(TINYOAI_EINVAL, "invalid product arguments");
+  if (!w->mx.d.codes) return fail(TINYOAI_EINVAL, "products of MXFP4 rows need an MXFP4 weight, not type %d", w->m.desc.fmt);
+  if (int rc = check_mxfp4_rows(codes_dev, scales_dev)) return rc;
+  if (int rc = check_device(w->device, "weight")) return rc;
+  hipStream_t st = stream ? (hipStream_t)stream : w->stream;
+  MxProduct p = mx_weight_product(w, nullptr, n, out_dev);
+  p.xdtype = FMT_MXFP4;
+  p.x = codes_dev;
+  p.xscales = scales_dev;
+  return w->scratch.run(st, mx_scratch(p), [&](void *scratch) { return launch_mx_product(p, scratch, st); });
 } catch (const std::exception &e) {
   return fail(TINYOAI_ENOMEM, "product: %s", e.what());
 }
@@ -2590,8 +2544,9 @@ extern "C" {
 int tinyoai_weight_mul_device_noalloc(tinyoai_weight *w, const float *x_dev, int32_t n, float *out_dev, void *stream) {
   if (!w || !x_dev || !out_dev || n <= 0) return fail(TINYOAI_EINVAL, "invalid product arguments");
   const Matrix &m = w->m.desc;
-  if ((size_t)n * m.cols > kScratchValues)
-    return fail(TINYOAI_EINVAL, "product of %d x %d activation values exceeds the no-allocation limit of %zu", n, m.cols,
+  const int cols = (int)w->cols();
+  if ((size_t)n * cols > kScratchValues)
+    return fail(TINYOAI_EINVAL, "product of %d x %d activation values exceeds the no-allocation limit of %zu", n, cols,
                 kScratchValues);
   int dev = 0;
   hipError_t e = hipGetDevice(&dev);
@@ -2608,30 +2563,32 @@ int tinyoai_weight_mul_device_noalloc(tinyoai_weight *w, const float *x_dev, int
   hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
   if ((e = hipStreamIsCapturing(st, &cap)) != hipSuccess) return hip_fail(e, "hipStreamIsCapturing");
   const bool order = cap == hipStreamCaptureStatusNone;
-  const Product p = plan_product(m, x_dev, n);
-  if (p.bytes() > sizeof(scratch))
-    return fail(TINYOAI_EINVAL, "product of %d x %d needs more than the no-allocation limit of %zu bytes", n, m.cols,
+  const bool mx = w->mx.d.codes != nullptr;
+  const MxProduct mp = mx ? mx_weight_product(w, x_dev, n, out_dev) : MxProduct{};
+  const Product p = mx ? Product{} : plan_product(m, x_dev, n);
+  if ((mx ? mx_scratch(mp) : p.bytes()) > sizeof(scratch))
+    return fail(TINYOAI_EINVAL, "product of %d x %d needs more than the no-allocation limit of %zu bytes", n, cols,
                 sizeof(scratch));
   if (order && (e = hipStreamWaitEvent(st, d->done, 0)) != hipSuccess) return hip_fail(e, "no-allocation ordering");
-  e = product_launch(p, m, x_dev, n, out_dev, d->ptr, st);
+  e = mx ? launch_mx_product(mp, d->ptr, st) : product_launch(p, m, x_dev, n, out_dev, d->ptr, st);
   if (e == hipSuccess && order) e = hipEventRecord(d->done, st);
   return e == hipSuccess ? TINYOAI_OK : hip_fail(e, "product launch");
 }
 
 int tinyoai_weight_mul(tinyoai_weight *w, const float *x, int32_t n, float *out) {
   if (!w || !x || !out || n <= 0) return fail(TINYOAI_EINVAL, "invalid product arguments");
-  const Matrix &m = w->m.desc;
+  const size_t rows = w->rows(), cols = w->cols();
   float *dx = nullptr, *dout = nullptr;
-  hipError_t e = device_alloc(&dx, (size_t)n * m.cols * 4);
-  if (e == hipSuccess) e = device_alloc(&dout, (size_t)n * m.rows * 4);
+  hipError_t e = device_alloc(&dx, n * cols * 4);
+  if (e == hipSuccess) e = device_alloc(&dout, n * rows * 4);
   if (e != hipSuccess) {
     hipFree(dx);
     return fail(TINYOAI_ENOMEM, "hipMalloc: %s", hipGetErrorString(e));
   }
-  e = hipMemcpyAsync(dx, x, (size_t)n * m.cols * 4, hipMemcpyHostToDevice, w->stream);
+  e = hipMemcpyAsync(dx, x, n * cols * 4, hipMemcpyHostToDevice, w->stream);
   int rc = e == hipSuccess ? tinyoai_weight_mul_device(w, dx, n, dout, w->stream) : hip_fail(e, "product input");
   if (!rc) {
-    e = hipMemcpyAsync(out, dout, (size_t)n * m.rows * 4, hipMemcpyDeviceToHost, w->stream);
+    e = hipMemcpyAsync(out, dout, n * rows * 4, hipMemcpyDeviceToHost, w->stream);
     if (e == hipSuccess) e = hipStreamSynchronize(w->stream);
     if (e != hipSuccess) rc = hip_fail(e, "product output");
   }

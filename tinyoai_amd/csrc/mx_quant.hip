@@ -1,0 +1,200 @@
+// MXFP4 rows: quantisation, the values that the codes stand for, and the
+// placing of GGUF matrices into the tiles of mx.h.
+//
+// Quantisation of a block of 32 values x: with a = max |x|, the scale is 2^e,
+// e = floor(log2 a) - 2 (2 is the exponent of 6, the largest code) within
+// [-127, 127], and each code is x / 2^e rounded to the nearest, halfway cases
+// to the code with a zero fraction bit, at most 6. A block of zeros takes e =
+// -127; a block with an infinity or NaN takes the NaN scale and zero codes.
+//
+// What bounds it: HBM (each value read once, 17 bytes written for 32 of
+// them). Eight values a lane: four lanes hold a block, whose largest
+// magnitude they exchange by two lane moves.
+#include "mx.h"
+
+namespace {
+
+constexpr int kT = 256;
+
+// Eight values of a row from column c on (c + 8 <= cols).
+template <int D, bool VEC>
+__device__ __forceinline__ void load8(const void *x, int64_t i, float (&v)[8]) {
+  if constexpr (D == FMT_F32) {
+    const float *p = static_cast<const float *>(x) + i;
+    if constexpr (VEC) {
+      const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
+      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; j++) v[j] = p[j];
+    }
+  } else {
+    const uint16_t *p = static_cast<const uint16_t *>(x) + i;
+    uint16_t h[8];
+    if constexpr (VEC) {
+      *reinterpret_cast<uint4 *>(h) = *reinterpret_cast<const uint4 *>(p);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; j++) h[j] = p[j];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++) v[j] = D == FMT_F16 ? hw_half(h[j]) : bf16_to_float(h[j]);
+  }
+}
+
+// One item: eight values of a row of `units` * 128 columns (zeros past cols).
+template <int D, bool VEC>
+__global__ __launch_bounds__(kT) void quantize_kernel(const void *x, int64_t ldx, int64_t n, int64_t cols, int64_t units,
+                                                      uint32_t *codes, uint32_t *scales) {
+  const int64_t per = units * 16, total = n * per;  // a multiple of 16: the 16 lanes of a scale word stay together
+  for (int64_t i = blockIdx.x * (int64_t)kT + threadIdx.x; i < total; i += (int64_t)gridDim.x * kT) {
+    const int64_t row = i / per, c = (i - row * per) * 8;
+    float v[8] = {};
+    if (c < cols) load8<D, VEC>(x, row * ldx + c, v);
+    uint32_t most = 0;
+#pragma unroll
+    for (int j = 0; j < 8; j++) most = max(most, __float_as_uint(v[j]) & 0x7fffffffu);
+    most = max(most, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)most, 0xb1, 0xf, 0xf, false));  // lanes 1, 0, 3, 2
+    most = max(most, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)most, 0x4e, 0xf, 0xf, false));  // lanes 2, 3, 0, 1
+    const bool bad = most >= 0x7f800000u;
+    // the scale byte: the largest's exponent field less 2, 0 (2^-127) at least
+    const uint32_t s = bad ? 255u : max((int)(most >> 23) - 2, 0);
+    const float inv = __uint_as_float((254u - s) << 23);  // 2^(127 - s): s <= 252 (bad ones are not used)
+    uint32_t word = 0;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const float a = fabsf(v[j]) * inv;
+      const uint32_t sign = __float_as_uint(v[j]) >> 31;
+      // the halfway points: the even code takes them
+      const uint32_t m = (a > 0.25f) + (a >= 0.75f) + (a > 1.25f) + (a >= 1.75f) + (a > 2.5f) + (a >= 3.5f) + (a > 5.f);
+      word |= (bad ? 0u : m | sign << 3) << (4 * j);
+    }
+    codes[i] = word;
+    // lane 0 of 16 writes the word of four blocks' scales
+    const uint32_t s1 = __shfl(s, (threadIdx.x & 48) + 4), s2 = __shfl(s, (threadIdx.x & 48) + 8),
+                   s3 = __shfl(s, (threadIdx.x & 48) + 12);
+    if ((threadIdx.x & 15) == 0) scales[i >> 4] = s | s1 << 8 | s2 << 16 | s3 << 24;
+  }
+}
+
+template <int D, bool VEC>
+__global__ __launch_bounds__(kT) void dequantize_kernel(const uint32_t *codes, const uint8_t *scales, int64_t n,
+                                                        int64_t cols, int64_t units, void *out, int64_t ldo) {
+  const int64_t per = cols / 8, total = n * per;
+  for (int64_t i = blockIdx.x * (int64_t)kT + threadIdx.x; i < total; i += (int64_t)gridDim.x * kT) {
+    const int64_t row = i / per, c = i - row * per;
+    const uint32_t word = codes[row * units * 16 + c];
+    const float s = mx_scale(scales[row * units * 4 + c / 4]);
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) v[j] = mx_code((word >> (4 * j)) & 15) * s;
+    const int64_t o = row * ldo + c * 8;
+    if constexpr (D == FMT_F32) {
+      float *p = static_cast<float *>(out) + o;
+      if constexpr (VEC) {
+        reinterpret_cast<float4 *>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+        reinterpret_cast<float4 *>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++) p[j] = v[j];
+      }
+    } else {
+      uint16_t *p = static_cast<uint16_t *>(out) + o;
+      uint16_t h[8];
+#pragma unroll
+      for (int j = 0; j < 8; j++) h[j] = mx_narrow(D, v[j]);
+      if constexpr (VEC) {
+        *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<const uint4 *>(h);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++) p[j] = h[j];
+      }
+    }
+  }
+}
+
+// GGUF rows -> tiles. MXFP4 blocks are {scale, 16 bytes}, byte j the codes of
+// values j (low) and j + 16; BF16 rows are plain values.
+__global__ __launch_bounds__(kT) void place_mxfp4_kernel(MxMat m, uint8_t *codes, uint8_t *scales, const uint8_t *raw,
+                                                         int phase) {
+  const int64_t nb = m.cols / 32, total = m.rows * nb;
+  for (int64_t i = blockIdx.x * (int64_t)kT + threadIdx.x; i < total; i += (int64_t)gridDim.x * kT) {
+    const int row = mx_stored_row(m, (int)(i / nb), phase), col = (int)(i % nb) * 32;
+    const uint8_t *src = raw + i * 17;
+    uint8_t *dst = codes + mx_code_at(m, row, col);
+    for (int j = 0; j < 8; j++) {
+      const uint32_t a = src[1 + 2 * j], b = src[2 + 2 * j];
+      dst[j] = (uint8_t)((a & 15) | (b & 15) << 4);
+      dst[j + 8] = (uint8_t)((a >> 4) | (b >> 4) << 4);
+    }
+    scales[mx_scale_at(m, row, col)] = src[0];
+  }
+}
+__global__ __launch_bounds__(kT) void place_bf16_kernel(MxMat m, uint8_t *codes, const uint16_t *raw, int phase) {
+  const int64_t total = (int64_t)m.rows * m.cols;
+  for (int64_t i = blockIdx.x * (int64_t)kT + threadIdx.x; i < total; i += (int64_t)gridDim.x * kT) {
+    const int row = mx_stored_row(m, (int)(i / m.cols), phase), col = (int)(i % m.cols);
+    *reinterpret_cast<uint16_t *>(codes + mx_code_at(m, row, col)) = raw[i];
+  }
+}
+
+__global__ __launch_bounds__(kT) void read_kernel(MxMat m, int64_t offset, int64_t n, float *out) {
+  for (int64_t i = blockIdx.x * (int64_t)kT + threadIdx.x; i < n; i += (int64_t)gridDim.x * kT) {
+    const int64_t e = offset + i;
+    out[i] = mx_value(m, 0, (int)(e / m.cols), (int)(e % m.cols));
+  }
+}
+
+int blocks_for(int64_t items) { return (int)std::max<int64_t>(1, std::min<int64_t>((items + kT - 1) / kT, 16384)); }
+bool aligned16(const void *p, int64_t ld, size_t width) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * (int64_t)width % 16 == 0;
+}
+
+}  // namespace
+
+hipError_t launch_mx_quantize(int dtype, const void *x, int64_t ldx, int64_t n, int64_t cols, uint8_t *codes,
+                              uint8_t *scales, hipStream_t st) {
+  const int64_t units = (cols + 127) / 128;
+  const dim3 grid(blocks_for(n * units * 16));
+  const bool vec = aligned16(x, ldx, mx_width(dtype));
+  auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, grid, dim3(kT), 0, st, x, ldx, n, cols, units, reinterpret_cast<uint32_t *>(codes),
+                       reinterpret_cast<uint32_t *>(scales));
+  };
+  if (dtype == FMT_F32) vec ? go(quantize_kernel<FMT_F32, true>) : go(quantize_kernel<FMT_F32, false>);
+  else if (dtype == FMT_F16) vec ? go(quantize_kernel<FMT_F16, true>) : go(quantize_kernel<FMT_F16, false>);
+  else vec ? go(quantize_kernel<FMT_BF16, true>) : go(quantize_kernel<FMT_BF16, false>);
+  return hipGetLastError();
+}
+
+hipError_t launch_mx_dequantize(const uint8_t *codes, const uint8_t *scales, int64_t n, int64_t cols, int dtype, void *out,
+                                int64_t ldo, hipStream_t st) {
+  const int64_t units = (cols + 127) / 128;
+  const dim3 grid(blocks_for(n * cols / 8));
+  const bool vec = aligned16(out, ldo, mx_width(dtype));
+  auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, grid, dim3(kT), 0, st, reinterpret_cast<const uint32_t *>(codes), scales, n, cols, units,
+                       out, ldo);
+  };
+  if (dtype == FMT_F32) vec ? go(dequantize_kernel<FMT_F32, true>) : go(dequantize_kernel<FMT_F32, false>);
+  else if (dtype == FMT_F16) vec ? go(dequantize_kernel<FMT_F16, true>) : go(dequantize_kernel<FMT_F16, false>);
+  else vec ? go(dequantize_kernel<FMT_BF16, true>) : go(dequantize_kernel<FMT_BF16, false>);
+  return hipGetLastError();
+}
+
+hipError_t launch_mx_place(const MxMat &m, const uint8_t *raw, int expert, int phase, hipStream_t st) {
+  uint8_t *codes = const_cast<uint8_t *>(m.codes) + expert * mx_code_bytes(m);
+  uint8_t *scales = const_cast<uint8_t *>(m.scales) + expert * mx_scale_bytes(m);
+  if (m.fmt == FMT_MXFP4)
+    hipLaunchKernelGGL(place_mxfp4_kernel, dim3(blocks_for((int64_t)m.rows * m.cols / 32)), dim3(kT), 0, st, m, codes,
+                       scales, raw, phase);
+  else
+    hipLaunchKernelGGL(place_bf16_kernel, dim3(blocks_for((int64_t)m.rows * m.cols)), dim3(kT), 0, st, m, codes,
+                       reinterpret_cast<const uint16_t *>(raw), phase);
+  return hipGetLastError();
+}
+
+hipError_t launch_mx_read(const MxMat &m, int64_t offset, int64_t n, float *out, hipStream_t st) {
+  hipLaunchKernelGGL(read_kernel, dim3(blocks_for(n)), dim3(kT), 0, st, m, offset, n, out);
+  return hipGetLastError();
+}

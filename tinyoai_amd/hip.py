@@ -29,6 +29,9 @@ EXPORTS = [
     "tinyoai_weight_upload",
     "tinyoai_weight_read_values", "tinyoai_weight_mul", "tinyoai_weight_mul_device",
     "tinyoai_weight_mul_device_noalloc", "tinyoai_weight_free",
+    "tinyoai_mxfp4_quantize_device", "tinyoai_mxfp4_dequantize_device", "tinyoai_weight_mul_mxfp4_device",
+    "tinyoai_route_device", "tinyoai_combine_device", "tinyoai_experts_upload", "tinyoai_experts_mul_device",
+    "tinyoai_experts_free",
 ]
 
 
@@ -101,6 +104,15 @@ def lib():
         L.tinyoai_weight_mul_device.argtypes = [P, P, C.c_int32, P, P]
         L.tinyoai_weight_mul_device_noalloc.argtypes = [P, P, C.c_int32, P, P]
         L.tinyoai_weight_free.argtypes = [P]
+        i32, i64 = C.c_int32, C.c_int64
+        L.tinyoai_mxfp4_quantize_device.argtypes = [i32, P, i64, i64, i64, P, P, P]
+        L.tinyoai_mxfp4_dequantize_device.argtypes = [P, P, i64, i64, i32, P, i64, P]
+        L.tinyoai_weight_mul_mxfp4_device.argtypes = [P, P, P, i32, P, P]
+        L.tinyoai_route_device.argtypes = [i32, P, i64, i32, i32, i32, i32, P, P, P, P, P, P]
+        L.tinyoai_combine_device.argtypes = [i32, P, i64, i32, P, P, i32, i32, i64, i32, P, i64, P]
+        L.tinyoai_experts_upload.argtypes = [i32, i32, i64, i64, P, P, C.c_uint64, C.POINTER(P)]
+        L.tinyoai_experts_mul_device.argtypes = [P, i32, P, P, i64, i32, P, P, i32, i32, P, i64, P]
+        L.tinyoai_experts_free.argtypes = [P]
         _lib = L
     return _lib
 
@@ -137,6 +149,79 @@ def summarize_logits(logits: np.ndarray, targets, count: int):
     return chosen, ids, lp
 
 
+# ---------------------------------------------------------------- mixture-of-experts operators
+# Buffers are device addresses (as Weight.mul_device takes them); `stream` is a
+# hipStream_t, 0 the current device's default stream (a handle's methods: its
+# own stream). Types are the codes of tinyoai_amd.weights.
+def mxfp4_row_bytes(cols: int) -> tuple[int, int]:
+    """(code bytes, scale bytes) of a row of MXFP4 values."""
+    units = -(-cols // 128)
+    return 64 * units, 4 * units
+
+
+def quantize_mxfp4(dtype: int, x_ptr: int, ldx: int, n: int, cols: int, codes_ptr: int, scales_ptr: int,
+                   stream: int = 0) -> None:
+    """n rows of `cols` values, ldx apart, to MXFP4 rows (mxfp4_row_bytes each)."""
+    check(lib().tinyoai_mxfp4_quantize_device(dtype, x_ptr, ldx, n, cols, codes_ptr, scales_ptr, stream or None))
+
+
+def dequantize_mxfp4(codes_ptr: int, scales_ptr: int, n: int, cols: int, dtype: int, out_ptr: int, ldo: int,
+                     stream: int = 0) -> None:
+    """The values of n MXFP4 rows, rows of the output ldo apart."""
+    check(lib().tinyoai_mxfp4_dequantize_device(codes_ptr, scales_ptr, n, cols, dtype, out_ptr, ldo, stream or None))
+
+
+def route(dtype: int, logits_ptr: int, ld: int, n: int, experts: int, k: int, over_all: bool, ids_ptr: int,
+          weights_ptr: int, offsets_ptr: int, tokens_ptr: int, positions_ptr: int, stream: int = 0) -> None:
+    """The k best experts of n tokens: ids and softmax weights [n][k] (over
+    the chosen logits, or over all), and the choices sorted by expert: offsets
+    [experts + 1], the rows' tokens [n * k], the choices' rows [n][k]."""
+    check(lib().tinyoai_route_device(dtype, logits_ptr, ld, n, experts, k, int(over_all), ids_ptr, weights_ptr,
+                                     offsets_ptr, tokens_ptr, positions_ptr, stream or None))
+
+
+def combine(dtype: int, y_ptr: int, ldy: int, y_rows: int, positions_ptr: int, weights_ptr: int, n: int, k: int, cols: int,
+            out_dtype: int, out_ptr: int, ldo: int, stream: int = 0) -> None:
+    """out[t] = sum of weights[t][j] * y[positions[t][j]] over j < k."""
+    check(lib().tinyoai_combine_device(dtype, y_ptr, ldy, y_rows, positions_ptr, weights_ptr, n, k, cols, out_dtype,
+                                       out_ptr, ldo, stream or None))
+
+
+class Experts:
+    """Matrices [rows][cols] of `experts` experts (MXFP4 or BF16, raw bytes
+    one after another); with `up`, (gate, up) pairs whose products are
+    silu(gate) * up."""
+
+    def __init__(self, dtype: int, experts: int, rows: int, cols: int, data: np.ndarray, up: np.ndarray | None = None):
+        self.dtype, self.experts, self.rows, self.cols = dtype, experts, rows, cols
+        self.h = None
+        a = [np.ascontiguousarray(d).view(np.uint8).reshape(-1) for d in (data, up) if d is not None]
+        if len(a) == 2 and a[0].size != a[1].size:
+            raise TinyoaiError(f"gate and up matrices of {a[0].size} and {a[1].size} bytes")
+        h = C.c_void_p()
+        check(lib().tinyoai_experts_upload(dtype, experts, rows, cols, a[0].ctypes.data,
+                                           a[1].ctypes.data if len(a) == 2 else None, a[0].size, C.byref(h)))
+        self.h = h
+
+    def mul_device(self, x_dtype: int, x_ptr: int, x_scales_ptr: int, ldx: int, x_rows: int, offsets_ptr: int,
+                   index_ptr: int, n: int, out_dtype: int, out_ptr: int, ldo: int, stream: int = 0) -> None:
+        """out[r] = x[index[r]] * W_e^T for the rows r of each expert e (offsets,
+        index: as route lists them; index 0: x[r]), n rows in all."""
+        check(lib().tinyoai_experts_mul_device(self.h, x_dtype, x_ptr, x_scales_ptr or None, ldx, x_rows, offsets_ptr,
+                                               index_ptr or None, n, out_dtype, out_ptr, ldo, stream or None))
+
+    def close(self):
+        if self.h:
+            lib().tinyoai_experts_free(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
 class Weight:
     """One weight matrix in HBM (weightTensor, safetensors.go:193-280)."""
 
@@ -160,6 +245,10 @@ class Weight:
 
     def mul_device(self, x_ptr: int, n: int, out_ptr: int, stream: int = 0) -> None:
         check(lib().tinyoai_weight_mul_device(self.h, x_ptr, n, out_ptr, stream or None))
+
+    def mul_mxfp4_device(self, codes_ptr: int, scales_ptr: int, n: int, out_ptr: int, stream: int = 0) -> None:
+        """The product of n MXFP4 rows (quantize_mxfp4) with an MXFP4 weight."""
+        check(lib().tinyoai_weight_mul_mxfp4_device(self.h, codes_ptr, scales_ptr, n, out_ptr, stream or None))
 
     def mul_device_noalloc(self, x_ptr: int, n: int, out_ptr: int, stream: int = 0) -> None:
         """mul_device without any allocation (operand planes in the

@@ -17,12 +17,13 @@ import numpy as np
 
 # GGUF tensor type codes (gguf.go:183-214); Q4_K (12) is the public GGML code.
 F32, F16, Q5_1, Q8_0, Q4_K, Q5_K, Q6_K, BF16 = 0, 1, 7, 8, 12, 13, 14, 30
+MXFP4 = 39  # single weights and experts only: microscaled 4-bit floating point
 DTYPE_NAMES = {F32: "F32", F16: "F16", Q5_1: "Q5_1", Q8_0: "Q8_0", Q4_K: "Q4_K",
-               Q5_K: "Q5_K", Q6_K: "Q6_K", BF16: "BF16"}
+               Q5_K: "Q5_K", Q6_K: "Q6_K", BF16: "BF16", MXFP4: "MXFP4"}
 NAME_DTYPES = {v: k for k, v in DTYPE_NAMES.items()}
 # (values per block, bytes per block)
 BLOCKS = {F32: (1, 4), F16: (1, 2), BF16: (1, 2), Q8_0: (32, 34), Q5_1: (32, 24),
-          Q4_K: (256, 144), Q5_K: (256, 176), Q6_K: (256, 210)}
+          Q4_K: (256, 144), Q5_K: (256, 176), Q6_K: (256, 210), MXFP4: (32, 17)}
 
 
 def nbytes(dtype: int, rows: int, cols: int) -> int:
@@ -135,6 +136,17 @@ def encode_q8_0(scales: np.ndarray, qs: np.ndarray) -> np.ndarray:
     out = np.empty((nb, 34), np.uint8)
     out[:, :2] = np.asarray(scales, np.uint16).reshape(nb, 1).view(np.uint8)
     out[:, 2:] = np.asarray(qs, np.int8).reshape(nb, 32).view(np.uint8)
+    return out.reshape(-1)
+
+
+def encode_mxfp4(codes: np.ndarray, scales: np.ndarray) -> np.ndarray:
+    """MXFP4 blocks {scale, 16 bytes} of codes [rows, cols] (0..15, one a
+    byte) and scale bytes [rows, cols / 32]: byte j of a block holds the codes
+    of values j (low half) and j + 16."""
+    q = np.asarray(codes, np.uint8).reshape(-1, 32)
+    out = np.empty((q.shape[0], 17), np.uint8)
+    out[:, 0] = np.asarray(scales, np.uint8).reshape(-1)
+    out[:, 1:] = q[:, :16] | q[:, 16:] << 4
     return out.reshape(-1)
 
 
