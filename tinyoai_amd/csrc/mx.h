@@ -89,7 +89,7 @@ __device__ __forceinline__ void mx_store(int dtype, void *p, int64_t i, float v)
 // g / (1 + e^-g) * u in fp32 (stablelm.go:371-373).
 __device__ __forceinline__ float mx_gate(float g, float u) { return g / (1.f + expf(-g)) * u; }
 
-inline size_t mx_width(int dtype) { return dtype == FMT_F32 ? 4 : 2; }
+__host__ __device__ inline size_t mx_width(int dtype) { return dtype == FMT_F32 ? 4 : 2; }
 
 // out[r] = x[index ? index[r] : r] * W[e]^T for the rows r of [offsets[e],
 // offsets[e + 1]) (clamped to [0, n)), for every expert e; offsets null: all
@@ -121,6 +121,9 @@ hipError_t launch_mx_dequantize(const uint8_t *codes, const uint8_t *scales, int
 // The product, with mx_scratch bytes of scratch.
 size_t mx_scratch(const MxProduct &p);
 hipError_t launch_mx_product(const MxProduct &p, void *scratch, hipStream_t st);
+// A few rows (or a few for each expert) on the streaming kernel.
+bool mx_few_supported(const MxProduct &p);
+hipError_t launch_mx_few(const MxProduct &p, hipStream_t st);
 
 struct RouteArgs {
   int32_t dtype;

@@ -73,6 +73,7 @@ __global__ __launch_bounds__(kT) void product_kernel(MxProduct p) {
 size_t mx_scratch(const MxProduct &p) { return 0; }
 
 hipError_t launch_mx_product(const MxProduct &p, void *scratch, hipStream_t st) {
+  if (mx_few_supported(p)) return launch_mx_few(p, st);
   const int tiles = (p.n + kRows - 1) / kRows + (p.offsets ? p.w.experts : 0);
   hipLaunchKernelGGL(product_kernel, dim3(tiles, (p.w.rows + kOut - 1) / kOut), dim3(kT), 0, st, p);
   return hipGetLastError();

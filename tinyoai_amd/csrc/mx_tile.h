@@ -1,0 +1,169 @@
+// Device parts that the matrix-core products of mx.h share: operands, the
+// planes of X and their places in LDS.
+#pragma once
+
+#include <type_traits>
+
+#include "mx.h"
+
+// bf16 planes that hold a type's values exactly (MXFP4: none).
+__host__ __device__ inline int mx_planes(int dtype) { return dtype == FMT_F32 ? 3 : dtype == FMT_F16 ? 2 : 1; }
+
+namespace tinyoai_mx {
+
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+template <int WF>
+constexpr int mx_cols() { return WF == FMT_MXFP4 ? 128 : 64; }
+
+__device__ __forceinline__ f32x4 mfma_bf16(uint4 a, uint4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+// MXFP4 times MXFP4: a's scale is byte A of sa, b's byte 0 of sb.
+template <int A>
+__device__ __forceinline__ f32x4 mfma_mx(uint4 a, uint4 b, f32x4 c, uint32_t sa, uint32_t sb) {
+  const i32x8 x = {(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0}, y = {(int)b.x, (int)b.y, (int)b.z, (int)b.w, 0, 0, 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 4, 4, A, (int)sa, 0, (int)sb);
+}
+// Eight codes times 2^(exponent of s - 127) as bf16, exact within bf16's range.
+__device__ __forceinline__ uint4 fp4_bf16(uint32_t c, float s) {
+  auto two = [](bf16x2 v) { return __builtin_bit_cast(uint32_t, v); };
+  return make_uint4(two(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 0)), two(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 1)),
+                    two(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 2)), two(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 3)));
+}
+
+// A value's planes as fp32 bit patterns whose low halves are zero: what is
+// left after a plane has eight bits fewer, and the difference is exact. An
+// infinity or NaN is all in the first plane.
+template <int P>
+__device__ __forceinline__ void planes_of(float v, uint32_t (&h)[P]) {
+  uint32_t u = __float_as_uint(v);
+  if constexpr (P == 1) {
+    h[0] = u;  // a bf16 value
+  } else {
+    const uint32_t mag = u & 0x7fffffffu;
+    if (mag > 0x7f800000u) u |= 0x00400000u;  // the half kept must not read as an infinity
+    h[0] = u & 0xffff0000u;
+    const bool finite = mag < 0x7f800000u;
+    float rest = finite ? v - __uint_as_float(h[0]) : 0.f;
+#pragma unroll
+    for (int i = 1; i < P; i++) {
+      h[i] = __float_as_uint(rest) & 0xffff0000u;
+      rest -= __uint_as_float(h[i]);
+    }
+  }
+}
+__device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) {  // a's below b's
+  return __builtin_amdgcn_perm(b, a, 0x07060302u);
+}
+
+// Raw bits of eight values of row `src` from column k on; zeros past `cols`.
+// XT: the type.
+template <int XT>
+struct Raw8 {
+  uint4 a[XT == FMT_F32 ? 2 : 1];
+};
+template <int XT>
+__device__ __forceinline__ Raw8<XT> load_x8(const MxProduct &p, int64_t src, int k) {
+  using V = std::conditional_t<XT == FMT_F32, uint32_t, uint16_t>;
+  const V *s = static_cast<const V *>(p.x) + src * p.ldx + k;
+  Raw8<XT> r;
+  if (k + 8 <= p.w.cols && (reinterpret_cast<uintptr_t>(s) & 15) == 0) {
+    r.a[0] = reinterpret_cast<const uint4 *>(s)[0];
+    if constexpr (XT == FMT_F32) r.a[1] = reinterpret_cast<const uint4 *>(s)[1];
+  } else {
+    V v[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) v[j] = k + j < p.w.cols ? s[j] : V(0);
+    memcpy(&r, v, sizeof r);
+  }
+  return r;
+}
+// Their planes, each as eight bf16 values.
+template <int XT>
+__device__ __forceinline__ void planes8(const Raw8<XT> &r, uint4 (&out)[XT == FMT_F32 ? 3 : XT == FMT_F16 ? 2 : 1]) {
+  if constexpr (XT == FMT_BF16) {
+    out[0] = r.a[0];
+  } else {
+    constexpr int P = XT == FMT_F32 ? 3 : 2;
+    uint32_t w[XT == FMT_F32 ? 8 : 4], h[8][P];
+    memcpy(w, &r, sizeof w);
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+      planes_of<P>(XT == FMT_F32 ? __uint_as_float(w[j]) : hw_half((uint16_t)(w[j / 2] >> (16 * (j & 1)))), h[j]);
+#pragma unroll
+    for (int pl = 0; pl < P; pl++)
+      out[pl] = make_uint4(high_halves(h[0][pl], h[1][pl]), high_halves(h[2][pl], h[3][pl]), high_halves(h[4][pl], h[5][pl]),
+                           high_halves(h[6][pl], h[7][pl]));
+  }
+}
+
+// The few-row kernel's X in LDS: for each column chunk and virtual column v,
+// the chunk's values in 16-byte pieces, piece c at a place that depends on v,
+// so that the 16 columns' reads of one piece hit distinct banks.
+template <int WF>
+__device__ __forceinline__ int few_x_at(int v, int c) {
+  return WF == FMT_MXFP4 ? v * 256 + ((c ^ (v & 15)) << 4) : v * 128 + ((c ^ ((v >> 1) & 7)) << 4);
+}
+template <int WF, int XM>
+__host__ __device__ inline size_t few_x_bytes(int chunks, int V) {
+  return ((size_t)chunks * V * (XM == 0 ? 68 : mx_cols<WF>() * 2) + 15) / 16 * 16;
+}
+
+// X's columns [k0, k0 + count) of rows r0 .. r0 + m - 1 into LDS: virtual
+// column plane * m + row. MXFP4 rows: per chunk and row 64 code bytes, then
+// all the scale words (`seg` chunks at most). `between` is called once, after
+// the first loads are issued: what it loads is not waited for here.
+template <int WF, int XM, int T, typename Between>
+__device__ __forceinline__ void stage_few(const MxProduct &p, uint8_t *lds, int r0, int m, int V, int k0, int count, int seg,
+                                          int tid, const Between &between) {
+  constexpr int XT = XM == 3 ? FMT_F32 : XM == 2 ? FMT_F16 : FMT_BF16, B = 4;  // items a thread loads together
+  const int pieces = XM == 0 ? count / 32 : count / 8;  // 16-byte pieces of a row
+  const int items = m * pieces;
+  for (int i0 = 0; i0 < items; i0 += B * T) {
+    Raw8<XT> raw[B];
+    uint32_t sc[B];
+    int64_t src[B];
+#pragma unroll
+    for (int b = 0; b < B; b++) {
+      const int i = i0 + b * T + tid, r = r0 + min(i / pieces, m - 1);
+      src[b] = p.index ? p.index[r] : r;
+    }
+#pragma unroll
+    for (int b = 0; b < B; b++) {
+      const int i = i0 + b * T + tid, c = i % pieces;
+      memset(&raw[b], 0, sizeof raw[b]);
+      sc[b] = 0;
+      if (i >= items || src[b] < 0 || src[b] >= p.x_rows) continue;
+      if constexpr (XM == 0) {
+        const int64_t at = src[b] * p.w.chunks + k0 / 128 + c / 4;
+        raw[b].a[0] = *reinterpret_cast<const uint4 *>(static_cast<const uint8_t *>(p.x) + at * 64 + (c & 3) * 16);
+        if ((c & 3) == 0) sc[b] = reinterpret_cast<const uint32_t *>(p.xscales)[at];
+      } else {
+        raw[b] = load_x8<XT>(p, src[b], k0 + c * 8);
+      }
+    }
+    if (i0 == 0) between();
+#pragma unroll
+    for (int b = 0; b < B; b++) {
+      const int i = i0 + b * T + tid, r = i / pieces, c = i - r * pieces;
+      if (i >= items) break;
+      if constexpr (XM == 0) {
+        *reinterpret_cast<uint4 *>(lds + ((size_t)(c >> 2) * V + r) * 64 + (((c & 3) ^ ((r >> 2) & 3)) << 4)) = raw[b].a[0];
+        if ((c & 3) == 0) reinterpret_cast<uint32_t *>(lds + (size_t)seg * V * 64)[(c >> 2) * V + r] = sc[b];
+      } else {
+        uint4 h[XM];
+        planes8<XT>(raw[b], h);
+        constexpr int per = mx_cols<WF>() / 8;
+        uint8_t *base = lds + (size_t)(c / per) * V * (mx_cols<WF>() * 2);
+#pragma unroll
+        for (int pl = 0; pl < XM; pl++) *reinterpret_cast<uint4 *>(base + few_x_at<WF>(pl * m + r, c % per)) = h[pl];
+      }
+    }
+  }
+}
+
+}  // namespace tinyoai_mx
