@@ -376,9 +376,10 @@ int tinyoai_experts_upload(int32_t dtype, int32_t experts, int64_t rows, int64_t
  * tinyoai_route_device lists them; index NULL: x[r]. Other rows of out stay as
  * they are. x: F32, F16 or BF16 [x_rows][ldx], or MXFP4 rows (x_scales_dev their
  * scales, ldx = cols; MXFP4 experts). Sums are fp32: F32 and F16 rows count
- * with all their bits. An index outside [0, x_rows) gives a row of zeros;
- * offsets outside [0, n] or falling count as the nearest that are not. The
- * current device must be the handle's. */
+ * with all their bits. An index outside [0, x_rows) gives a row of zeros.
+ * Offsets that leave [0, n] count as the nearest that do not; they must not
+ * fall (rows of such groups may be left out; nothing outside `out` is touched).
+ * The current device must be the handle's. */
 int tinyoai_experts_mul_device(tinyoai_experts *e, int32_t x_dtype, const void *x_dev, const uint8_t *x_scales_dev,
                                int64_t ldx, int32_t x_rows, const int32_t *offsets_dev, const int32_t *index_dev,
                                int32_t n, int32_t out_dtype, void *out_dev, int64_t ldo, void *stream);

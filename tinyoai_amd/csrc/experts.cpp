@@ -10,6 +10,15 @@
 #include "stream_scratch.h"
 #include "tinyoai_hip.h"
 
+// ---------------------------------------------------------------- products
+static bool on_tiles(const MxProduct &p) { return !mx_few_supported(p) && mx_tiles_supported(p); }
+
+size_t mx_scratch(const MxProduct &p) { return on_tiles(p) ? mx_tiles_scratch(p) : 0; }
+
+hipError_t launch_mx_product(const MxProduct &p, void *scratch, hipStream_t st) {
+  return on_tiles(p) ? launch_mx_tiles(p, scratch, st) : launch_mx_few(p, st);
+}
+
 namespace tinyoai {
 
 // ---------------------------------------------------------------- scratch

@@ -124,6 +124,10 @@ hipError_t launch_mx_product(const MxProduct &p, void *scratch, hipStream_t st);
 // A few rows (or a few for each expert) on the streaming kernel.
 bool mx_few_supported(const MxProduct &p);
 hipError_t launch_mx_few(const MxProduct &p, hipStream_t st);
+// Many rows on LDS tiles.
+bool mx_tiles_supported(const MxProduct &p);
+size_t mx_tiles_scratch(const MxProduct &p);
+hipError_t launch_mx_tiles(const MxProduct &p, void *scratch, hipStream_t st);
 
 struct RouteArgs {
   int32_t dtype;
