@@ -7,11 +7,16 @@
 //
 // Matrices are stored in the order in which the matrix cores take them, so a
 // wave's loads are contiguous and need no address arithmetic per lane. Rows
-// are cut into tiles of 16, columns into chunks; one tile's chunk is
+// are cut into tiles of 16, columns into chunks. Sixteen tiles form a group (the
+// last one may have fewer, a multiple of four), and a group holds its tiles'
+// first chunk, then their second, and so on: what a block of many rows loads
+// for a step is contiguous (a tile's chunks one after another put a step's 16
+// loads on the same few memory channels). One tile's chunk is
 //   MXFP4: 128 columns, 1 KB: lane l's 16 bytes are the codes of row l % 16,
 //          columns 32 (l / 16) .. + 31, two a byte, the earlier one low. The
-//          scales of four tiles' chunk are 256 bytes: lane l's word holds
-//          tile t's scale of row l % 16 and block l / 16 in byte t;
+//          scales of four tiles' chunk, in an array of their own and in the
+//          same order, are 256 bytes: lane l's word holds tile t's scale of
+//          row l % 16 and block l / 16 in byte t;
 //   BF16:  64 columns, 2 KB: lane l's 16 bytes of half j are the values of
 //          row l % 16, columns 16 (l / 16) + 8 j .. + 7.
 // Rows and columns past the matrix hold zeros. Of a (gate, up) pair, the gate
@@ -43,16 +48,26 @@ __host__ __device__ inline int64_t mx_code_bytes(const MxMat &m) {  // of one ex
 __host__ __device__ inline int64_t mx_scale_bytes(const MxMat &m) {
   return m.fmt == FMT_MXFP4 ? (int64_t)m.tiles / 4 * m.chunks * 256 : 0;
 }
+// Where a tile's chunk begins, and its scale quad's (bytes within an expert).
+__host__ __device__ inline int mx_group_tiles(const MxMat &m, int tile) {
+  const int left = m.tiles - (tile & ~15);
+  return left < 16 ? left : 16;
+}
+__host__ __device__ inline int64_t mx_tile_at(const MxMat &m, int tile, int chunk) {
+  return ((int64_t)(tile >> 4) * 16 * m.chunks + (int64_t)chunk * mx_group_tiles(m, tile) + (tile & 15)) * mx_chunk_bytes(m.fmt);
+}
+__host__ __device__ inline int64_t mx_quad_at(const MxMat &m, int tile, int chunk) {
+  return ((int64_t)(tile >> 4) * 4 * m.chunks + (int64_t)chunk * (mx_group_tiles(m, tile) / 4) + ((tile & 15) >> 2)) * 256;
+}
 // The byte of value (row of the stored tiles, column) within an expert.
 __host__ __device__ inline int64_t mx_code_at(const MxMat &m, int row, int col) {
   const int cc = mx_chunk_cols(m.fmt), k = col % cc;
-  const int64_t at = ((int64_t)(row >> 4) * m.chunks + col / cc) * mx_chunk_bytes(m.fmt);
+  const int64_t at = mx_tile_at(m, row >> 4, col / cc);
   if (m.fmt == FMT_MXFP4) return at + ((k >> 5) * 16 + (row & 15)) * 16 + (k & 31) / 2;
   return at + ((k >> 3) & 1) * 1024 + ((k >> 4) * 16 + (row & 15)) * 16 + (k & 7) * 2;
 }
 __host__ __device__ inline int64_t mx_scale_at(const MxMat &m, int row, int col) {
-  const int tile = row >> 4;
-  return ((int64_t)(tile >> 2) * m.chunks + col / 128) * 256 + (((col & 127) >> 5) * 16 + (row & 15)) * 4 + (tile & 3);
+  return mx_quad_at(m, row >> 4, col / 128) + (((col & 127) >> 5) * 16 + (row & 15)) * 4 + ((row >> 4) & 3);
 }
 // The stored row of output row `row` (phase 1: its up row).
 __host__ __device__ inline int mx_stored_row(const MxMat &m, int row, int phase) {

@@ -83,11 +83,11 @@ __global__ __launch_bounds__(kT) void few_kernel(FewArgs g) {
     int fleft = max((fhi - fi + kAhead - 1) / kAhead * kAhead, kAhead);
     auto fetch = [&](Fetch<WF, NT> &f) {
       const bool real = fu < u_end && fi < fhi;
-      const int64_t tile = (int64_t)(real ? fu : 0) * NT, c = real ? fs * g.seg + fi : 0;
+      const int tile = (real ? fu : 0) * NT, c = real ? fs * g.seg + fi : 0;
 #pragma unroll
       for (int t = 0; t < NT; t++) {
         const __amdgpu_buffer_rsrc_t r =
-            plane_rsrc(codes + ((tile + t) * chunks + c) * mx_chunk_bytes(WF), real ? mx_chunk_bytes(WF) : 0);
+            plane_rsrc(codes + mx_tile_at(p.w, tile + t, c), real ? mx_chunk_bytes(WF) : 0);
 #pragma unroll
         for (int j = 0; j < (WF == FMT_BF16 ? 2 : 1); j++) {
           const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(r, lane * 16 + j * 1024, 0, 0);
@@ -95,7 +95,7 @@ __global__ __launch_bounds__(kT) void few_kernel(FewArgs g) {
         }
       }
       if constexpr (WF == FMT_MXFP4)
-        f.s = __builtin_amdgcn_raw_buffer_load_b32(plane_rsrc(scales + ((tile >> 2) * chunks + c) * 256, real ? 256 : 0),
+        f.s = __builtin_amdgcn_raw_buffer_load_b32(plane_rsrc(scales + mx_quad_at(p.w, tile, c), real ? 256 : 0),
                                                    lane * 4, 0, 0);
       fi++;
       if (--fleft == 0) {

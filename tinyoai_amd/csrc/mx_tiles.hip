@@ -19,7 +19,8 @@
 //
 // Groups: the row tiles of all groups are numbered in a row; a wave finds its
 // tile's group from the offsets, 64 experts at a time by lane moves. Tiles go
-// to the XCDs in runs, those of one group and the same matrix rows together.
+// to the XCDs in runs of bands, kBand row tiles by all matrix tiles, so that
+// the blocks that run together on an XCD share both operands through its L2.
 #include <algorithm>
 
 #include "mx_tile.h"
@@ -28,7 +29,7 @@ namespace {
 
 using namespace tinyoai_mx;
 
-constexpr int kT = 256;
+constexpr int kT = 256, kBand = 8;
 constexpr uint32_t kNone = 0x80000000u, kPast = 0x40000000u;
 
 struct TileArgs {
@@ -59,12 +60,14 @@ struct Shape {
 // in the whole grid, whose size only the offsets give.
 template <int BM>
 __device__ __forceinline__ bool find_tile(const MxProduct &p, int lane, int ntiles, int block, int &e, int &r0, int &r1, int &nt) {
-  auto place = [&](int mtiles, int &mt) {  // runs of tiles for each XCD; row tiles of one matrix tile next to each other
+  auto place = [&](int mtiles, int &mt) {
     const int64_t total = (int64_t)mtiles * ntiles, per = (total + 7) / 8;
     const int64_t t = (block & 7) * per + (block >> 3);
     if ((block >> 3) >= per || t >= total) return false;
-    nt = (int)(t / mtiles);
-    mt = (int)(t - (int64_t)nt * mtiles);
+    const int64_t band = (int64_t)kBand * ntiles, b = t / band;
+    const int wide = min(kBand, mtiles - (int)b * kBand), in = (int)(t - b * band);
+    nt = in / wide;
+    mt = (int)b * kBand + in - nt * wide;
     return true;
   };
   int mt;
@@ -110,7 +113,7 @@ __device__ __forceinline__ bool find_tile(const MxProduct &p, int lane, int ntil
 }
 
 template <int WF, int XM, int BM, int BN, int WM, int STAGES>
-__global__ __launch_bounds__(kT) void tile_kernel(TileArgs g) {
+__global__ __launch_bounds__(kT, 2) void tile_kernel(TileArgs g) {
   using S = Shape<WF, XM, BM, BN>;
   constexpr bool Q = S::Q;
   constexpr int P = S::P, WN = 4 / WM, MF = BM / 16 / WM, NF = BN / 16 / WN;
@@ -142,11 +145,12 @@ __global__ __launch_bounds__(kT) void tile_kernel(TileArgs g) {
                          : reinterpret_cast<const uint8_t *>(g.planes + i * g.plane_stride) + xrow * xld,
                        xrows * xld);
   const __amdgpu_buffer_rsrc_t rxs = plane_rsrc(Q ? p.xscales + xrow * p.w.chunks * 4 : p.w.codes, Q ? xrows * p.w.chunks * 4 : 0);
-  const int64_t wtiles = min(BN / 16, p.w.tiles - t0);
+  const int gt = mx_group_tiles(p.w, t0), tg = t0 & 15, wtiles = min(BN / 16, gt - tg);
   const __amdgpu_buffer_rsrc_t rw =
-      plane_rsrc(p.w.codes + e * mx_code_bytes(p.w) + (int64_t)t0 * p.w.chunks * CB, wtiles * p.w.chunks * CB);
-  const __amdgpu_buffer_rsrc_t rws = plane_rsrc(p.w.scales + e * mx_scale_bytes(p.w) + (int64_t)(t0 / 4) * p.w.chunks * 256,
-                                                WF == FMT_MXFP4 ? (wtiles + 3) / 4 * p.w.chunks * 256 : 0);
+      plane_rsrc(p.w.codes + e * mx_code_bytes(p.w) + mx_tile_at(p.w, t0, 0), ((int64_t)(p.w.chunks - 1) * gt + wtiles) * CB);
+  const __amdgpu_buffer_rsrc_t rws =
+      plane_rsrc(p.w.scales + e * mx_scale_bytes(p.w) + mx_quad_at(p.w, t0, 0),
+                 WF == FMT_MXFP4 ? ((int64_t)(p.w.chunks - 1) * (gt / 4) + (wtiles + 3) / 4) * 256 : 0);
 
   // This lane's offsets at the first step.
   auto source = [&](int row) -> uint32_t {  // of X's row in the buffer, in rows; kNone: no row
@@ -172,9 +176,10 @@ __global__ __launch_bounds__(kT) void tile_kernel(TileArgs g) {
   for (int i = 0; i < S::NW; i++) {
     const int piece = (wave + 4 * i) * 64 + lane;  // of 16 bytes
     constexpr int per = Q ? 64 : WF == FMT_BF16 ? 128 : 32;  // pieces of a tile's step
-    woff[i] = (uint32_t)(piece / per) * (uint32_t)(p.w.chunks * CB) + (uint32_t)(piece % per) * 16;
+    woff[i] = piece / per < wtiles ? (uint32_t)(piece / per) * CB + (uint32_t)(piece % per) * 16 : kNone;
   }
-  if constexpr (WF == FMT_MXFP4) wsoff = (uint32_t)(wave % (BN / 64)) * (uint32_t)(p.w.chunks * 256) + lane * 4;
+  if constexpr (WF == FMT_MXFP4)
+    if (wave % (BN / 64) < wtiles / 4) wsoff = (uint32_t)(wave % (BN / 64)) * 256 + lane * 4;
 
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void *)lds;
   constexpr uint32_t kXS0 = P * S::kX, kW0 = kXS0 + S::kXS, kWS0 = kW0 + S::kW;
@@ -187,11 +192,13 @@ __global__ __launch_bounds__(kT) void tile_kernel(TileArgs g) {
 #pragma unroll
       for (int j = 0; j < S::NX; j++) lds_dma16(rx[i], xoff[j] + kx, mine + i * S::kX + j * 4096);
     if constexpr (Q) lds_dma4(rxs, xsoff + (in ? (uint32_t)kb * 4 : kPast), base + kXS0 + (wave % (BM / 64)) * 256);
-    const uint32_t kw = in ? (uint32_t)kb * (WF == FMT_MXFP4 && !Q ? 512 : CB) : kPast;
+    constexpr bool kHalf = WF == FMT_MXFP4 && !Q;  // a step is half a chunk
+    const uint32_t chunk = kHalf ? kb >> 1 : kb;
+    const uint32_t kw = in ? chunk * (uint32_t)(gt * CB) + (kHalf ? (kb & 1) * 512 : 0) : kPast;
 #pragma unroll
     for (int j = 0; j < S::NW; j++) lds_dma16(rw, woff[j] + kw, mine + kW0 + j * 4096);
     if constexpr (WF == FMT_MXFP4)
-      lds_dma4(rws, wsoff + (in ? (uint32_t)(Q ? kb : kb >> 1) * 256 : kPast), base + kWS0 + (wave % (BN / 64)) * 256);
+      lds_dma4(rws, wsoff + (in ? chunk * (uint32_t)(gt * 64) : kPast), base + kWS0 + (wave % (BN / 64)) * 256);
   };
 
   f32x4 acc[MF][NF];
@@ -404,9 +411,9 @@ hipError_t launch_mx_tiles(const MxProduct &p, void *scratch, hipStream_t st) {
     if (xm == 0) return launch<FMT_MXFP4, 0, 128, 256, 2, 3>(g, st);
     if (xm == 1) return launch<FMT_MXFP4, 1, 128, 256, 2, 3>(g, st);
     if (xm == 2) return launch<FMT_MXFP4, 2, 128, 256, 2, 3>(g, st);
-    return launch<FMT_MXFP4, 3, 128, 256, 2, 2>(g, st);
+    return launch<FMT_MXFP4, 3, 64, 256, 1, 2>(g, st);
   }
   if (xm == 1) return launch<FMT_BF16, 1, 128, 256, 2, 3>(g, st);
-  if (xm == 2) return launch<FMT_BF16, 2, 128, 256, 2, 2>(g, st);
-  return launch<FMT_BF16, 3, 128, 256, 2, 2>(g, st);
+  if (xm == 2) return launch<FMT_BF16, 2, 64, 256, 1, 2>(g, st);
+  return launch<FMT_BF16, 3, 64, 256, 1, 2>(g, st);
 }
