@@ -323,10 +323,11 @@ int tinyoai_weight_free(tinyoai_weight *w);
  * Types are TINYOAI_F32, TINYOAI_F16 and TINYOAI_BF16; rows of a buffer are
  * `ld` values apart.
  *
- * MXFP4 rows: for each row 64 bytes of codes (two a byte, the earlier value in
- * the low half) and 4 scale bytes per 128 columns, ceil(cols / 128) of them;
- * columns past `cols` hold zeros, as tinyoai_mxfp4_quantize_device writes them.
- * Codes lie on a 16-byte boundary, scales on a 4-byte one. */
+ * MXFP4 rows, n of them: codes [ceil(cols / 128)][n][64], the 64 bytes of a
+ * row's 128 columns two codes a byte, the earlier value in the low half; scales
+ * [ceil(cols / 128)][n][4], a byte for each 32 columns. Columns past `cols` hold
+ * zeros, as tinyoai_mxfp4_quantize_device writes them. Codes lie on a 16-byte
+ * boundary, scales on a 4-byte one. */
 
 /* n rows of `cols` values (a multiple of 32) to MXFP4: a block's scale is
  * 2^(floor(log2 m) - 2), m its largest magnitude, within 2^-127 .. 2^127; values

@@ -123,7 +123,9 @@ def mx_rows(codes, scales):
     c[:, :cols] = codes
     s = np.zeros((n, units * 4), np.uint8)
     s[:, :scales.shape[1]] = scales
-    return c[:, ::2] | c[:, 1::2] << 4, s
+    c = c[:, ::2] | c[:, 1::2] << 4
+    return (np.ascontiguousarray(c.reshape(n, units, 64).transpose(1, 0, 2)),
+            np.ascontiguousarray(s.reshape(n, units, 4).transpose(1, 0, 2)))
 
 
 def random_mx(rng, rows, cols, low=118, high=126):

@@ -262,9 +262,9 @@ def test_grouped_product_offsets(hip, dev, fmt, xdtype):
             for r in range(a, b):
                 allowed[r].append(i)
         assert (got[~seen] == 7).all()
-        for r in np.nonzero(seen)[0]:  # a row of two groups is either's
-            ok = [np.all(np.abs(got[r] - x[r] @ w[i].T) <= _tolerance(x[r:r + 1], w[i], cols)[0] * 2) for i in allowed[r]]
-            assert any(ok), (offsets, r)
+        for r in np.nonzero(seen)[0]:  # each output of a row of two groups is either's (both write it, in any order)
+            ok = [np.abs(got[r] - x[r] @ w[i].T) <= _tolerance(x[r:r + 1], w[i], cols)[0] * 2 for i in allowed[r]]
+            assert np.all(np.any(ok, 0)), (offsets, r)
     e.close()
 
 

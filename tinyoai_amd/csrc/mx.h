@@ -23,8 +23,11 @@
 // rows are the even tiles and the up rows the odd ones: one lane then holds
 // both halves of four consecutive outputs.
 //
-// Rows of quantised activations: 64 bytes of codes (two a byte, the earlier
-// one low) and 4 scale bytes for each 128 columns, zeros past the last.
+// Rows of quantised activations: for each 128 columns, 64 bytes of codes (two
+// a byte, the earlier one low) of every row, one row after another, and in an
+// array of their own 4 scale bytes of every row; zeros past the last column.
+// (What a block loads for a step is contiguous: with whole rows together, loads
+// took 64 bytes each from as many lines, and came at 14.5 TB/s instead of 24.6.)
 #pragma once
 
 #include "kernels.h"

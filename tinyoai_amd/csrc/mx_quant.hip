@@ -9,7 +9,8 @@
 //
 // What bounds it: HBM (each value read once, 17 bytes written for 32 of
 // them). Eight values a lane: four lanes hold a block, whose largest
-// magnitude they exchange by two lane moves.
+// magnitude they exchange by two lane moves; sixteen a row's 128 columns, and
+// a wave four rows', which lie together in the codes.
 #include "mx.h"
 
 namespace {
@@ -42,13 +43,13 @@ __device__ __forceinline__ void load8(const void *x, int64_t i, float (&v)[8]) {
   }
 }
 
-// One item: eight values of a row of `units` * 128 columns (zeros past cols).
+// One item: eight values of a row's 128 columns (zeros past cols).
 template <int D, bool VEC>
 __global__ __launch_bounds__(kT) void quantize_kernel(const void *x, int64_t ldx, int64_t n, int64_t cols, int64_t units,
                                                       uint32_t *codes, uint32_t *scales) {
-  const int64_t per = units * 16, total = n * per;  // a multiple of 16: the 16 lanes of a scale word stay together
+  const int64_t total = n * units * 16;  // a multiple of 16: the 16 lanes of a scale word stay together
   for (int64_t i = blockIdx.x * (int64_t)kT + threadIdx.x; i < total; i += (int64_t)gridDim.x * kT) {
-    const int64_t row = i / per, c = (i - row * per) * 8;
+    const int64_t unit = i / (n * 16), row = (i - unit * n * 16) >> 4, c = unit * 128 + (i & 15) * 8;
     float v[8] = {};
     if (c < cols) load8<D, VEC>(x, row * ldx + c, v);
     uint32_t most = 0;
@@ -82,9 +83,9 @@ __global__ __launch_bounds__(kT) void dequantize_kernel(const uint32_t *codes, c
                                                         int64_t cols, int64_t units, void *out, int64_t ldo) {
   const int64_t per = cols / 8, total = n * per;
   for (int64_t i = blockIdx.x * (int64_t)kT + threadIdx.x; i < total; i += (int64_t)gridDim.x * kT) {
-    const int64_t row = i / per, c = i - row * per;
-    const uint32_t word = codes[row * units * 16 + c];
-    const float s = mx_scale(scales[row * units * 4 + c / 4]);
+    const int64_t row = i / per, c = i - row * per, at = (c >> 4) * n + row;
+    const uint32_t word = codes[at * 16 + (c & 15)];
+    const float s = mx_scale(scales[at * 4 + ((c & 15) >> 2)]);
     float v[8];
 #pragma unroll
     for (int j = 0; j < 8; j++) v[j] = mx_code((word >> (4 * j)) & 15) * s;

@@ -14,6 +14,7 @@ namespace tinyoai_mx {
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 template <int WF>
@@ -22,7 +23,15 @@ constexpr int mx_cols() { return WF == FMT_MXFP4 ? 128 : 64; }
 __device__ __forceinline__ f32x4 mfma_bf16(uint4 a, uint4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
-// MXFP4 times MXFP4: a's scale is byte A of sa, b's byte 0 of sb.
+__device__ __forceinline__ f32x16 mfma_bf16_32(uint4 a, uint4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+// MXFP4 times MXFP4: a's scale is byte A of sa, b's byte B of sb.
+template <int A, int B>
+__device__ __forceinline__ f32x16 mfma_mx_32(uint4 a, uint4 b, f32x16 c, uint32_t sa, uint32_t sb) {
+  const i32x8 x = {(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0}, y = {(int)b.x, (int)b.y, (int)b.z, (int)b.w, 0, 0, 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x, y, c, 4, 4, A, (int)sa, B, (int)sb);
+}
 template <int A>
 __device__ __forceinline__ f32x4 mfma_mx(uint4 a, uint4 b, f32x4 c, uint32_t sa, uint32_t sb) {
   const i32x8 x = {(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0}, y = {(int)b.x, (int)b.y, (int)b.z, (int)b.w, 0, 0, 0, 0};
@@ -139,7 +148,7 @@ __device__ __forceinline__ void stage_few(const MxProduct &p, uint8_t *lds, int 
       sc[b] = 0;
       if (i >= items || src[b] < 0 || src[b] >= p.x_rows) continue;
       if constexpr (XM == 0) {
-        const int64_t at = src[b] * p.w.chunks + k0 / 128 + c / 4;
+        const int64_t at = (int64_t)(k0 / 128 + c / 4) * p.x_rows + src[b];
         raw[b].a[0] = *reinterpret_cast<const uint4 *>(static_cast<const uint8_t *>(p.x) + at * 64 + (c & 3) * 16);
         if ((c & 3) == 0) sc[b] = reinterpret_cast<const uint32_t *>(p.xscales)[at];
       } else {

@@ -3,16 +3,21 @@
 // A block forms BM rows of one group times BN = 256 stored matrix rows; both
 // operands go straight to LDS (buffer loads to LDS, rows picked by the index
 // on the way), a ring of stages ahead of the products, and each wave holds MF x
-// NF tiles of 16 x 16 sums. What bounds it: the matrix cores. The matrix is
-// the first operand, so a lane ends with four consecutive outputs of a row.
+// NF tiles of 32 x 32 sums. What bounds it: the matrix cores, and at a short K
+// the output's stores. The matrix is the first operand, so a lane ends with
+// four runs of four outputs of a row, and of a pair with both halves; the sums
+// go through LDS so that whole rows of a wave's outputs are stored together
+// (as they are, a store would take 16-byte pieces of 32 rows).
+// (v_mfma of 16 x 16 x 4 k at the same rate on paper: alone on its SIMD a wave
+// keeps it at half of that, and at 0.9 of the 32 x 32 one.)
 //
 //   planes of X (1, 2 or 3, bf16; mx_tile.h) times BF16, or times MXFP4 codes
 //   that become bf16 times their scale as a wave reads them (exact): 64
-//   columns a step, v_mfma_f32_16x16x32_bf16. Lane l of an operand holds the
-//   step's columns 16 (l / 16) .. + 15 of its row, eight for each of the two
-//   products;
-//   MXFP4 times MXFP4: 128 columns a step, one
-//   v_mfma_scale_f32_16x16x128_f8f6f4 a tile.
+//   columns a step, four v_mfma_f32_32x32x16_bf16. Lane (row, h) takes columns
+//   32 b + 16 h + 8 t .. + 7 of its row for product 2 b + t;
+//   MXFP4 times MXFP4: 128 columns a step, two
+//   v_mfma_scale_f32_32x32x64_f8f6f4; lane (row, h) takes block 2 j + h for
+//   product j.
 //
 // X rows in LDS: the step's 16-byte pieces of a row, piece c at a place that
 // depends on the row, so that 16 rows' reads of one piece hit distinct banks.
@@ -29,7 +34,7 @@ namespace {
 
 using namespace tinyoai_mx;
 
-constexpr int kT = 256, kBand = 8;
+constexpr int kBand = 8;
 constexpr uint32_t kNone = 0x80000000u, kPast = 0x40000000u;
 
 struct TileArgs {
@@ -40,7 +45,7 @@ struct TileArgs {
   int mtiles;  // row tiles there can be
 };
 
-template <int WF, int XM, int BM, int BN>
+template <int WF, int XM, int BM, int BN, int WAVES>
 struct Shape {
   static constexpr bool Q = XM == 0;
   static constexpr int P = Q ? 1 : XM;
@@ -50,9 +55,10 @@ struct Shape {
   static constexpr int kWS = WF == FMT_MXFP4 ? BN / 64 * 256 : 0;
   static constexpr int kStage = P * kX + kXS + kW + kWS;
   // wave loads of a step
-  static constexpr int NX = kX / 4096, NXS = Q ? 1 : 0, NW = kW / 4096, NWS = WF == FMT_MXFP4 ? 1 : 0;
+  static constexpr int kAll = WAVES * 1024;  // bytes of a load of every wave
+  static constexpr int NX = kX / kAll, NXS = Q ? 1 : 0, NW = kW / kAll, NWS = WF == FMT_MXFP4 ? 1 : 0;
   static constexpr int kLoads = P * NX + NXS + NW + NWS;
-  static_assert(kX % 4096 == 0 && kW % 4096 == 0 && BN % 64 == 0 && BN <= 256, "whole loads of every wave");
+  static_assert(kX % kAll == 0 && kW % kAll == 0 && BN % 64 == 0 && BN <= 256, "whole loads of every wave");
 };
 
 // This block's group and first row, from its number among all row tiles;
@@ -112,16 +118,16 @@ __device__ __forceinline__ bool find_tile(const MxProduct &p, int lane, int ntil
   return false;
 }
 
-template <int WF, int XM, int BM, int BN, int WM, int STAGES>
-__global__ __launch_bounds__(kT, 2) void tile_kernel(TileArgs g) {
-  using S = Shape<WF, XM, BM, BN>;
+template <int WF, int XM, int BM, int BN, int WAVES, int WM, int STAGES>
+__global__ __launch_bounds__(WAVES * 64, WAVES == 4 ? 2 : 1) void tile_kernel(TileArgs g) {
+  using S = Shape<WF, XM, BM, BN, WAVES>;
   constexpr bool Q = S::Q;
-  constexpr int P = S::P, WN = 4 / WM, MF = BM / 16 / WM, NF = BN / 16 / WN;
-  static_assert(MF * WM * 16 == BM && NF * WN * 16 == BN && NF % 4 == 0, "whole scale quads a wave");
+  constexpr int P = S::P, WN = WAVES / WM, MF = BM / 32 / WM, NF = BN / 32 / WN;
+  static_assert(MF * WM * 32 == BM && NF * WN * 32 == BN && NF % 2 == 0, "whole scale quads a wave");
   extern __shared__ __align__(16) uint8_t lds[];
   const MxProduct &p = g.p;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int l16 = lane & 15, q = lane >> 4;
+  const int l32 = lane & 31, h = lane >> 5;
   const int wm = wave / WN, wn = wave - wm * WN;
 
   int e, r0, r1, nt;
@@ -136,15 +142,17 @@ __global__ __launch_bounds__(kT, 2) void tile_kernel(TileArgs g) {
   // Buffers: X from its first row (no index: from the tile's), the matrix from
   // the block's first tile; past them reads zeros.
   const int64_t xrow = p.index ? 0 : r0;
-  const int64_t xld = Q ? (int64_t)p.w.chunks * 64 : g.ldp * 2;  // bytes
+  const int64_t xld = Q ? 64 : g.ldp * 2;  // bytes
+  const int64_t xunit = Q ? (int64_t)p.x_rows * 64 : 128;  // from one step's columns to the next
   const int64_t xrows = p.index ? p.x_rows : min(BM, p.x_rows - r0);
   __amdgpu_buffer_rsrc_t rx[P];
 #pragma unroll
   for (int i = 0; i < P; i++)
     rx[i] = plane_rsrc(Q ? static_cast<const uint8_t *>(p.x) + xrow * xld
                          : reinterpret_cast<const uint8_t *>(g.planes + i * g.plane_stride) + xrow * xld,
-                       xrows * xld);
-  const __amdgpu_buffer_rsrc_t rxs = plane_rsrc(Q ? p.xscales + xrow * p.w.chunks * 4 : p.w.codes, Q ? xrows * p.w.chunks * 4 : 0);
+                       Q ? (steps - 1) * xunit + xrows * 64 : xrows * xld);
+  const __amdgpu_buffer_rsrc_t rxs =
+      plane_rsrc(Q ? p.xscales + xrow * 4 : p.w.codes, Q ? (int64_t)(steps - 1) * p.x_rows * 4 + xrows * 4 : 0);
   const int gt = mx_group_tiles(p.w, t0), tg = t0 & 15, wtiles = min(BN / 16, gt - tg);
   const __amdgpu_buffer_rsrc_t rw =
       plane_rsrc(p.w.codes + e * mx_code_bytes(p.w) + mx_tile_at(p.w, t0, 0), ((int64_t)(p.w.chunks - 1) * gt + wtiles) * CB);
@@ -163,18 +171,18 @@ __global__ __launch_bounds__(kT, 2) void tile_kernel(TileArgs g) {
   uint32_t xoff[S::NX], woff[S::NW], xsoff = kNone, wsoff = kNone;
 #pragma unroll
   for (int i = 0; i < S::NX; i++) {
-    const int row = (wave + 4 * i) * (Q ? 16 : 8) + (Q ? lane >> 2 : lane >> 3);
+    const int row = (wave + WAVES * i) * (Q ? 16 : 8) + (Q ? lane >> 2 : lane >> 3);
     const uint32_t piece = Q ? (lane & 3) ^ ((row >> 2) & 3) : (lane & 7) ^ ((row >> 1) & 7);
     const uint32_t src = source(row);
     xoff[i] = src == kNone ? kNone : src * (uint32_t)xld + piece * 16;
   }
   if constexpr (Q) {  // (waves past BM / 64 repeat the others' loads)
     const uint32_t src = source((wave % (BM / 64)) * 64 + lane);
-    xsoff = src == kNone ? kNone : src * (uint32_t)(p.w.chunks * 4);
+    xsoff = src == kNone ? kNone : src * 4;
   }
 #pragma unroll
   for (int i = 0; i < S::NW; i++) {
-    const int piece = (wave + 4 * i) * 64 + lane;  // of 16 bytes
+    const int piece = (wave + WAVES * i) * 64 + lane;  // of 16 bytes
     constexpr int per = Q ? 64 : WF == FMT_BF16 ? 128 : 32;  // pieces of a tile's step
     woff[i] = piece / per < wtiles ? (uint32_t)(piece / per) * CB + (uint32_t)(piece % per) * 16 : kNone;
   }
@@ -186,146 +194,199 @@ __global__ __launch_bounds__(kT, 2) void tile_kernel(TileArgs g) {
   auto issue = [&](int kb, int slot) {
     const bool in = kb < steps;
     const uint32_t base = lds0 + slot * S::kStage, mine = base + wave * 1024;
-    const uint32_t kx = in ? (uint32_t)kb * (Q ? 64 : 128) : kPast;
+    const uint32_t kx = in ? (uint32_t)kb * (uint32_t)xunit : kPast;
 #pragma unroll
     for (int i = 0; i < P; i++)
 #pragma unroll
-      for (int j = 0; j < S::NX; j++) lds_dma16(rx[i], xoff[j] + kx, mine + i * S::kX + j * 4096);
-    if constexpr (Q) lds_dma4(rxs, xsoff + (in ? (uint32_t)kb * 4 : kPast), base + kXS0 + (wave % (BM / 64)) * 256);
+      for (int j = 0; j < S::NX; j++) lds_dma16(rx[i], xoff[j] + kx, mine + i * S::kX + j * S::kAll);
+    if constexpr (Q) lds_dma4(rxs, xsoff + (in ? (uint32_t)kb * (uint32_t)(p.x_rows * 4) : kPast), base + kXS0 + (wave % (BM / 64)) * 256);
     constexpr bool kHalf = WF == FMT_MXFP4 && !Q;  // a step is half a chunk
     const uint32_t chunk = kHalf ? kb >> 1 : kb;
     const uint32_t kw = in ? chunk * (uint32_t)(gt * CB) + (kHalf ? (kb & 1) * 512 : 0) : kPast;
 #pragma unroll
-    for (int j = 0; j < S::NW; j++) lds_dma16(rw, woff[j] + kw, mine + kW0 + j * 4096);
+    for (int j = 0; j < S::NW; j++) lds_dma16(rw, woff[j] + kw, mine + kW0 + j * S::kAll);
     if constexpr (WF == FMT_MXFP4)
       lds_dma4(rws, wsoff + (in ? chunk * (uint32_t)(gt * 64) : kPast), base + kWS0 + (wave % (BN / 64)) * 256);
   };
 
-  f32x4 acc[MF][NF];
+  f32x16 acc[MF][NF];
 #pragma unroll
   for (int f = 0; f < MF; f++)
 #pragma unroll
-    for (int n = 0; n < NF; n++) acc[f][n] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const int xr = wm * MF * 16 + l16;  // this lane's row of the wave's first row tile
-  auto compute = [&](int kb, int slot) {
+    for (int n = 0; n < NF; n++)
+#pragma unroll
+      for (int v = 0; v < 16; v++) acc[f][n][v] = 0.f;
+  const int xr = wm * MF * 32 + l32;            // this lane's row of the wave's first row tile
+  const int wt = (lane & 31) >> 4, l16 = lane & 15;  // its matrix row: of the pair's tile wt, row l16
+  // A step's operands go through registers in two halves, each read from LDS
+  // while the products of the half before it run: a wave meets the barrier
+  // between them, so neither it nor the reads leave the matrix cores waiting.
+  struct Half {
+    uint4 x[MF][P][Q ? 1 : 2];
+    uint4 w[WF == FMT_BF16 || Q ? NF : 1][Q ? 1 : 2];
+    uint2 c[WF == FMT_MXFP4 && !Q ? NF : 1];  // codes
+    uint32_t sw[NF / 2], sx[Q ? MF : 1];
+  };
+  auto read = [&](Half &H, int kb, int slot, int b) {
     const uint8_t *st = lds + slot * S::kStage;
-    if constexpr (Q) {
-      uint4 x[MF];
-      uint32_t sx[MF];
 #pragma unroll
-      for (int f = 0; f < MF; f++) {
-        const int row = xr + f * 16;
-        x[f] = *reinterpret_cast<const uint4 *>(st + row * 64 + ((q ^ ((row >> 2) & 3)) << 4));
-        sx[f] = *reinterpret_cast<const uint32_t *>(st + kXS0 + row * 4) >> (8 * q);
+    for (int f = 0; f < MF; f++) {
+      const int row = xr + f * 32;
+      if constexpr (Q) {
+        H.x[f][0][0] = *reinterpret_cast<const uint4 *>(st + row * 64 + (((2 * b + h) ^ ((row >> 2) & 3)) << 4));
+        H.sx[f] = *reinterpret_cast<const uint32_t *>(st + kXS0 + row * 4);
+      } else {
+#pragma unroll
+        for (int i = 0; i < P; i++)
+#pragma unroll
+          for (int t = 0; t < 2; t++)
+            H.x[f][i][t] = *reinterpret_cast<const uint4 *>(st + i * S::kX + row * 128 + (((4 * b + 2 * h + t) ^ ((row >> 1) & 7)) << 4));
       }
+    }
 #pragma unroll
-      for (int n4 = 0; n4 < NF / 4; n4++) {
-        const uint32_t sw = *reinterpret_cast<const uint32_t *>(st + kWS0 + (wn * NF / 4 + n4) * 256 + lane * 4);
-        uint4 w[4];
+    for (int n = 0; n < NF; n++) {
+      const int tile = (wn * NF + n) * 2 + wt;
+      if constexpr (Q)
+        H.w[n][0] = *reinterpret_cast<const uint4 *>(st + kW0 + tile * 1024 + (2 * b + h) * 256 + l16 * 16);
+      else if constexpr (WF == FMT_BF16)
 #pragma unroll
-        for (int i = 0; i < 4; i++) w[i] = *reinterpret_cast<const uint4 *>(st + kW0 + (wn * NF + n4 * 4 + i) * 1024 + lane * 16);
+        for (int t = 0; t < 2; t++)
+          H.w[n][t] = *reinterpret_cast<const uint4 *>(st + kW0 + tile * 2048 + t * 1024 + ((2 * b + h) * 16 + l16) * 16);
+      else
+        H.c[n] = *reinterpret_cast<const uint2 *>(st + kW0 + tile * 512 + b * 256 + l16 * 16 + h * 8);
+    }
+    if constexpr (WF == FMT_MXFP4)
+#pragma unroll
+      for (int n = 0; n < NF / 2; n++)  // the word of four tiles' scales of this row and block
+        H.sw[n] = *reinterpret_cast<const uint32_t *>(st + kWS0 + (wn * NF / 2 + n) * 256 +
+                                                      ((Q ? 2 * b + h : (kb & 1) * 2 + b) * 16 + l16) * 4);
+  };
+  auto multiply = [&](const Half &H, auto half) {
+    constexpr int b = decltype(half)::value;
+    if constexpr (Q) {
+#pragma unroll
+      for (int n = 0; n < NF; n += 2) {
+        const uint32_t sw = H.sw[n / 2] >> (8 * wt);  // bytes 0 and 2: the pair's two tiles of this lane's row
 #pragma unroll
         for (int f = 0; f < MF; f++) {
-          acc[f][n4 * 4 + 0] = mfma_mx<0>(w[0], x[f], acc[f][n4 * 4 + 0], sw, sx[f]);
-          acc[f][n4 * 4 + 1] = mfma_mx<1>(w[1], x[f], acc[f][n4 * 4 + 1], sw, sx[f]);
-          acc[f][n4 * 4 + 2] = mfma_mx<2>(w[2], x[f], acc[f][n4 * 4 + 2], sw, sx[f]);
-          acc[f][n4 * 4 + 3] = mfma_mx<3>(w[3], x[f], acc[f][n4 * 4 + 3], sw, sx[f]);
+          const uint32_t sx = H.sx[f] >> (8 * h);  // bytes 0 and 2: blocks h, 2 + h
+          acc[f][n] = mfma_mx_32<0, 2 * b>(H.w[n][0], H.x[f][0][0], acc[f][n], sw, sx);
+          acc[f][n + 1] = mfma_mx_32<2, 2 * b>(H.w[n + 1][0], H.x[f][0][0], acc[f][n + 1], sw, sx);
         }
       }
     } else {
       uint4 w[NF][2];
-      if constexpr (WF == FMT_BF16) {
 #pragma unroll
-        for (int n = 0; n < NF; n++)
-#pragma unroll
-          for (int j = 0; j < 2; j++) w[n][j] = *reinterpret_cast<const uint4 *>(st + kW0 + (wn * NF + n) * 2048 + j * 1024 + lane * 16);
-      } else {
-        // lane (row, q): block q / 2 of the step's two, its bytes 8 (q % 2) .. + 7
-        const int at = (q >> 1) * 256 + l16 * 16 + (q & 1) * 8;
-        const int sl = ((kb & 1) * 2 + (q >> 1)) * 16 + l16;  // where the chunk's scale word of this row and block is
-#pragma unroll
-        for (int n4 = 0; n4 < NF / 4; n4++) {
-          const uint32_t sw = *reinterpret_cast<const uint32_t *>(st + kWS0 + (wn * NF / 4 + n4) * 256 + sl * 4);
+      for (int n = 0; n < NF; n++) {
+        if constexpr (WF == FMT_BF16) {
+          w[n][0] = H.w[n][0];
+          w[n][1] = H.w[n][1];
+        } else {
           // the tile's scale byte in an exponent's place; the conversion takes no other bit
-          const uint32_t sc[4] = {sw << 23, sw << 15, sw << 7, sw >> 1};
-#pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const uint2 c = *reinterpret_cast<const uint2 *>(st + kW0 + (wn * NF + n4 * 4 + i) * 512 + at);
-            w[n4 * 4 + i][0] = fp4_bf16(c.x, __uint_as_float(sc[i]));
-            w[n4 * 4 + i][1] = fp4_bf16(c.y, __uint_as_float(sc[i]));
-          }
+          const uint32_t sw = H.sw[n / 2] >> (8 * wt);
+          const float sc = __uint_as_float(n & 1 ? sw << 7 : sw << 23);
+          w[n][0] = fp4_bf16(H.c[n].x, sc);
+          w[n][1] = fp4_bf16(H.c[n].y, sc);
         }
       }
 #pragma unroll
-      for (int j = 0; j < 2; j++)
+      for (int t = 0; t < 2; t++)
 #pragma unroll
-        for (int i = 0; i < P; i++) {
-          uint4 x[MF];
-#pragma unroll
-          for (int f = 0; f < MF; f++) {
-            const int row = xr + f * 16;
-            x[f] = *reinterpret_cast<const uint4 *>(st + i * S::kX + row * 128 + (((2 * q + j) ^ ((row >> 1) & 7)) << 4));
-          }
+        for (int i = 0; i < P; i++)
 #pragma unroll
           for (int f = 0; f < MF; f++)
 #pragma unroll
-            for (int n = 0; n < NF; n++) acc[f][n] = mfma_bf16(w[n][j], x[f], acc[f][n]);
-        }
+            for (int n = 0; n < NF; n++) acc[f][n] = mfma_bf16_32(w[n][t], H.x[f][i][t], acc[f][n]);
     }
   };
 
 #pragma unroll
   for (int i = 0; i < STAGES - 1; i++) issue(i, i);
-  int slot = 0;
-  for (int kb = 0; kb < steps; kb++) {
-    wait_vmcnt<S::kLoads *(STAGES - 2)>();  // this wave's loads of kb (later steps' may be in flight)
-    __syncthreads();
-    issue(kb + STAGES - 1, slot == 0 ? STAGES - 1 : slot - 1);
-    compute(kb, slot);
-    slot = slot + 1 == STAGES ? 0 : slot + 1;
+  wait_vmcnt<S::kLoads *(STAGES - 2)>();
+  __syncthreads();
+  Half A, B;
+  read(A, 0, 0, 0);
+  issue(STAGES - 1, STAGES - 1);
+  for (int kb = 0, slot = 0; kb < steps; kb++) {
+    const int next = slot + 1 == STAGES ? 0 : slot + 1;
+    read(B, kb, slot, 1);
+    multiply(A, std::integral_constant<int, 0>());
+    __builtin_amdgcn_sched_barrier(0);
+    wait_vmcnt<S::kLoads *(STAGES - 2)>();  // this wave's loads of kb + 1 (later steps' may be in flight)
+    __syncthreads();                        // every wave's; and all are past their reads of kb
+    issue(kb + STAGES, slot);
+    read(A, kb + 1, next, 0);  // (past the last step: zeros)
+    multiply(B, std::integral_constant<int, 1>());
+    __builtin_amdgcn_sched_barrier(0);
+    slot = next;
   }
-  wait_vmcnt<0>();  // nothing may land in LDS after the block
+  wait_vmcnt<0>();  // nothing may land in LDS any more
+  __syncthreads();
 
-  // Lane: row l16 of row tile f, outputs 4 q .. + 3 of tile n.
-  const bool vec = p.ldo % 4 == 0 && reinterpret_cast<uintptr_t>(p.out) % (p.odtype == FMT_F32 ? 16 : 8) == 0;
+  // Lane: row l32 of row tile f; sum v of tile n is of matrix row 8 (v / 4) +
+  // 4 h + v % 4. The wave's outputs of a row tile as rows in its part of LDS,
+  // then to memory a whole row's at a time.
+  const int C = p.w.gate ? NF * 16 : NF * 32, pitch = C + 4;
+  float *mine = reinterpret_cast<float *>(lds) + wave * (32 * (NF * 32 + 4));
+  const bool wide = p.odtype == FMT_F32;
+  const int V = wide ? 4 : 8, lanes = C / V, at = lane % lanes * V;  // outputs of a lane, lanes of a row
+  const bool vec = p.ldo % V == 0 && reinterpret_cast<uintptr_t>(p.out) % 16 == 0;
+  const int o = (p.w.gate ? (t0 + wn * NF * 2) / 2 : t0 + wn * NF * 2) * 16 + at;
 #pragma unroll
   for (int f = 0; f < MF; f++) {
-    const int r = r0 + xr + f * 16;
-    if (r >= r1) continue;
-    bool none = false;
-    if (p.index) {
-      const int src = p.index[r];
+    const int first = r0 + wm * MF * 32 + f * 32;
+    if (first >= r1) break;
+    bool none = false;  // the index names no row: zeros, whatever the matrix holds
+    if (p.index && first + l32 < r1) {
+      const int src = p.index[first + l32];
       none = src < 0 || src >= p.x_rows;
     }
-    const int64_t row = r * p.ldo;
-    auto put = [&](int tile, f32x4 v) {
-      const int o = tile * 16 + 4 * q;
-      if (none) v = f32x4{0.f, 0.f, 0.f, 0.f};  // whatever the matrix holds
-      if (vec && o + 3 < p.w.rows) {
-        if (p.odtype == FMT_F32)
-          *reinterpret_cast<f32x4 *>(static_cast<float *>(p.out) + row + o) = v;
-        else
-          *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + row + o) =
-              make_uint2(mx_narrow(p.odtype, v[0]) | (uint32_t)mx_narrow(p.odtype, v[1]) << 16,
-                         mx_narrow(p.odtype, v[2]) | (uint32_t)mx_narrow(p.odtype, v[3]) << 16);
-      } else {
+    const uint32_t zeros = (uint32_t)__ballot(none);
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-          if (o + i < p.w.rows) mx_store(p.odtype, p.out, row + o + i, v[i]);
-      }
-    };
-    if (p.w.gate) {
+    for (int n = 0; n < NF; n++)
 #pragma unroll
-      for (int n = 0; n < NF; n += 2) {
+      for (int u = 0; u < 4; u++) {
+        if (p.w.gate && u >= 2) continue;
         f32x4 v;
 #pragma unroll
-        for (int i = 0; i < 4; i++) v[i] = mx_gate(acc[f][n][i], acc[f][n + 1][i]);
-        put((t0 + wn * NF + n) / 2, v);
+        for (int i = 0; i < 4; i++) v[i] = p.w.gate ? mx_gate(acc[f][n][u * 4 + i], acc[f][n][(u * 4 + i + 8) & 15]) : acc[f][n][u * 4 + i];
+        *reinterpret_cast<f32x4 *>(mine + l32 * pitch + n * (p.w.gate ? 16 : 32) + u * 8 + h * 4) = v;
       }
-    } else {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll 4
+    for (int i = 0; i < 32; i += 64 / lanes) {
+      const int row = i + lane / lanes, r = first + row;
+      if (r >= r1 || o >= p.w.rows) continue;
+      const bool zero = zeros >> row & 1;
+      float v[8];
 #pragma unroll
-      for (int n = 0; n < NF; n++) put(t0 + wn * NF + n, acc[f][n]);
+      for (int j = 0; j < 8; j += 4) {
+        if (j && wide) continue;
+        const f32x4 a = *reinterpret_cast<const f32x4 *>(mine + row * pitch + at + j);
+#pragma unroll
+        for (int k = 0; k < 4; k++) v[j + k] = zero ? 0.f : a[k];
+      }
+      const int64_t to = r * p.ldo + o;
+      if (vec && o + V <= p.w.rows) {
+        if (wide) {
+          __builtin_nontemporal_store(f32x4{v[0], v[1], v[2], v[3]}, reinterpret_cast<f32x4 *>(static_cast<float *>(p.out) + to));
+        } else {
+          uint32_t w[4];
+#pragma unroll
+          for (int k = 0; k < 4; k++) w[k] = mx_narrow(p.odtype, v[2 * k]) | (uint32_t)mx_narrow(p.odtype, v[2 * k + 1]) << 16;
+          __builtin_nontemporal_store(u32x4{w[0], w[1], w[2], w[3]}, reinterpret_cast<u32x4 *>(static_cast<uint16_t *>(p.out) + to));
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+          if (k < V && o + k < p.w.rows) mx_store(p.odtype, p.out, to + k, v[k]);
+      }
     }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
   }
 }
 
@@ -349,14 +410,15 @@ bool direct(const MxProduct &p) {
   return p.xdtype == FMT_BF16 && p.w.cols % 64 == 0 && p.ldx % 8 == 0 && reinterpret_cast<uintptr_t>(p.x) % 16 == 0;
 }
 
-template <int WF, int XM, int BM, int BN, int WM, int STAGES>
+template <int WF, int XM, int BM, int BN, int WAVES, int WM, int STAGES>
 hipError_t launch(TileArgs &g, hipStream_t st) {
-  using S = Shape<WF, XM, BM, BN>;
+  using S = Shape<WF, XM, BM, BN, WAVES>;
   const MxProduct &p = g.p;
-  constexpr int bytes = STAGES * S::kStage;
+  constexpr int rows = WAVES * 32 * (BN / (WAVES / WM) + 4) * 4;  // the waves' outputs
+  constexpr int bytes = STAGES * S::kStage > rows ? STAGES * S::kStage : rows;
   static_assert(bytes <= 160 * 1024, "LDS of a CU");
   static bool set = false;
-  const auto kernel = &tile_kernel<WF, XM, BM, BN, WM, STAGES>;
+  const auto kernel = &tile_kernel<WF, XM, BM, BN, WAVES, WM, STAGES>;
   if (!set) {
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != hipSuccess) return e;
@@ -366,7 +428,7 @@ hipError_t launch(TileArgs &g, hipStream_t st) {
   const int64_t groups = p.offsets ? std::min(p.w.experts, p.n) : 1;
   const int64_t mtiles = p.offsets ? (p.n + groups * (BM - 1)) / BM : (p.n + BM - 1) / BM;
   const int64_t blocks = (mtiles * ((p.w.tiles * 16 + BN - 1) / BN) + 7) / 8 * 8;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kT), bytes, st, g);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(WAVES * 64), bytes, st, g);
   return hipGetLastError();
 }
 
@@ -377,11 +439,13 @@ size_t mx_tiles_scratch(const MxProduct &p) {
   return (size_t)mx_planes(p.xdtype) * p.x_rows * padded_cols(p) * 2;
 }
 
-// Offsets within a buffer stay below 2^31 bytes: X where an index may name any
-// of its rows (else the tile's rows alone), a block's 256 matrix rows.
+// Offsets within a buffer stay below 2^30 bytes: MXFP4 rows, and X where an
+// index may name any of its rows (else the tile's rows alone); a block's 256
+// matrix rows.
 bool mx_tiles_supported(const MxProduct &p) {
-  const int64_t ld = p.xdtype == FMT_MXFP4 ? (int64_t)p.w.chunks * 64 : direct(p) ? p.ldx * 2 : padded_cols(p) * 2;
-  return (p.index ? p.x_rows : 256) * ld < kPast && (int64_t)p.w.chunks * mx_chunk_bytes(p.w.fmt) * 16 < kPast;
+  const bool mx = p.xdtype == FMT_MXFP4;
+  const int64_t ld = mx ? (int64_t)p.w.chunks * 64 : direct(p) ? p.ldx * 2 : padded_cols(p) * 2;
+  return (p.index || mx ? p.x_rows : 256) * ld < kPast && (int64_t)p.w.chunks * mx_chunk_bytes(p.w.fmt) * 16 < kPast;
 }
 
 hipError_t launch_mx_tiles(const MxProduct &p, void *scratch, hipStream_t st) {
@@ -408,12 +472,12 @@ hipError_t launch_mx_tiles(const MxProduct &p, void *scratch, hipStream_t st) {
   }
   const int xm = p.xdtype == FMT_MXFP4 ? 0 : mx_planes(p.xdtype);
   if (p.w.fmt == FMT_MXFP4) {
-    if (xm == 0) return launch<FMT_MXFP4, 0, 128, 256, 2, 3>(g, st);
-    if (xm == 1) return launch<FMT_MXFP4, 1, 128, 256, 2, 3>(g, st);
-    if (xm == 2) return launch<FMT_MXFP4, 2, 128, 256, 2, 3>(g, st);
-    return launch<FMT_MXFP4, 3, 64, 256, 1, 2>(g, st);
+    if (xm == 0) return launch<FMT_MXFP4, 0, 128, 256, 4, 2, 3>(g, st);
+    if (xm == 1) return launch<FMT_MXFP4, 1, 128, 256, 4, 2, 3>(g, st);
+    if (xm == 2) return launch<FMT_MXFP4, 2, 128, 256, 4, 2, 3>(g, st);
+    return launch<FMT_MXFP4, 3, 64, 256, 4, 1, 2>(g, st);
   }
-  if (xm == 1) return launch<FMT_BF16, 1, 128, 256, 2, 3>(g, st);
-  if (xm == 2) return launch<FMT_BF16, 2, 64, 256, 1, 2>(g, st);
-  return launch<FMT_BF16, 3, 64, 256, 1, 2>(g, st);
+  if (xm == 1) return launch<FMT_BF16, 1, 128, 256, 4, 2, 3>(g, st);
+  if (xm == 2) return launch<FMT_BF16, 2, 64, 256, 4, 1, 2>(g, st);
+  return launch<FMT_BF16, 3, 64, 256, 4, 1, 2>(g, st);
 }

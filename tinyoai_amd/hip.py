@@ -154,7 +154,8 @@ def summarize_logits(logits: np.ndarray, targets, count: int):
 # hipStream_t, 0 the current device's default stream (a handle's methods: its
 # own stream). Types are the codes of tinyoai_amd.weights.
 def mxfp4_row_bytes(cols: int) -> tuple[int, int]:
-    """(code bytes, scale bytes) of a row of MXFP4 values."""
+    """(code bytes, scale bytes) that a row of MXFP4 values adds to its
+    buffers (all rows' bytes of 128 columns lie together)."""
     units = -(-cols // 128)
     return 64 * units, 4 * units
 
