@@ -127,9 +127,7 @@ int ExpertMatrix::upload(int32_t dtype, int32_t experts, int64_t rows, int64_t c
       const uint8_t *src = (const uint8_t *)(phase ? up : data) + (size_t)i * each;
       if (e == hipSuccess) e = hipMemcpyAsync(raw, src, each, hipMemcpyHostToDevice, st);
       if (e == hipSuccess) e = launch_mx_place(m, (const uint8_t *)raw, i, phase, st);
-      // One copy from the caller's pageable memory at a time: the next one takes
-      // the same buffer, and may be of the same or of a neighbouring host page.
-      if (e == hipSuccess) e = hipStreamSynchronize(st);
+      if (e == hipSuccess) e = hipStreamSynchronize(st);  // the next copy takes the same buffer
     }
   hipFree(raw);
   if (e != hipSuccess) return hip_fail(e, "expert upload");
