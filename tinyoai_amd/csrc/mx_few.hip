@@ -1,10 +1,14 @@
 // Products of a few rows with expert matrices (mx.h): one decode step.
 //
 // y[r][o] = sum over k of x[r][k] w[o][k]. What bounds it: each matrix that
-// some row needs is read once from HBM, so a wave streams 1 KB (BF16: 2 KB) of
-// one tile of 16 matrix rows an instruction, in the order of the matrix
-// cores' operand, several loads ahead; the rows of X, which every wave of a
-// block shares, sit in LDS.
+// some row needs is read once from HBM. The waves of a block share the
+// columns: a wave holds its columns of X in registers, as operands of the
+// matrix cores, and streams its columns of one tile of 16 matrix rows after
+// another (pairs: of two), each chunk's registers loaded again for the next
+// tile once it is multiplied; a load takes 1 KB of a tile as it is stored. So nothing but sums goes through LDS: the
+// waves' parts of a tile meet there. (With X in LDS, every wave whole tiles of
+// its own, a block had to stage the rows in parts, and eight waves fitted a CU:
+// 16 tokens' gate and up of 32 experts, 1728 x 2560, took 43 us.)
 //
 // fp32 and fp16 rows keep all their bits: a value is the exact sum of three
 // (fp16: two) bf16 planes, truncations of what is left, and each plane is an
@@ -21,255 +25,301 @@ namespace {
 
 using namespace tinyoai_mx;
 
-constexpr int kT = 512, kWaves = 8, kCols = 4;  // column tiles: 64 virtual columns
-constexpr int kAhead = 4;                       // chunks in flight a wave
+constexpr uint32_t kNone = 0x80000000u;  // past every buffer
+
+// LDS written by the wave is read by its other lanes.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+__device__ __forceinline__ uint4 load16(__amdgpu_buffer_rsrc_t r, uint32_t at) {
+  const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(r, (int)at, 0, 0);
+  return make_uint4(v.x, v.y, v.z, v.w);
+}
 
 struct FewArgs {
   MxProduct p;
-  int ksplit, kshift;  // waves that share a unit's columns: 1, 2, 4 or 8; its logarithm
-  int units;     // tiles (pairs: of both) of an expert
-  int per;       // units of a block, a multiple of kWaves / ksplit
-  int seg;       // column chunks in LDS at once
-  int rows;      // rows of X at once (rows * planes <= 16 * kCols)
+  int units;  // tiles (pairs: of both) of an expert
+  int per;    // units of a block
+  int64_t x_bytes;
 };
 
-// X's bytes in LDS for one chunk of columns and one virtual column.
-template <int WF, int XM>
-constexpr int chunk_bytes() { return XM == 0 ? 68 : mx_cols<WF>() * 2; }
+constexpr int NC = 4;  // column chunks of a wave, at most
 
-template <int WF>
-struct Raw {
-  uint4 w[WF == FMT_MXFP4 ? 1 : 2];
-};
-template <int WF, int NT>
-struct Fetch {
-  Raw<WF> t[NT];
-  uint32_t s;  // the scale quad's word
-};
-
-template <int WF, int XM, bool GATE>
-__global__ __launch_bounds__(kT) void few_kernel(FewArgs g) {
-  constexpr int NT = GATE ? 2 : 1, P = XM == 0 ? 1 : XM;
-  constexpr int kUnitCols = mx_cols<WF>();  // columns of a chunk
-  extern __shared__ __align__(16) uint8_t lds[];
+// CT: column tiles (16 operand columns).
+template <int WF, int XM, bool GATE, int kWaves, int CT>
+__global__ __launch_bounds__(kWaves * 64) void few_kernel(FewArgs g) {
+  constexpr int NT = GATE ? 2 : 1, P = XM == 0 ? 1 : XM, NJ = WF == FMT_MXFP4 ? 4 : 2;
+  constexpr int kChunk = mx_cols<WF>();
+  constexpr int kRows = 16 * CT / P;            // rows of X at once
+  constexpr int kRed = kWaves * NT * CT * 256;  // sums of a unit
+  constexpr int kT = kWaves * 64;
+  constexpr int kStaged = XM >= 2 ? kWaves * CT * 16 * kChunk / 4 : 0;  // floats; half of each wave's planes of a chunk
+  __shared__ __align__(16) float red[2][kRed > kStaged ? kRed : kStaged];
   const MxProduct &p = g.p;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int e = blockIdx.y;
+  const int e = blockIdx.y, l16 = lane & 15, q = lane >> 4;
   int r_lo = 0, r_hi = p.n;
   if (p.offsets) {
     r_lo = min(max(p.offsets[e], 0), p.n);
     r_hi = min(max(p.offsets[e + 1], r_lo), p.n);
   }
-  const int G = kWaves / g.ksplit, part = wave % g.ksplit, u0 = blockIdx.x * g.per + wave / g.ksplit;
-  const int u_end = min((int)(blockIdx.x + 1) * g.per, g.units);
-  const int passes = (min(g.per, g.units - (int)blockIdx.x * g.per) + G - 1) / G;  // groups of G units
-  const int chunks = p.w.chunks, nseg = (chunks + g.seg - 1) / g.seg;
-  const uint8_t *codes = p.w.codes + e * mx_code_bytes(p.w), *scales = p.w.scales + e * mx_scale_bytes(p.w);
-  const int l16 = lane & 15, q = lane >> 4;
+  const int chunks = p.w.chunks, c0 = chunks * wave / kWaves, nc = chunks * (wave + 1) / kWaves - c0;
+  const __amdgpu_buffer_rsrc_t rx = plane_rsrc(static_cast<const uint8_t *>(p.x), g.x_bytes);
+  const __amdgpu_buffer_rsrc_t rxs = plane_rsrc(p.xscales, XM == 0 ? (int64_t)p.x_rows * chunks * 4 : 0);
+  const int u0 = blockIdx.x * g.per, u1 = min(u0 + g.per, g.units);
 
-  for (int r0 = r_lo; r0 < r_hi; r0 += g.rows) {
-    const int m = min(g.rows, r_hi - r0), V = m * P, nct = (V + 15) / 16;
-    // The wave's chunks of segment sg: [lo, hi), as places in the segment.
-    auto range = [&](int sg, int &lo, int &hi) {
-      const int n = min(g.seg, chunks - sg * g.seg);
-      lo = n * part >> g.kshift;
-      hi = n * (part + 1) >> g.kshift;
-    };
-    // Loads run kAhead chunks ahead of the products, over segments and units.
-    // Each run of chunks starts at the ring's first slot; the slots past its
-    // end load nothing (a buffer of no bytes).
-    int fu = u0, fs = 0, fi, fhi;
-    range(0, fi, fhi);
-    int fleft = max((fhi - fi + kAhead - 1) / kAhead * kAhead, kAhead);
-    auto fetch = [&](Fetch<WF, NT> &f) {
-      const bool real = fu < u_end && fi < fhi;
-      const int tile = (real ? fu : 0) * NT, c = real ? fs * g.seg + fi : 0;
+  // A unit's part of this wave; chunks past it read zeros (an offset past the buffer).
+  struct Tile {
+    uint4 w[NC][NT][WF == FMT_MXFP4 ? 1 : 2];
+    uint32_t s[NC];  // the scale quad's words
+  };
+  const __amdgpu_buffer_rsrc_t rw = plane_rsrc(p.w.codes + e * mx_code_bytes(p.w), mx_code_bytes(p.w));
+  const __amdgpu_buffer_rsrc_t rs = plane_rsrc(p.w.scales + e * mx_scale_bytes(p.w), mx_scale_bytes(p.w));
+  auto fetch = [&](Tile &f, int u, int i) {
+    const bool real = u < u1 && i < nc;
+    const int tile = real ? u * NT : 0, c = real ? c0 + i : 0;
+    const uint32_t at = (uint32_t)mx_tile_at(p.w, tile, c), sat = (uint32_t)mx_quad_at(p.w, tile, c);
 #pragma unroll
-      for (int t = 0; t < NT; t++) {
-        const __amdgpu_buffer_rsrc_t r =
-            plane_rsrc(codes + mx_tile_at(p.w, tile + t, c), real ? mx_chunk_bytes(WF) : 0);
+    for (int t = 0; t < NT; t++)
 #pragma unroll
-        for (int j = 0; j < (WF == FMT_BF16 ? 2 : 1); j++) {
-          const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(r, lane * 16 + j * 1024, 0, 0);
-          f.t[t].w[j] = make_uint4(v.x, v.y, v.z, v.w);
-        }
-      }
-      if constexpr (WF == FMT_MXFP4)
-        f.s = __builtin_amdgcn_raw_buffer_load_b32(plane_rsrc(scales + mx_quad_at(p.w, tile, c), real ? 256 : 0),
-                                                   lane * 4, 0, 0);
-      fi++;
-      if (--fleft == 0) {
-        if (++fs == nseg) fs = 0, fu += G;
-        range(fs, fi, fhi);
-        fleft = max((fhi - fi + kAhead - 1) / kAhead * kAhead, kAhead);
-      }
-    };
-    Fetch<WF, NT> ring[kAhead];
-    auto prime = [&]() {
-#pragma unroll
-      for (int i = 0; i < kAhead; i++) fetch(ring[i]);
-    };
+      for (int j = 0; j < (WF == FMT_BF16 ? 2 : 1); j++)
+        f.w[i][t][j] = load16(rw, real ? at + t * mx_chunk_bytes(WF) + j * 1024 + lane * 16 : kNone);
+    if constexpr (WF == FMT_MXFP4)
+      f.s[i] = __builtin_amdgcn_raw_buffer_load_b32(rs, real ? (int)(sat + lane * 4) : (int)kNone, 0, 0);
+  };
 
-    for (int ps = 0; ps < passes; ps++) {
-      const int u = u0 + ps * G;
-      f32x4 acc[NT][kCols];
+  for (int r0 = r_lo; r0 < r_hi; r0 += kRows) {
+    const int m = min(kRows, r_hi - r0);
+    Tile a;
 #pragma unroll
-      for (int t = 0; t < NT; t++)
+    for (int i = 0; i < NC; i++) fetch(a, u0, i);
+    __builtin_amdgcn_sched_barrier(0);
+    // X: operand column v = plane * m + row of column tile v / 16; columns
+    // past the planes, and rows that the index does not name, are zeros.
+    uint4 x[NC][CT][XM == 0 ? 1 : NJ];
+    uint32_t xs[XM == 0 ? NC : 1][CT];
+    auto source = [&](int r) {  // the row of X, or -1
+      const int src = p.index ? p.index[r0 + r] : r0 + r;
+      return src < p.x_rows ? src : -1;
+    };
+    if constexpr (XM <= 1) {  // as they are stored
 #pragma unroll
-        for (int c = 0; c < kCols; c++) acc[t][c] = f32x4{0.f, 0.f, 0.f, 0.f};
-      for (int sg = 0; sg < nseg; sg++) {
-        if (nseg > 1 || ps == 0) {  // X's columns of the segment into LDS
-          __syncthreads();
-          const int k0 = sg * g.seg * kUnitCols, count = min(g.seg, chunks - sg * g.seg) * kUnitCols;
-          stage_few<WF, XM, kT>(p, lds, r0, m, V, k0, count, g.seg, tid, [&]() {
-            if (ps + sg == 0) prime();  // the ring's first loads behind X's
-          });
-          __syncthreads();
-        }
-        int lo, hi;
-        range(sg, lo, hi);
-        const bool mine = u < u_end;
-        const int shift = 8 * ((u * NT) & 3);  // this tile's byte of the scale words
-        auto consume = [&](const Fetch<WF, NT> &f, int c) {
-          const uint32_t fs = f.s >> shift;
-          const uint8_t *xs = lds + (size_t)c * V * (XM == 0 ? 64 : kUnitCols * 2);
-          if constexpr (XM == 0) {  // both operands MXFP4
-            const uint32_t *ss = reinterpret_cast<const uint32_t *>(lds + (size_t)g.seg * V * 64) + c * V;
+      for (int ct = 0; ct < CT; ct++) {
+        const int v = ct * 16 + l16, src = v < m ? source(v) : -1;
 #pragma unroll
-            for (int ct = 0; ct < kCols; ct++) {
-              if (ct >= nct) break;
-              const int v = min(ct * 16 + l16, V - 1);
-              const uint4 x = *reinterpret_cast<const uint4 *>(xs + v * 64 + ((q ^ ((v >> 2) & 3)) << 4));
-              const uint32_t sx = ss[v] >> (8 * q);
-              acc[0][ct] = mfma_mx<0>(f.t[0].w[0], x, acc[0][ct], fs, sx);
-              if constexpr (GATE) acc[1][ct] = mfma_mx<1>(f.t[1].w[0], x, acc[1][ct], fs, sx);
-            }
+        for (int i = 0; i < NC; i++) {
+          const bool in = src >= 0 && i < nc;
+          if constexpr (XM == 0) {
+            const uint32_t at = (uint32_t)(c0 + i) * (uint32_t)p.x_rows + (uint32_t)src;
+            x[i][ct][0] = load16(rx, in ? at * 64 + q * 16 : kNone);
+            xs[i][ct] = __builtin_amdgcn_raw_buffer_load_b32(rxs, in ? (int)(at * 4) : (int)kNone, 0, 0);
           } else {
-            constexpr int NJ = WF == FMT_MXFP4 ? 4 : 2;
-            uint4 w[NT][NJ];
 #pragma unroll
-            for (int t = 0; t < NT; t++) {
-              if constexpr (WF == FMT_BF16) {
-                w[t][0] = f.t[t].w[0];
-                w[t][1] = f.t[t].w[1];
-              } else {
-                // the scale's byte in the exponent's place; the conversion takes no other bit of it
-                const float sc = __uint_as_float(t ? fs << 15 : fs << 23);
-                w[t][0] = fp4_bf16(f.t[t].w[0].x, sc);
-                w[t][1] = fp4_bf16(f.t[t].w[0].y, sc);
-                w[t][2] = fp4_bf16(f.t[t].w[0].z, sc);
-                w[t][3] = fp4_bf16(f.t[t].w[0].w, sc);
-              }
-            }
-#pragma unroll
-            for (int ct = 0; ct < kCols; ct++) {
-              if (ct >= nct) break;
-              const int v = min(ct * 16 + l16, V - 1);
-#pragma unroll
-              for (int j = 0; j < NJ; j++) {
-                const uint4 x = *reinterpret_cast<const uint4 *>(xs + few_x_at<WF>(v, NJ * q + j));
-#pragma unroll
-                for (int t = 0; t < NT; t++) acc[t][ct] = mfma_bf16(w[t][j], x, acc[t][ct]);
-              }
+            for (int j = 0; j < NJ; j++) {
+              const int k = (c0 + i) * kChunk + (NJ * q + j) * 8;
+              x[i][ct][j] = load16(rx, in && k < p.w.cols ? (uint32_t)src * (uint32_t)(p.ldx * 2) + k * 2 : kNone);
             }
           }
-        };
-        int c = lo;
-        do {
-#pragma unroll
-          for (int i = 0; i < kAhead; i++) {
-            if (mine && c + i < hi) consume(ring[i], c + i);
-            fetch(ring[i]);
-          }
-          c += kAhead;
-        } while (c < hi);
+        }
       }
-      // [wave][tile][virtual column][16 matrix rows], in the LDS past X
-      float *red = reinterpret_cast<float *>(lds + few_x_bytes<WF, XM>(g.seg, V));
-      const int V16 = nct * 16;
-      if (ps) __syncthreads();
+    } else {
+      // The wave's columns of the rows, four values a lane, cut into planes
+      // and through its part of LDS into the operand's places.
+      constexpr int kQuads = kChunk / 4, kItems = (kRows * kQuads + 63) / 64, kBytes = XM == 3 ? 4 : 2;
+      uint8_t *mine = reinterpret_cast<uint8_t *>(red) + wave * (CT * 16 * kChunk * 2);
+      uint32_t raw[NC][kItems][XM == 3 ? 4 : 2];
+#pragma unroll
+      for (int it = 0; it < kItems; it++) {
+        const int item = it * 64 + lane, r = item / kQuads, src = r < m ? source(r) : -1;
+#pragma unroll
+        for (int i = 0; i < NC; i++) {
+          const int k = (c0 + i) * kChunk + item % kQuads * 4;
+          const uint32_t at = src >= 0 && i < nc && k < p.w.cols ? ((uint32_t)src * (uint32_t)p.ldx + k) * kBytes : kNone;
+          if constexpr (XM == 3) {
+            const uint4 w = load16(rx, at);
+            raw[i][it][0] = w.x, raw[i][it][1] = w.y, raw[i][it][2] = w.z, raw[i][it][3] = w.w;
+          } else {
+            const u32x2 w = __builtin_amdgcn_raw_buffer_load_b64(rx, (int)at, 0, 0);
+            raw[i][it][0] = w.x, raw[i][it][1] = w.y;
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < NC; i++) {
+        if (i >= nc) {
+#pragma unroll
+          for (int ct = 0; ct < CT; ct++)
+#pragma unroll
+            for (int j = 0; j < NJ; j++) x[i][ct][j] = make_uint4(0, 0, 0, 0);
+          continue;
+        }
+#pragma unroll
+        for (int it = 0; it < kItems; it++) {
+          if (it * 64 >= m * kQuads) break;
+          const int item = it * 64 + lane, r = item / kQuads, c = item % kQuads;
+          uint32_t h[4][P];
+#pragma unroll
+          for (int j = 0; j < 4; j++)
+            planes_of<P>(XM == 3 ? __uint_as_float(raw[i][it][j & (XM == 3 ? 3 : 1)])
+                                 : hw_half((uint16_t)(raw[i][it][j / 2] >> (16 * (j & 1)))), h[j]);
+          if (r < m)
+#pragma unroll
+            for (int pl = 0; pl < P; pl++)
+              *reinterpret_cast<uint2 *>(mine + few_x_at<WF>(pl * m + r, c / 2) + (c & 1) * 8) =
+                  make_uint2(high_halves(h[0][pl], h[1][pl]), high_halves(h[2][pl], h[3][pl]));
+        }
+        wave_sync();
+#pragma unroll
+        for (int ct = 0; ct < CT; ct++) {
+          const int v = ct * 16 + l16;
+#pragma unroll
+          for (int j = 0; j < NJ; j++) {
+            x[i][ct][j] = *reinterpret_cast<const uint4 *>(mine + few_x_at<WF>(v, NJ * q + j));
+            if (v >= m * P) x[i][ct][j] = make_uint4(0, 0, 0, 0);
+          }
+        }
+        wave_sync();
+      }
+      __syncthreads();  // the sums take this LDS
+    }
+    if constexpr (XM == 0) {
+#pragma unroll
+      for (int i = 0; i < NC; i++)
+#pragma unroll
+        for (int ct = 0; ct < CT; ct++) xs[i][ct] >>= 8 * q;
+    }
+
+    auto unit = [&](Tile &f, int u, int buf) {
+      f32x4 acc[NT][CT];
 #pragma unroll
       for (int t = 0; t < NT; t++)
 #pragma unroll
-        for (int ct = 0; ct < kCols; ct++)
-          if (ct < nct)
-            *reinterpret_cast<f32x4 *>(red + ((wave * NT + t) * V16 + ct * 16 + l16) * 16 + 4 * q) = acc[t][ct];
-      __syncthreads();
-      for (int i = tid; i < G * m * 16; i += kT) {
-        const int o = i & 15, r = (i >> 4) % m, gu = (i >> 4) / m;
-        const int unit = blockIdx.x * g.per + ps * G + gu, out = unit * 16 + o;
-        if (unit >= u_end || out >= p.w.rows) continue;
+        for (int ct = 0; ct < CT; ct++) acc[t][ct] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < NC; i++) {
+        if (i >= nc) break;
+        __builtin_amdgcn_sched_barrier(0);
+        const uint32_t s = f.s[i] >> (8 * ((u * NT) & 3));  // this tile's byte (and the next one's above it)
+        if constexpr (XM == 0) {
+#pragma unroll
+          for (int ct = 0; ct < CT; ct++) {
+            acc[0][ct] = mfma_mx<0>(f.w[i][0][0], x[i][ct][0], acc[0][ct], s, xs[i][ct]);
+            if constexpr (GATE) acc[1][ct] = mfma_mx<1>(f.w[i][1][0], x[i][ct][0], acc[1][ct], s, xs[i][ct]);
+          }
+        } else {
+#pragma unroll
+          for (int t = 0; t < NT; t++) {
+            uint4 w[NJ];
+            if constexpr (WF == FMT_BF16) {
+              w[0] = f.w[i][t][0];
+              w[1] = f.w[i][t][1];
+            } else {
+              // the scale's byte in the exponent's place; the conversion takes no other bit of it
+              const float sc = __uint_as_float(t ? s << 15 : s << 23);
+              w[0] = fp4_bf16(f.w[i][t][0].x, sc);
+              w[1] = fp4_bf16(f.w[i][t][0].y, sc);
+              w[2] = fp4_bf16(f.w[i][t][0].z, sc);
+              w[3] = fp4_bf16(f.w[i][t][0].w, sc);
+            }
+#pragma unroll
+            for (int j = 0; j < NJ; j++)
+#pragma unroll
+              for (int ct = 0; ct < CT; ct++) acc[t][ct] = mfma_bf16(w[j], x[i][ct][j], acc[t][ct]);
+          }
+        }
+        fetch(f, u + 1, i);
+      }
+      // [wave][tile][operand column][16 matrix rows]
+#pragma unroll
+      for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int ct = 0; ct < CT; ct++)
+          *reinterpret_cast<f32x4 *>(&red[buf][((wave * NT + t) * CT + ct) * 256 + l16 * 16 + 4 * q]) = acc[t][ct];
+    };
+    auto finish = [&](int u, int buf) {  // the waves' and planes' sums of the unit
+      for (int i = tid; i < m * 16; i += kT) {
+        const int o = i & 15, r = i >> 4, out = u * 16 + o;
+        if (out >= p.w.rows) continue;
         float v[NT];
 #pragma unroll
         for (int t = 0; t < NT; t++) {
           v[t] = 0.f;
-          for (int s = 0; s < g.ksplit; s++)
 #pragma unroll
-            for (int pl = P - 1; pl >= 0; pl--)  // the smallest first
-              v[t] += red[(((gu * g.ksplit + s) * NT + t) * V16 + pl * m + r) * 16 + o];
+          for (int pl = P - 1; pl >= 0; pl--)  // the smallest first
+#pragma unroll
+            for (int w = 0; w < kWaves; w++) v[t] += red[buf][(w * NT + t) * CT * 256 + (pl * m + r) * 16 + o];
         }
         float y = GATE ? mx_gate(v[0], v[NT - 1]) : v[0];
         if (p.index) {
           const int src = p.index[r0 + r];
-          if (src < 0 || src >= p.x_rows) y = 0.f;
+          if (src < 0 || src >= p.x_rows) y = 0.f;  // whatever the matrix holds
         }
         mx_store(p.odtype, p.out, (int64_t)(r0 + r) * p.ldo + out, y);
       }
+    };
+    // (the sums' buffer of two units ago is free once every wave is past the
+    // barrier of the unit between)
+    for (int u = u0; u < u1; u++) {
+      unit(a, u, u & 1);
+      __syncthreads();
+      finish(u, u & 1);
     }
-    __syncthreads();
+    if (r0 + kRows < r_hi) __syncthreads();
   }
 }
 
-template <int WF, int XM, bool GATE>
-hipError_t launch(FewArgs &g, int active, hipStream_t st) {
-  constexpr int P = XM == 0 ? 1 : XM;
-  constexpr size_t kLds = 160 * 1024;
+int groups(const MxProduct &p) { return p.offsets ? std::min(p.w.experts, p.n) : 1; }
+
+int64_t x_bytes(const MxProduct &p) {
+  if (p.xdtype == FMT_MXFP4) return (int64_t)p.x_rows * p.w.chunks * 64;
+  return ((int64_t)(p.x_rows - 1) * p.ldx + p.w.cols) * (int64_t)mx_width(p.xdtype);
+}
+
+template <int WF, int XM, bool GATE, int kWaves, int CT>
+hipError_t launch(FewArgs &g, hipStream_t st) {
   const MxProduct &p = g.p;
-  const int cus = device_cu_count();
   g.units = (p.w.rows + 15) / 16;
-  // Enough waves for the chip: a unit's columns go to more of them where units are few.
-  g.ksplit = 1;
-  while (g.ksplit < 8 && (int64_t)active * g.units * g.ksplit < (int64_t)cus * 12 && p.w.chunks >= 2 * g.ksplit) g.ksplit *= 2;
-  g.kshift = g.ksplit == 8 ? 3 : g.ksplit / 2;
-  const int G = kWaves / g.ksplit;
-  const int64_t blocks = (int64_t)active * ((g.units + G - 1) / G);
-  const int runs = (int)std::max<int64_t>(1, std::min<int64_t>(blocks / (cus * 2), 16));
-  g.per = G * runs;
-  const int most = p.offsets ? p.n : std::min(p.n, 16 * kCols / P);
-  g.rows = std::min(16 * kCols / P, most);
-  const int V = g.rows * P, V16 = (V + 15) / 16 * 16;
-  const size_t red = (size_t)kWaves * (GATE ? 2 : 1) * V16 * 64;
-  g.seg = p.w.chunks;
-  while (few_x_bytes<WF, XM>(g.seg, V) + red > kLds) g.seg = (g.seg + 1) / 2;
-  const size_t bytes = few_x_bytes<WF, XM>(g.seg, V) + red;
-  static bool set = false;
-  if (!set) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&few_kernel<WF, XM, GATE>),
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)kLds);
-    if (e != hipSuccess) return e;
-    set = true;
-  }
-  hipLaunchKernelGGL((few_kernel<WF, XM, GATE>), dim3((g.units + g.per - 1) / g.per, p.offsets ? p.w.experts : 1), dim3(kT),
-                     bytes, st, g);
+  // A block a CU, each with units of its own (two in turn would both bring X:
+  // 6912 x 2560 MXFP4 times an fp32 row 8.9 us instead of 6.0); two with MXFP4
+  // rows of groups, which cost little and are uneven (16 tokens' gate and up of
+  // 32 experts 21.9 us instead of 23.6).
+  const int64_t blocks = (int64_t)device_cu_count() * (XM == 0 && p.offsets ? 2 : 1);
+  g.per = (int)std::max<int64_t>(1, ((int64_t)groups(p) * g.units + blocks - 1) / blocks);
+  hipLaunchKernelGGL((few_kernel<WF, XM, GATE, kWaves, CT>), dim3((g.units + g.per - 1) / g.per, p.offsets ? p.w.experts : 1),
+                     dim3(kWaves * 64), 0, st, g);
   return hipGetLastError();
 }
 
 }  // namespace
 
-// Whether the few-row kernel takes the product: its rows fill no more than
-// kCols column tiles.
+// Whether the few-row kernel takes the product: its rows fill one or two
+// column tiles (one, with sixteen waves), its columns no more than four chunks
+// of sixteen waves (pairs and planes: of eight, or registers spill), X comes in
+// whole 16-byte pieces, and offsets within X and a matrix fit 31 bits.
 bool mx_few_supported(const MxProduct &p) {
-  const int planes = mx_planes(p.xdtype);
-  const int active = p.offsets ? std::min(p.w.experts, p.n) : 1;
-  return (int64_t)p.n * planes <= (int64_t)active * 16 * kCols;
+  const bool pieces = p.xdtype == FMT_MXFP4 || (p.w.cols % 8 == 0 && p.ldx * mx_width(p.xdtype) % 16 == 0 &&
+                                                reinterpret_cast<uintptr_t>(p.x) % 16 == 0);
+  const int waves = p.w.gate && p.xdtype != FMT_MXFP4 ? 8 : 16;
+  return p.w.chunks <= waves * NC && pieces && x_bytes(p) < kNone && mx_code_bytes(p.w) < kNone &&
+         (int64_t)p.n * mx_planes(p.xdtype) <= (int64_t)groups(p) * (p.w.chunks <= 8 * NC ? 32 : 16);
 }
 
 hipError_t launch_mx_few(const MxProduct &p, hipStream_t st) {
   FewArgs g{p};
-  const int active = p.offsets ? std::min(p.w.experts, p.n) : 1;
+  g.x_bytes = x_bytes(p);
+  // column tiles: one for a dense product of few rows; groups are uneven
+  const bool two = (int64_t)p.n * mx_planes(p.xdtype) > (p.offsets ? 4 : 16) * (int64_t)groups(p);
   auto go = [&](auto wf, auto xm) {
     constexpr int WF = decltype(wf)::value, XM = decltype(xm)::value;
-    return p.w.gate ? launch<WF, XM, true>(g, active, st) : launch<WF, XM, false>(g, active, st);
+    if (p.w.chunks > 8 * NC) {
+      if constexpr (XM == 0)
+        if (p.w.gate) return launch<WF, XM, true, 16, 1>(g, st);
+      return launch<WF, XM, false, 16, 1>(g, st);
+    }
+    if (two) return p.w.gate ? launch<WF, XM, true, 8, 2>(g, st) : launch<WF, XM, false, 8, 2>(g, st);
+    return p.w.gate ? launch<WF, XM, true, 8, 1>(g, st) : launch<WF, XM, false, 8, 1>(g, st);
   };
   using std::integral_constant;
   const int xm = p.xdtype == FMT_MXFP4 ? 0 : mx_planes(p.xdtype);

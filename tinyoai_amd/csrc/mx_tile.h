@@ -117,62 +117,4 @@ template <int WF>
 __device__ __forceinline__ int few_x_at(int v, int c) {
   return WF == FMT_MXFP4 ? v * 256 + ((c ^ (v & 15)) << 4) : v * 128 + ((c ^ ((v >> 1) & 7)) << 4);
 }
-template <int WF, int XM>
-__host__ __device__ inline size_t few_x_bytes(int chunks, int V) {
-  return ((size_t)chunks * V * (XM == 0 ? 68 : mx_cols<WF>() * 2) + 15) / 16 * 16;
-}
-
-// X's columns [k0, k0 + count) of rows r0 .. r0 + m - 1 into LDS: virtual
-// column plane * m + row. MXFP4 rows: per chunk and row 64 code bytes, then
-// all the scale words (`seg` chunks at most). `between` is called once, after
-// the first loads are issued: what it loads is not waited for here.
-template <int WF, int XM, int T, typename Between>
-__device__ __forceinline__ void stage_few(const MxProduct &p, uint8_t *lds, int r0, int m, int V, int k0, int count, int seg,
-                                          int tid, const Between &between) {
-  constexpr int XT = XM == 3 ? FMT_F32 : XM == 2 ? FMT_F16 : FMT_BF16, B = 4;  // items a thread loads together
-  const int pieces = XM == 0 ? count / 32 : count / 8;  // 16-byte pieces of a row
-  const int items = m * pieces;
-  for (int i0 = 0; i0 < items; i0 += B * T) {
-    Raw8<XT> raw[B];
-    uint32_t sc[B];
-    int64_t src[B];
-#pragma unroll
-    for (int b = 0; b < B; b++) {
-      const int i = i0 + b * T + tid, r = r0 + min(i / pieces, m - 1);
-      src[b] = p.index ? p.index[r] : r;
-    }
-#pragma unroll
-    for (int b = 0; b < B; b++) {
-      const int i = i0 + b * T + tid, c = i % pieces;
-      memset(&raw[b], 0, sizeof raw[b]);
-      sc[b] = 0;
-      if (i >= items || src[b] < 0 || src[b] >= p.x_rows) continue;
-      if constexpr (XM == 0) {
-        const int64_t at = (int64_t)(k0 / 128 + c / 4) * p.x_rows + src[b];
-        raw[b].a[0] = *reinterpret_cast<const uint4 *>(static_cast<const uint8_t *>(p.x) + at * 64 + (c & 3) * 16);
-        if ((c & 3) == 0) sc[b] = reinterpret_cast<const uint32_t *>(p.xscales)[at];
-      } else {
-        raw[b] = load_x8<XT>(p, src[b], k0 + c * 8);
-      }
-    }
-    if (i0 == 0) between();
-#pragma unroll
-    for (int b = 0; b < B; b++) {
-      const int i = i0 + b * T + tid, r = i / pieces, c = i - r * pieces;
-      if (i >= items) break;
-      if constexpr (XM == 0) {
-        *reinterpret_cast<uint4 *>(lds + ((size_t)(c >> 2) * V + r) * 64 + (((c & 3) ^ ((r >> 2) & 3)) << 4)) = raw[b].a[0];
-        if ((c & 3) == 0) reinterpret_cast<uint32_t *>(lds + (size_t)seg * V * 64)[(c >> 2) * V + r] = sc[b];
-      } else {
-        uint4 h[XM];
-        planes8<XT>(raw[b], h);
-        constexpr int per = mx_cols<WF>() / 8;
-        uint8_t *base = lds + (size_t)(c / per) * V * (mx_cols<WF>() * 2);
-#pragma unroll
-        for (int pl = 0; pl < XM; pl++) *reinterpret_cast<uint4 *>(base + few_x_at<WF>(pl * m + r, c % per)) = h[pl];
-      }
-    }
-  }
-}
-
 }  // namespace tinyoai_mx
