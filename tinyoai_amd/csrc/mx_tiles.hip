@@ -50,15 +50,18 @@ struct Shape {
   static constexpr bool Q = XM == 0;
   static constexpr int P = Q ? 1 : XM;
   static constexpr int kCols = Q ? 128 : 64;                                     // columns of a step
-  static constexpr int kX = BM * (Q ? 64 : 128), kXS = Q ? BM * 4 : 0;           // bytes of a plane, of the scale words
+  static constexpr int kX = BM * (Q ? 64 : 128);                                 // bytes of a plane
+  static constexpr int kXS = !Q ? 0 : BM < 64 ? 256 : BM * 4;                    // of the scale words
   static constexpr int kW = BN / 16 * (Q ? 1024 : WF == FMT_BF16 ? 2048 : 512);  // of the codes
   static constexpr int kWS = WF == FMT_MXFP4 ? BN / 64 * 256 : 0;
   static constexpr int kStage = P * kX + kXS + kW + kWS;
-  // wave loads of a step
-  static constexpr int kAll = WAVES * 1024;  // bytes of a load of every wave
-  static constexpr int NX = kX / kAll, NXS = Q ? 1 : 0, NW = kW / kAll, NWS = WF == FMT_MXFP4 ? 1 : 0;
+  // A step's loads of 1 KB, and how many of them a wave makes (every wave the
+  // same number: where there are fewer, some repeat others')
+  static constexpr int LX = kX / 1024, LW = kW / 1024, LXS = kXS / 256, LWS = BN / 64;
+  static constexpr int NX = (LX + WAVES - 1) / WAVES, NXS = Q ? 1 : 0, NW = (LW + WAVES - 1) / WAVES, NWS = WF == FMT_MXFP4 ? 1 : 0;
   static constexpr int kLoads = P * NX + NXS + NW + NWS;
-  static_assert(kX % kAll == 0 && kW % kAll == 0 && BN % 64 == 0 && BN <= 256, "whole loads of every wave");
+  static_assert((LX % WAVES == 0 || WAVES % LX == 0) && (LW % WAVES == 0 || WAVES % LW == 0), "loads of every wave");
+  static_assert(BN % 64 == 0 && BN <= 256 && LXS <= WAVES && LWS <= WAVES, "whole scale quads");
 };
 
 // This block's group and first row, from its number among all row tiles;
@@ -123,7 +126,7 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 ? 2 : 1) void tile_kernel(Ti
   using S = Shape<WF, XM, BM, BN, WAVES>;
   constexpr bool Q = S::Q;
   constexpr int P = S::P, WN = WAVES / WM, MF = BM / 32 / WM, NF = BN / 32 / WN;
-  static_assert(MF * WM * 32 == BM && NF * WN * 32 == BN && NF % 2 == 0, "whole scale quads a wave");
+  static_assert(MF * WM * 32 == BM && NF * WN * 32 == BN && (NF % 2 == 0 || NF == 1), "scale quads");
   extern __shared__ __align__(16) uint8_t lds[];
   const MxProduct &p = g.p;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -171,53 +174,61 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 ? 2 : 1) void tile_kernel(Ti
   uint32_t xoff[S::NX], woff[S::NW], xsoff = kNone, wsoff = kNone;
 #pragma unroll
   for (int i = 0; i < S::NX; i++) {
-    const int row = (wave + WAVES * i) * (Q ? 16 : 8) + (Q ? lane >> 2 : lane >> 3);
+    const int row = (wave + WAVES * i) % S::LX * (Q ? 16 : 8) + (Q ? lane >> 2 : lane >> 3);
     const uint32_t piece = Q ? (lane & 3) ^ ((row >> 2) & 3) : (lane & 7) ^ ((row >> 1) & 7);
     const uint32_t src = source(row);
     xoff[i] = src == kNone ? kNone : src * (uint32_t)xld + piece * 16;
   }
-  if constexpr (Q) {  // (waves past BM / 64 repeat the others' loads)
-    const uint32_t src = source((wave % (BM / 64)) * 64 + lane);
+  if constexpr (Q) {
+    const uint32_t src = source((wave % S::LXS) * 64 + lane);
     xsoff = src == kNone ? kNone : src * 4;
   }
 #pragma unroll
   for (int i = 0; i < S::NW; i++) {
-    const int piece = (wave + WAVES * i) * 64 + lane;  // of 16 bytes
+    const int piece = (wave + WAVES * i) % S::LW * 64 + lane;  // of 16 bytes
     constexpr int per = Q ? 64 : WF == FMT_BF16 ? 128 : 32;  // pieces of a tile's step
     woff[i] = piece / per < wtiles ? (uint32_t)(piece / per) * CB + (uint32_t)(piece % per) * 16 : kNone;
   }
   if constexpr (WF == FMT_MXFP4)
-    if (wave % (BN / 64) < wtiles / 4) wsoff = (uint32_t)(wave % (BN / 64)) * 256 + lane * 4;
+    if (wave % S::LWS < wtiles / 4) wsoff = (uint32_t)(wave % S::LWS) * 256 + lane * 4;
 
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void *)lds;
   constexpr uint32_t kXS0 = P * S::kX, kW0 = kXS0 + S::kXS, kWS0 = kW0 + S::kW;
   auto issue = [&](int kb, int slot) {
     const bool in = kb < steps;
-    const uint32_t base = lds0 + slot * S::kStage, mine = base + wave * 1024;
+    const uint32_t base = lds0 + slot * S::kStage;
     const uint32_t kx = in ? (uint32_t)kb * (uint32_t)xunit : kPast;
 #pragma unroll
     for (int i = 0; i < P; i++)
 #pragma unroll
-      for (int j = 0; j < S::NX; j++) lds_dma16(rx[i], xoff[j] + kx, mine + i * S::kX + j * S::kAll);
-    if constexpr (Q) lds_dma4(rxs, xsoff + (in ? (uint32_t)kb * (uint32_t)(p.x_rows * 4) : kPast), base + kXS0 + (wave % (BM / 64)) * 256);
+      for (int j = 0; j < S::NX; j++) lds_dma16(rx[i], xoff[j] + kx, base + i * S::kX + (wave + WAVES * j) % S::LX * 1024);
+    if constexpr (Q) lds_dma4(rxs, xsoff + (in ? (uint32_t)kb * (uint32_t)(p.x_rows * 4) : kPast), base + kXS0 + wave % S::LXS * 256);
     constexpr bool kHalf = WF == FMT_MXFP4 && !Q;  // a step is half a chunk
     const uint32_t chunk = kHalf ? kb >> 1 : kb;
     const uint32_t kw = in ? chunk * (uint32_t)(gt * CB) + (kHalf ? (kb & 1) * 512 : 0) : kPast;
 #pragma unroll
-    for (int j = 0; j < S::NW; j++) lds_dma16(rw, woff[j] + kw, mine + kW0 + j * S::kAll);
+    for (int j = 0; j < S::NW; j++) lds_dma16(rw, woff[j] + kw, base + kW0 + (wave + WAVES * j) % S::LW * 1024);
     if constexpr (WF == FMT_MXFP4)
-      lds_dma4(rws, wsoff + (in ? chunk * (uint32_t)(gt * 64) : kPast), base + kWS0 + (wave % (BN / 64)) * 256);
+      lds_dma4(rws, wsoff + (in ? chunk * (uint32_t)(gt * 64) : kPast), base + kWS0 + wave % S::LWS * 256);
   };
 
-  f32x16 acc[MF][NF];
+  // (a single tile has four sums, added at the end: each product would wait
+  // for the one before)
+  constexpr int NA = MF * NF == 1 ? 4 : 1;
+  f32x16 acc[MF][NF], more[NA];
 #pragma unroll
-  for (int f = 0; f < MF; f++)
+  for (int v = 0; v < 16; v++) {
 #pragma unroll
-    for (int n = 0; n < NF; n++)
+    for (int f = 0; f < MF; f++)
 #pragma unroll
-      for (int v = 0; v < 16; v++) acc[f][n][v] = 0.f;
+      for (int n = 0; n < NF; n++) acc[f][n][v] = 0.f;
+#pragma unroll
+    for (int a = 0; a < NA; a++) more[a][v] = 0.f;
+  }
   const int xr = wm * MF * 32 + l32;            // this lane's row of the wave's first row tile
   const int wt = (lane & 31) >> 4, l16 = lane & 15;  // its matrix row: of the pair's tile wt, row l16
+  const int mine = 8 * wt + (NF == 1 ? 16 * (wn & 1) : 0);  // where a scale word has the byte of this lane's row in tile 0
+
   // A step's operands go through registers in two halves, each read from LDS
   // while the products of the half before it run: a wave meets the barrier
   // between them, so neither it nor the reads leave the matrix cores waiting.
@@ -225,7 +236,7 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 ? 2 : 1) void tile_kernel(Ti
     uint4 x[MF][P][Q ? 1 : 2];
     uint4 w[WF == FMT_BF16 || Q ? NF : 1][Q ? 1 : 2];
     uint2 c[WF == FMT_MXFP4 && !Q ? NF : 1];  // codes
-    uint32_t sw[NF / 2], sx[Q ? MF : 1];
+    uint32_t sw[(NF + 1) / 2], sx[Q ? MF : 1];
   };
   auto read = [&](Half &H, int kb, int slot, int b) {
     const uint8_t *st = lds + slot * S::kStage;
@@ -257,7 +268,7 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 ? 2 : 1) void tile_kernel(Ti
     }
     if constexpr (WF == FMT_MXFP4)
 #pragma unroll
-      for (int n = 0; n < NF / 2; n++)  // the word of four tiles' scales of this row and block
+      for (int n = 0; n < (NF + 1) / 2; n++)  // the word of four tiles' scales of this row and block
         H.sw[n] = *reinterpret_cast<const uint32_t *>(st + kWS0 + (wn * NF / 2 + n) * 256 +
                                                       ((Q ? 2 * b + h : (kb & 1) * 2 + b) * 16 + l16) * 4);
   };
@@ -266,12 +277,14 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 ? 2 : 1) void tile_kernel(Ti
     if constexpr (Q) {
 #pragma unroll
       for (int n = 0; n < NF; n += 2) {
-        const uint32_t sw = H.sw[n / 2] >> (8 * wt);  // bytes 0 and 2: the pair's two tiles of this lane's row
+        const uint32_t sw = H.sw[n / 2] >> mine;  // bytes 0 and 2: the tile of this lane's row of tiles n and n + 1
 #pragma unroll
         for (int f = 0; f < MF; f++) {
           const uint32_t sx = H.sx[f] >> (8 * h);  // bytes 0 and 2: blocks h, 2 + h
-          acc[f][n] = mfma_mx_32<0, 2 * b>(H.w[n][0], H.x[f][0][0], acc[f][n], sw, sx);
-          acc[f][n + 1] = mfma_mx_32<2, 2 * b>(H.w[n + 1][0], H.x[f][0][0], acc[f][n + 1], sw, sx);
+          f32x16 &to = NA > 1 ? more[b] : acc[f][n];
+          to = mfma_mx_32<0, 2 * b>(H.w[n][0], H.x[f][0][0], to, sw, sx);
+          if constexpr (NF > 1)
+            acc[f][n + 1] = mfma_mx_32<2, 2 * b>(H.w[n + 1][0], H.x[f][0][0], acc[f][n + 1], sw, sx);
         }
       }
     } else {
@@ -283,7 +296,7 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 ? 2 : 1) void tile_kernel(Ti
           w[n][1] = H.w[n][1];
         } else {
           // the tile's scale byte in an exponent's place; the conversion takes no other bit
-          const uint32_t sw = H.sw[n / 2] >> (8 * wt);
+          const uint32_t sw = H.sw[n / 2] >> mine;
           const float sc = __uint_as_float(n & 1 ? sw << 7 : sw << 23);
           w[n][0] = fp4_bf16(H.c[n].x, sc);
           w[n][1] = fp4_bf16(H.c[n].y, sc);
@@ -296,7 +309,10 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 ? 2 : 1) void tile_kernel(Ti
 #pragma unroll
           for (int f = 0; f < MF; f++)
 #pragma unroll
-            for (int n = 0; n < NF; n++) acc[f][n] = mfma_bf16_32(w[n][t], H.x[f][i][t], acc[f][n]);
+            for (int n = 0; n < NF; n++) {
+              f32x16 &to = NA > 1 ? more[(t * P + i) % NA] : acc[f][n];
+              to = mfma_bf16_32(w[n][t], H.x[f][i][t], to);
+            }
     }
   };
 
@@ -320,6 +336,9 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 ? 2 : 1) void tile_kernel(Ti
     __builtin_amdgcn_sched_barrier(0);
     slot = next;
   }
+  if constexpr (NA > 1)
+#pragma unroll
+    for (int v = 0; v < 16; v++) acc[0][0][v] = (more[0][v] + more[1][v]) + (more[2][v] + more[3][v]);
   wait_vmcnt<0>();  // nothing may land in LDS any more
   __syncthreads();
 
@@ -327,7 +346,7 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 ? 2 : 1) void tile_kernel(Ti
   // 4 h + v % 4. The wave's outputs of a row tile as rows in its part of LDS,
   // then to memory a whole row's at a time.
   const int C = p.w.gate ? NF * 16 : NF * 32, pitch = C + 4;
-  float *mine = reinterpret_cast<float *>(lds) + wave * (32 * (NF * 32 + 4));
+  float *outs = reinterpret_cast<float *>(lds) + wave * (32 * (NF * 32 + 4));
   const bool wide = p.odtype == FMT_F32;
   const int V = wide ? 4 : 8, lanes = C / V, at = lane % lanes * V;  // outputs of a lane, lanes of a row
   const bool vec = p.ldo % V == 0 && reinterpret_cast<uintptr_t>(p.out) % 16 == 0;
@@ -350,7 +369,7 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 ? 2 : 1) void tile_kernel(Ti
         f32x4 v;
 #pragma unroll
         for (int i = 0; i < 4; i++) v[i] = p.w.gate ? mx_gate(acc[f][n][u * 4 + i], acc[f][n][(u * 4 + i + 8) & 15]) : acc[f][n][u * 4 + i];
-        *reinterpret_cast<f32x4 *>(mine + l32 * pitch + n * (p.w.gate ? 16 : 32) + u * 8 + h * 4) = v;
+        *reinterpret_cast<f32x4 *>(outs + l32 * pitch + n * (p.w.gate ? 16 : 32) + u * 8 + h * 4) = v;
       }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -364,7 +383,7 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 ? 2 : 1) void tile_kernel(Ti
 #pragma unroll
       for (int j = 0; j < 8; j += 4) {
         if (j && wide) continue;
-        const f32x4 a = *reinterpret_cast<const f32x4 *>(mine + row * pitch + at + j);
+        const f32x4 a = *reinterpret_cast<const f32x4 *>(outs + row * pitch + at + j);
 #pragma unroll
         for (int k = 0; k < 4; k++) v[j + k] = zero ? 0.f : a[k];
       }
@@ -470,14 +489,47 @@ hipError_t launch_mx_tiles(const MxProduct &p, void *scratch, hipStream_t st) {
       if (e != hipSuccess) return e;
     }
   }
-  const int xm = p.xdtype == FMT_MXFP4 ? 0 : mx_planes(p.xdtype);
-  if (p.w.fmt == FMT_MXFP4) {
-    if (xm == 0) return launch<FMT_MXFP4, 0, 128, 256, 4, 2, 3>(g, st);
-    if (xm == 1) return launch<FMT_MXFP4, 1, 128, 256, 4, 2, 3>(g, st);
-    if (xm == 2) return launch<FMT_MXFP4, 2, 128, 256, 4, 2, 3>(g, st);
-    return launch<FMT_MXFP4, 3, 64, 256, 4, 1, 2>(g, st);
+  // The largest tiles that give most CUs a block, and of groups no taller than
+  // their rows need (BM x BN, measured at K = 2560; "rows" of each group on
+  // average):
+  //   6912 outputs, MXFP4 rows: 64 rows 8.1 us with 32 x 128, 12.3 with 64 x
+  //   256; 256 rows 10.3 with 64 x 128, 11.7 and 12.9; 1024 rows 19.5 with 64 x
+  //   256, 24.7 with 64 x 128; fp32 rows 25 and 47, 39 and 52, 98 and 112;
+  //   64 pairs of 1728: fp32, 16 rows: 124 with 32 x 128, 152 with 64 x 256,
+  //   64 rows: 270 and 248; MXFP4, 64 rows: 79 with 64 x 256, 78 with 128 x 256,
+  //   256 rows: 181 and 163;
+  //   BF16, 32 pairs: 32 rows 110 with 64 x 256, 113 with 128 x 256, 128 rows: 180
+  //   and 151; 8 experts of 2560 x 1728, 512 rows: 60 and 51 with 256 x 256.
+  const int64_t groups = p.offsets ? std::min(p.w.experts, p.n) : 1, rows = p.n / groups;
+  const int64_t cus = device_cu_count(), stored = p.w.tiles * 16;
+  auto blocks = [&](int bm, int bn) { return groups * ((rows + bm - 1) / bm) * ((stored + bn - 1) / bn); };
+  auto fills = [&](int bm, int bn) { return blocks(bm, bn) * 4 >= cus * 3; };
+  const bool mx = p.xdtype == FMT_MXFP4, bf16 = p.w.fmt == FMT_BF16;
+  const int planes = mx_planes(p.xdtype);
+  const bool low = p.offsets && planes > 1 && rows <= 24;  // (one plane: the matrix's loads count for more)
+  auto go = [&](auto wf, auto xm) {
+    constexpr int WF = decltype(wf)::value, XM = decltype(xm)::value;
+    constexpr bool B = WF == FMT_BF16, Q = XM == 0;
+    if constexpr (B && XM == 1)
+      if (rows >= 384 && fills(256, 256)) return launch<WF, XM, 256, 256, 8, 4, 2>(g, st);
+    if constexpr (Q)
+      if (rows >= 128 && fills(128, 256)) return launch<WF, XM, 128, 256, 4, 2, 3>(g, st);
+    if constexpr (B)
+      if (rows >= 96 && fills(128, 256)) return launch<WF, XM, 128, 256, 8, 2, XM == 1 ? 3 : 2>(g, st);
+    if (!low && fills(64, 256)) return launch<WF, XM, 64, 256, 4, 1, Q ? 3 : 2>(g, st);
+    if (!low && fills(64, 128)) return launch<WF, XM, 64, 128, 4, 2, Q || XM == 1 && !B ? 6 : XM == 3 ? 2 : 3>(g, st);
+    return launch<WF, XM, 32, 128, 4, 1, Q ? 6 : B ? 5 - XM : XM == 1 ? 8 : 4>(g, st);
+  };
+  using std::integral_constant;
+  if (bf16) {
+    const integral_constant<int, FMT_BF16> wf;
+    return planes == 1 ? go(wf, integral_constant<int, 1>())
+           : planes == 2 ? go(wf, integral_constant<int, 2>())
+                         : go(wf, integral_constant<int, 3>());
   }
-  if (xm == 1) return launch<FMT_BF16, 1, 128, 256, 4, 2, 3>(g, st);
-  if (xm == 2) return launch<FMT_BF16, 2, 64, 256, 4, 1, 2>(g, st);
-  return launch<FMT_BF16, 3, 64, 256, 4, 1, 2>(g, st);
+  const integral_constant<int, FMT_MXFP4> wf;
+  return mx            ? go(wf, integral_constant<int, 0>())
+         : planes == 1 ? go(wf, integral_constant<int, 1>())
+         : planes == 2 ? go(wf, integral_constant<int, 2>())
+                       : go(wf, integral_constant<int, 3>());
 }
