@@ -329,7 +329,7 @@ int tinyoai_weight_free(tinyoai_weight *w);
  * zeros, as tinyoai_mxfp4_quantize_device writes them. Codes lie on a 16-byte
  * boundary, scales on a 4-byte one. */
 
-/* n rows of `cols` values (a multiple of 32) to MXFP4: a block's scale is
+/* n rows of `cols` values (a multiple of 32, at most 2^22) to MXFP4: a block's scale is
  * 2^(floor(log2 m) - 2), m its largest magnitude, within 2^-127 .. 2^127; values
  * over the scale go to the nearest code, halfway ones to the even code, those
  * past 6 to 6. A block with an infinity or NaN becomes NaN (scale 255). */

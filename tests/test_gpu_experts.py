@@ -449,7 +449,9 @@ def _route_expected(x, k, over_all):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("n,experts,k,over_all,pad", [(1, 1, 1, False, 0), (1, 8, 8, True, 0), (16, 64, 4, False, 3),
                                                       (32, 65, 8, True, 0), (33, 128, 2, False, 0), (7, 1000, 32, True, 1),
-                                                      (500, 200, 5, False, 0), (3000, 7, 3, True, 5), (1500, 512, 1, True, 0)])
+                                                      (500, 200, 5, False, 0), (3000, 7, 3, True, 5), (1500, 512, 1, True, 0),
+                                                      (4500, 130, 2, False, 0), (1100, 1024, 8, True, 0), (2, 1024, 32, False, 0),
+                                                      (9001, 1, 1, False, 0)])
 def test_route(hip, dev, dtype, n, experts, k, over_all, pad):
     """Ties, masked experts (-inf, NaN, every one of a token), infinities and zeros of both signs."""
     rng = np.random.default_rng(n + experts)

@@ -164,6 +164,8 @@ static int check_rows(const char *what, int32_t dtype, const void *p, int64_t ld
 
 using namespace tinyoai;
 
+static constexpr int64_t kMostCols = 1 << 22;  // of MXFP4 rows
+
 struct tinyoai_experts {
   ExpertMatrix m;
   int device = 0;
@@ -178,7 +180,7 @@ extern "C" {
 
 int tinyoai_mxfp4_quantize_device(int32_t dtype, const void *x_dev, int64_t ldx, int64_t n, int64_t cols,
                                   uint8_t *codes_dev, uint8_t *scales_dev, void *stream) {
-  if (n <= 0 || cols <= 0 || cols % 32 || n > INT32_MAX || cols > INT32_MAX)
+  if (n <= 0 || cols <= 0 || cols % 32 || n > INT32_MAX || cols > kMostCols)
     return fail(TINYOAI_EINVAL, "invalid MXFP4 shape [%lld, %lld]", (long long)n, (long long)cols);
   if (int rc = check_rows("x", dtype, x_dev, ldx, cols)) return rc;
   if (!codes_dev || !scales_dev) return fail(TINYOAI_EINVAL, "invalid MXFP4 rows");
@@ -189,7 +191,7 @@ int tinyoai_mxfp4_quantize_device(int32_t dtype, const void *x_dev, int64_t ldx,
 
 int tinyoai_mxfp4_dequantize_device(const uint8_t *codes_dev, const uint8_t *scales_dev, int64_t n, int64_t cols,
                                     int32_t dtype, void *out_dev, int64_t ldo, void *stream) {
-  if (n <= 0 || cols <= 0 || cols % 32 || n > INT32_MAX || cols > INT32_MAX)
+  if (n <= 0 || cols <= 0 || cols % 32 || n > INT32_MAX || cols > kMostCols)
     return fail(TINYOAI_EINVAL, "invalid MXFP4 shape [%lld, %lld]", (long long)n, (long long)cols);
   if (int rc = check_rows("out", dtype, out_dev, ldo, cols)) return rc;
   if (!codes_dev || !scales_dev) return fail(TINYOAI_EINVAL, "invalid MXFP4 rows");
@@ -216,7 +218,8 @@ int tinyoai_route_device(int32_t dtype, const void *logits_dev, int64_t ld, int3
 int tinyoai_combine_device(int32_t dtype, const void *y_dev, int64_t ldy, int32_t y_rows, const int32_t *positions_dev,
                            const float *weights_dev, int32_t n, int32_t k, int64_t cols, int32_t out_dtype, void *out_dev,
                            int64_t ldo, void *stream) {
-  if (n <= 0 || k <= 0 || y_rows < 0 || cols <= 0 || cols > INT32_MAX || (int64_t)n * k > (1 << 30))
+  if (n <= 0 || k <= 0 || y_rows < 0 || cols <= 0 || cols > INT32_MAX || (int64_t)n * k > (1 << 30) ||
+      n * ((cols + 255) / 256) > INT32_MAX)
     return fail(TINYOAI_EINVAL, "invalid sum of %d rows for %d tokens", k, n);
   if (int rc = check_rows("y", dtype, y_dev, ldy, cols)) return rc;
   if (int rc = check_rows("out", out_dtype, out_dev, ldo, cols)) return rc;

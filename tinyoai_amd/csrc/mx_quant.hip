@@ -11,6 +11,8 @@
 // them). Eight values a lane: four lanes hold a block, whose largest
 // magnitude they exchange by two lane moves; sixteen a row's 128 columns, and
 // a wave four rows', which lie together in the codes.
+#include <type_traits>
+
 #include "mx.h"
 
 namespace {
@@ -43,15 +45,16 @@ __device__ __forceinline__ void load8(const void *x, int64_t i, float (&v)[8]) {
   }
 }
 
-// One item: eight values of a row's 128 columns (zeros past cols).
+// An item: eight values of a row's 128 columns `unit` (zeros past cols).
 template <int D, bool VEC>
-__global__ __launch_bounds__(kT) void quantize_kernel(const void *x, int64_t ldx, int64_t n, int64_t cols, int64_t units,
-                                                      uint32_t *codes, uint32_t *scales) {
-  const int64_t total = n * units * 16;  // a multiple of 16: the 16 lanes of a scale word stay together
-  for (int64_t i = blockIdx.x * (int64_t)kT + threadIdx.x; i < total; i += (int64_t)gridDim.x * kT) {
-    const int64_t unit = i / (n * 16), row = (i - unit * n * 16) >> 4, c = unit * 128 + (i & 15) * 8;
+__global__ __launch_bounds__(kT) void quantize_kernel(const void *x, int64_t ldx, int64_t n, int64_t cols, uint32_t *codes,
+                                                      uint32_t *scales) {
+  const int64_t unit = blockIdx.y, first = unit * n * 16;
+  // (the 16 lanes of a row stay together: their number is a multiple of 16)
+  for (int64_t i = blockIdx.x * (int64_t)kT + threadIdx.x; i < n * 16; i += (int64_t)gridDim.x * kT) {
+    const int64_t c = unit * 128 + (i & 15) * 8;
     float v[8] = {};
-    if (c < cols) load8<D, VEC>(x, row * ldx + c, v);
+    if (c < cols) load8<D, VEC>(x, (i >> 4) * ldx + c, v);
     uint32_t most = 0;
 #pragma unroll
     for (int j = 0; j < 8; j++) most = max(most, __float_as_uint(v[j]) & 0x7fffffffu);
@@ -60,36 +63,41 @@ __global__ __launch_bounds__(kT) void quantize_kernel(const void *x, int64_t ldx
     const bool bad = most >= 0x7f800000u;
     // the scale byte: the largest's exponent field less 2, 0 (2^-127) at least
     const uint32_t s = bad ? 255u : max((int)(most >> 23) - 2, 0);
-    const float inv = __uint_as_float((254u - s) << 23);  // 2^(127 - s): s <= 252 (bad ones are not used)
+    // (the conversion takes the scale's exponent alone; nearest, ties to even, at most 6)
+    const float scale = __uint_as_float(s << 23);
     uint32_t word = 0;
-#pragma unroll
-    for (int j = 0; j < 8; j++) {
-      const float a = fabsf(v[j]) * inv;
-      const uint32_t sign = __float_as_uint(v[j]) >> 31;
-      // the halfway points: the even code takes them
-      const uint32_t m = (a > 0.25f) + (a >= 0.75f) + (a > 1.25f) + (a >= 1.75f) + (a > 2.5f) + (a >= 3.5f) + (a > 5.f);
-      word |= (bad ? 0u : m | sign << 3) << (4 * j);
-    }
-    codes[i] = word;
+    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[0], v[1], scale, 0);
+    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[2], v[3], scale, 1);
+    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[4], v[5], scale, 2);
+    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[6], v[7], scale, 3);
+    codes[first + i] = bad ? 0u : word;
     // lane 0 of 16 writes the word of four blocks' scales
     const uint32_t s1 = __shfl(s, (threadIdx.x & 48) + 4), s2 = __shfl(s, (threadIdx.x & 48) + 8),
                    s3 = __shfl(s, (threadIdx.x & 48) + 12);
-    if ((threadIdx.x & 15) == 0) scales[i >> 4] = s | s1 << 8 | s2 << 16 | s3 << 24;
+    if ((i & 15) == 0) scales[(first + i) >> 4] = s | s1 << 8 | s2 << 16 | s3 << 24;
   }
 }
 
 template <int D, bool VEC>
 __global__ __launch_bounds__(kT) void dequantize_kernel(const uint32_t *codes, const uint8_t *scales, int64_t n,
-                                                        int64_t cols, int64_t units, void *out, int64_t ldo) {
-  const int64_t per = cols / 8, total = n * per;
-  for (int64_t i = blockIdx.x * (int64_t)kT + threadIdx.x; i < total; i += (int64_t)gridDim.x * kT) {
-    const int64_t row = i / per, c = i - row * per, at = (c >> 4) * n + row;
-    const uint32_t word = codes[at * 16 + (c & 15)];
-    const float s = mx_scale(scales[at * 4 + ((c & 15) >> 2)]);
+                                                        int64_t cols, void *out, int64_t ldo) {
+  const int64_t unit = blockIdx.y, first = unit * n * 16;
+  for (int64_t i = blockIdx.x * (int64_t)kT + threadIdx.x; i < n * 16; i += (int64_t)gridDim.x * kT) {
+    const int64_t c = unit * 128 + (i & 15) * 8;
+    if (c >= cols) continue;
+    const uint32_t word = codes[first + i];
+    const float s = mx_scale(scales[(first + i) >> 2]);
     float v[8];
-#pragma unroll
-    for (int j = 0; j < 8; j++) v[j] = mx_code((word >> (4 * j)) & 15) * s;
-    const int64_t o = row * ldo + c * 8;
+    auto two = [&](auto sel) {
+      const auto w = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word, 1.f, decltype(sel)::value);
+      v[2 * decltype(sel)::value] = w[0] * s;
+      v[2 * decltype(sel)::value + 1] = w[1] * s;
+    };
+    two(std::integral_constant<int, 0>());
+    two(std::integral_constant<int, 1>());
+    two(std::integral_constant<int, 2>());
+    two(std::integral_constant<int, 3>());
+    const int64_t o = (i >> 4) * ldo + c;
     if constexpr (D == FMT_F32) {
       float *p = static_cast<float *>(out) + o;
       if constexpr (VEC) {
@@ -147,6 +155,10 @@ __global__ __launch_bounds__(kT) void read_kernel(MxMat m, int64_t offset, int64
 }
 
 int blocks_for(int64_t items) { return (int)std::max<int64_t>(1, std::min<int64_t>((items + kT - 1) / kT, 16384)); }
+// A 128-column unit of all rows for each y (2^15 at most).
+dim3 grid_for(int64_t n, int64_t cols) {
+  return dim3((unsigned)std::min<int64_t>((n * 16 + kT - 1) / kT, 1 << 20), (unsigned)((cols + 127) / 128));
+}
 bool aligned16(const void *p, int64_t ld, size_t width) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * (int64_t)width % 16 == 0;
 }
@@ -155,11 +167,10 @@ bool aligned16(const void *p, int64_t ld, size_t width) {
 
 hipError_t launch_mx_quantize(int dtype, const void *x, int64_t ldx, int64_t n, int64_t cols, uint8_t *codes,
                               uint8_t *scales, hipStream_t st) {
-  const int64_t units = (cols + 127) / 128;
-  const dim3 grid(blocks_for(n * units * 16));
+  const dim3 grid = grid_for(n, cols);
   const bool vec = aligned16(x, ldx, mx_width(dtype));
   auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, grid, dim3(kT), 0, st, x, ldx, n, cols, units, reinterpret_cast<uint32_t *>(codes),
+    hipLaunchKernelGGL(kernel, grid, dim3(kT), 0, st, x, ldx, n, cols, reinterpret_cast<uint32_t *>(codes),
                        reinterpret_cast<uint32_t *>(scales));
   };
   if (dtype == FMT_F32) vec ? go(quantize_kernel<FMT_F32, true>) : go(quantize_kernel<FMT_F32, false>);
@@ -170,12 +181,11 @@ hipError_t launch_mx_quantize(int dtype, const void *x, int64_t ldx, int64_t n, 
 
 hipError_t launch_mx_dequantize(const uint8_t *codes, const uint8_t *scales, int64_t n, int64_t cols, int dtype, void *out,
                                 int64_t ldo, hipStream_t st) {
-  const int64_t units = (cols + 127) / 128;
-  const dim3 grid(blocks_for(n * cols / 8));
+  const dim3 grid = grid_for(n, cols);
   const bool vec = aligned16(out, ldo, mx_width(dtype));
   auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, grid, dim3(kT), 0, st, reinterpret_cast<const uint32_t *>(codes), scales, n, cols, units,
-                       out, ldo);
+    hipLaunchKernelGGL(kernel, grid, dim3(kT), 0, st, reinterpret_cast<const uint32_t *>(codes), scales, n, cols, out,
+                       ldo);
   };
   if (dtype == FMT_F32) vec ? go(dequantize_kernel<FMT_F32, true>) : go(dequantize_kernel<FMT_F32, false>);
   else if (dtype == FMT_F16) vec ? go(dequantize_kernel<FMT_F16, true>) : go(dequantize_kernel<FMT_F16, false>);
