@@ -38,6 +38,8 @@ __device__ __forceinline__ uint4 load16(__amdgpu_buffer_rsrc_t r, uint32_t at) {
   return make_uint4(v.x, v.y, v.z, v.w);
 }
 
+constexpr int kMostChunks = 4;  // of a wave
+
 struct FewArgs {
   MxProduct p;
   int units;  // tiles (pairs: of both) of an expert
@@ -45,16 +47,17 @@ struct FewArgs {
   int64_t x_bytes;
 };
 
-constexpr int NC = 4;  // column chunks of a wave, at most
-
-// CT: column tiles (16 operand columns).
-template <int WF, int XM, bool GATE, int kWaves, int CT>
+// CT: column tiles (16 operand columns). NC: column chunks of a wave, at most.
+template <int WF, int XM, bool GATE, int kWaves, int CT, int NC>
 __global__ __launch_bounds__(kWaves * 64) void few_kernel(FewArgs g) {
   constexpr int NT = GATE ? 2 : 1, P = XM == 0 ? 1 : XM, NJ = WF == FMT_MXFP4 ? 4 : 2;
   constexpr int kChunk = mx_cols<WF>();
   constexpr int kRows = 16 * CT / P;            // rows of X at once
   constexpr int kRed = kWaves * NT * CT * 256;  // sums of a unit
   constexpr int kT = kWaves * 64;
+  // Units ahead (as many as the registers hold): two of pairs (16 tokens' fp32
+  // pairs of 32 experts 34.2 us with one, 31.7 so; of plain ones no gain).
+  constexpr int D = NC == 3 && XM != 0 && GATE ? 2 : 1;
   constexpr int kStaged = XM >= 2 ? kWaves * CT * 16 * kChunk / 4 : 0;  // floats; half of each wave's planes of a chunk
   __shared__ __align__(16) float red[2][kRed > kStaged ? kRed : kStaged];
   const MxProduct &p = g.p;
@@ -90,11 +93,13 @@ __global__ __launch_bounds__(kWaves * 64) void few_kernel(FewArgs g) {
       f.s[i] = __builtin_amdgcn_raw_buffer_load_b32(rs, real ? (int)(sat + lane * 4) : (int)kNone, 0, 0);
   };
 
-  for (int r0 = r_lo; r0 < r_hi; r0 += kRows) {
+  for (int r0 = r_lo + blockIdx.z * kRows; r0 < r_hi; r0 += gridDim.z * kRows) {
     const int m = min(kRows, r_hi - r0);
-    Tile a;
+    Tile ring[D];
 #pragma unroll
-    for (int i = 0; i < NC; i++) fetch(a, u0, i);
+    for (int d = 0; d < D; d++)
+#pragma unroll
+      for (int i = 0; i < NC; i++) fetch(ring[d], u0 + d, i);
     __builtin_amdgcn_sched_barrier(0);
     // X: operand column v = plane * m + row of column tile v / 16; columns
     // past the planes, and rows that the index does not name, are zeros.
@@ -229,7 +234,7 @@ __global__ __launch_bounds__(kWaves * 64) void few_kernel(FewArgs g) {
               for (int ct = 0; ct < CT; ct++) acc[t][ct] = mfma_bf16(w[j], x[i][ct][j], acc[t][ct]);
           }
         }
-        fetch(f, u + 1, i);
+        fetch(f, u + D, i);
       }
       // [wave][tile][operand column][16 matrix rows]
 #pragma unroll
@@ -261,12 +266,15 @@ __global__ __launch_bounds__(kWaves * 64) void few_kernel(FewArgs g) {
     };
     // (the sums' buffer of two units ago is free once every wave is past the
     // barrier of the unit between)
-    for (int u = u0; u < u1; u++) {
-      unit(a, u, u & 1);
-      __syncthreads();
-      finish(u, u & 1);
-    }
-    if (r0 + kRows < r_hi) __syncthreads();
+    for (int u = u0; u < u1; u += D)
+#pragma unroll
+      for (int d = 0; d < D; d++) {
+        if (u + d >= u1) break;
+        unit(ring[d], u + d, (u + d) & 1);
+        __syncthreads();
+        finish(u + d, (u + d) & 1);
+      }
+    __syncthreads();  // X of the next rows takes the sums' LDS
   }
 }
 
@@ -277,7 +285,7 @@ int64_t x_bytes(const MxProduct &p) {
   return ((int64_t)(p.x_rows - 1) * p.ldx + p.w.cols) * (int64_t)mx_width(p.xdtype);
 }
 
-template <int WF, int XM, bool GATE, int kWaves, int CT>
+template <int WF, int XM, bool GATE, int kWaves, int CT, int NC>
 hipError_t launch(FewArgs &g, hipStream_t st) {
   const MxProduct &p = g.p;
   g.units = (p.w.rows + 15) / 16;
@@ -287,8 +295,10 @@ hipError_t launch(FewArgs &g, hipStream_t st) {
   // 32 experts 21.9 us instead of 23.6).
   const int64_t blocks = (int64_t)device_cu_count() * (XM == 0 && p.offsets ? 2 : 1);
   g.per = (int)std::max<int64_t>(1, ((int64_t)groups(p) * g.units + blocks - 1) / blocks);
-  hipLaunchKernelGGL((few_kernel<WF, XM, GATE, kWaves, CT>), dim3((g.units + g.per - 1) / g.per, p.offsets ? p.w.experts : 1),
-                     dim3(kWaves * 64), 0, st, g);
+  // a group's rows past the first kRows have blocks of their own
+  const int rows = 16 * CT / (XM == 0 ? 1 : XM);
+  const dim3 grid((g.units + g.per - 1) / g.per, p.offsets ? p.w.experts : 1, std::min((p.n + rows - 1) / rows, p.offsets ? 4 : 1));
+  hipLaunchKernelGGL((few_kernel<WF, XM, GATE, kWaves, CT, NC>), grid, dim3(kWaves * 64), 0, st, g);
   return hipGetLastError();
 }
 
@@ -302,8 +312,8 @@ bool mx_few_supported(const MxProduct &p) {
   const bool pieces = p.xdtype == FMT_MXFP4 || (p.w.cols % 8 == 0 && p.ldx * mx_width(p.xdtype) % 16 == 0 &&
                                                 reinterpret_cast<uintptr_t>(p.x) % 16 == 0);
   const int waves = p.w.gate && p.xdtype != FMT_MXFP4 ? 8 : 16;
-  return p.w.chunks <= waves * NC && pieces && x_bytes(p) < kNone && mx_code_bytes(p.w) < kNone &&
-         (int64_t)p.n * mx_planes(p.xdtype) <= (int64_t)groups(p) * (p.w.chunks <= 8 * NC ? 32 : 16);
+  return p.w.chunks <= waves * kMostChunks && pieces && x_bytes(p) < kNone && mx_code_bytes(p.w) < kNone &&
+         (int64_t)p.n * mx_planes(p.xdtype) <= (int64_t)groups(p) * (p.w.chunks <= 8 * kMostChunks ? 32 : 16);
 }
 
 hipError_t launch_mx_few(const MxProduct &p, hipStream_t st) {
@@ -311,17 +321,24 @@ hipError_t launch_mx_few(const MxProduct &p, hipStream_t st) {
   g.x_bytes = x_bytes(p);
   // column tiles: one for a dense product of few rows; groups are uneven
   const bool two = (int64_t)p.n * mx_planes(p.xdtype) > (p.offsets ? 4 : 16) * (int64_t)groups(p);
+  using std::integral_constant;
   auto go = [&](auto wf, auto xm) {
     constexpr int WF = decltype(wf)::value, XM = decltype(xm)::value;
-    if (p.w.chunks > 8 * NC) {
-      if constexpr (XM == 0)
-        if (p.w.gate) return launch<WF, XM, true, 16, 1>(g, st);
-      return launch<WF, XM, false, 16, 1>(g, st);
-    }
-    if (two) return p.w.gate ? launch<WF, XM, true, 8, 2>(g, st) : launch<WF, XM, false, 8, 2>(g, st);
-    return p.w.gate ? launch<WF, XM, true, 8, 1>(g, st) : launch<WF, XM, false, 8, 1>(g, st);
+    auto gated = [&](auto waves, auto ct, auto nc) {
+      constexpr int K = decltype(waves)::value, CT = decltype(ct)::value, N = decltype(nc)::value;
+      if constexpr (K == 8 || XM == 0)
+        if (p.w.gate) return launch<WF, XM, true, K, CT, N>(g, st);
+      return launch<WF, XM, false, K, CT, N>(g, st);
+    };
+    const integral_constant<int, 1> one;
+    const integral_constant<int, 2> both;
+    const integral_constant<int, 3> three;
+    const integral_constant<int, 4> four;
+    const integral_constant<int, 8> eight;
+    if (p.w.chunks > 8 * 4) return gated(integral_constant<int, 16>(), one, four);
+    if (p.w.chunks > 8 * 3) return two ? gated(eight, both, four) : gated(eight, one, four);
+    return two ? gated(eight, both, three) : gated(eight, one, three);
   };
-  using std::integral_constant;
   const int xm = p.xdtype == FMT_MXFP4 ? 0 : mx_planes(p.xdtype);
   if (p.w.fmt == FMT_MXFP4) {
     const integral_constant<int, FMT_MXFP4> wf;
