@@ -366,8 +366,8 @@ int tinyoai_combine_device(int32_t dtype, const void *y_dev, int64_t ldy, int32_
                            const float *weights_dev, int32_t n, int32_t k, int64_t cols, int32_t out_dtype, void *out_dev,
                            int64_t ldo, void *stream);
 
-/* `experts` matrices [rows][cols] of type MXFP4 or BF16, one after another in
- * `data` (`nbytes` in all). With `up` (as `data`), each expert is a (gate, up)
+/* `experts` matrices [rows][cols] of type MXFP4 or BF16 (at most 65535, of 2^28
+ * rows and 2^22 columns), one after another in `data` (`nbytes` in all). With `up` (as `data`), each expert is a (gate, up)
  * pair and its products are silu(gate) * up (stablelm.go:371-373). */
 typedef struct tinyoai_experts tinyoai_experts;
 int tinyoai_experts_upload(int32_t dtype, int32_t experts, int64_t rows, int64_t cols, const void *data, const void *up,
@@ -376,10 +376,12 @@ int tinyoai_experts_upload(int32_t dtype, int32_t experts, int64_t rows, int64_t
  * pairs) for the rows r of expert e, offsets[e] <= r < offsets[e + 1] <= n, as
  * tinyoai_route_device lists them; index NULL: x[r]. Other rows of out stay as
  * they are. x: F32, F16 or BF16 [x_rows][ldx], or MXFP4 rows (x_scales_dev their
- * scales, ldx = cols; MXFP4 experts). Sums are fp32: F32 and F16 rows count
- * with all their bits. An index outside [0, x_rows) gives a row of zeros.
+ * scales, ldx = cols; MXFP4 experts, x_rows at most 2^25). Sums are fp32: F32
+ * and F16 rows count with all their bits (an infinity in the matrix makes their
+ * products with it NaN). An index outside [0, x_rows) gives a row of zeros.
  * Offsets that leave [0, n] count as the nearest that do not; they must not
  * fall (rows of such groups may be left out; nothing outside `out` is touched).
+ * n / 32 times rows / 128 (pairs: rows / 64) must stay below 2^24.
  * The current device must be the handle's. */
 int tinyoai_experts_mul_device(tinyoai_experts *e, int32_t x_dtype, const void *x_dev, const uint8_t *x_scales_dev,
                                int64_t ldx, int32_t x_rows, const int32_t *offsets_dev, const int32_t *index_dev,

@@ -41,6 +41,13 @@ class Device:
         self.bufs[p.value + at] = (p.value, at, n)
         return p.value + at
 
+    def room(self, nbytes):
+        """A buffer whose bytes are not set."""
+        p = C.c_void_p()
+        assert self.rt.hipMalloc(C.byref(p), nbytes) == 0
+        self.bufs[p.value] = (p.value, 0, nbytes)
+        return p.value
+
     def fill(self, ptr, a):
         a = np.ascontiguousarray(a)
         assert self.rt.hipMemcpy(ptr, a.ctypes.data, a.nbytes, 1) == 0

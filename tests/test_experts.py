@@ -83,6 +83,25 @@ def test_combine_refusals():
             call(**bad)
 
 
+def test_expert_upload_refusals():
+    L, h = hip.lib(), __import__("ctypes").c_void_p()
+    a = np.zeros(64, np.uint8)
+
+    def call(dtype=W.BF16, experts=1, rows=4, cols=8, nbytes=64, data=a.ctypes.data):
+        hip.check(L.tinyoai_experts_upload(dtype, experts, rows, cols, data, None, nbytes, h))
+
+    for bad in (dict(experts=0), dict(experts=65536), dict(rows=0), dict(rows=(1 << 28) + 1), dict(cols=0),
+                dict(cols=(1 << 22) + 1)):
+        _refused("invalid matrix shape", call, *[{**dict(dtype=W.BF16, experts=1, rows=4, cols=8), **bad}[k]
+                                                 for k in ("dtype", "experts", "rows", "cols")])
+    _refused("unsupported expert tensor type", call, W.F32)
+    _refused("whole quant blocks", call, W.MXFP4, 1, 4, 48)
+    _refused("need 64 bytes", call, W.BF16, 1, 4, 8, 63)
+    # (2^51 bytes each: their sum does not fit 64 bits)
+    _refused("bytes", call, W.BF16, 1 << 13, 1 << 28, 1 << 22, 0)
+    _refused("invalid expert upload", call, W.BF16, 1, 4, 8, 64, None)
+
+
 def test_absent_handles():
     L = hip.lib()
     assert L.tinyoai_weight_mul_mxfp4_device(None, A, A, 1, A, None) == -1

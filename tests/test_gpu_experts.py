@@ -6,7 +6,7 @@ import ctypes as C
 import numpy as np
 import pytest
 
-from experts_fixture import (EPS, Device, bits_dtype, decode, encode, matrices, mx_quantize, mx_rows, mx_values,
+from experts_fixture import (EPS, WIDTH, Device, bits_dtype, decode, encode, matrices, mx_quantize, mx_rows, mx_values,
                              random_mx, silu)
 from tinyoai_amd import weights as W
 
@@ -268,6 +268,46 @@ def test_grouped_product_offsets(hip, dev, fmt, xdtype):
     e.close()
 
 
+@pytest.mark.parametrize("counts", [[1, 0, 4], [40, 0, 90, 33]])
+@pytest.mark.parametrize("fmt,xdtype", PAIRS)
+def test_gathered_from_many_rows(hip, dev, fmt, xdtype, counts):
+    """An index into far more rows than it names, up to the last ones of more than 4 GiB."""
+    rng = np.random.default_rng(len(counts))
+    rows, cols, n, m = 40, 256, sum(counts) + 2, sum(counts)
+    raw, w = matrices(rng, fmt, len(counts), rows, cols)
+    e = hip.Experts(fmt, len(counts), rows, cols, raw)
+    unit = 64 if xdtype == W.MXFP4 else WIDTH[xdtype] * cols  # MXFP4: of a row's 128 columns, a unit after the other
+    x_rows = (1 << 32) // (unit * (2 if xdtype == W.MXFP4 else 1)) + 1000
+    if xdtype == W.MXFP4:
+        x_rows = min(x_rows, 1 << 25)
+    src = np.sort(rng.choice(x_rows - 1, n - 1, False))
+    src = np.append(src, x_rows - 1)[rng.permutation(n)].astype(np.int32)
+    px, ps = dev.room(x_rows * unit * (2 if xdtype == W.MXFP4 else 1)), 0
+    if xdtype == W.MXFP4:
+        ps = dev.room(x_rows * 8)
+        q = random_mx(rng, n, cols, 120, 130)
+        c, s = mx_rows(*q)
+        x = mx_values(*q)
+        for i, r in enumerate(src):
+            for u in range(2):
+                dev.fill(px + (u * x_rows + int(r)) * 64, c[u, i])
+                dev.fill(ps + (u * x_rows + int(r)) * 4, s[u, i])
+    else:
+        bits, x = encode(xdtype, rng.standard_normal((n, cols)))
+        for i, r in enumerate(src):
+            dev.fill(px + int(r) * unit, bits[i])
+    out = dev.put(np.full((n, rows), 7, np.float32))
+    offsets = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+    e.mul_device(xdtype, px, ps, cols, x_rows, dev.put(offsets), dev.put(src), n, W.F32, out, rows)
+    got = dev.get(out, (n, rows))
+    assert (got[m:] == 7).all()
+    for i in range(len(counts)):
+        r = slice(offsets[i], offsets[i + 1])
+        want, tol = _expected(x[r], w[i:i + 1], False, W.F32, cols)
+        assert np.all(np.abs(got[r] - want) <= tol), i
+    e.close()
+
+
 @pytest.mark.parametrize("n", [1, 5, 40, 200])
 @pytest.mark.parametrize("fmt,xdtype", [(W.MXFP4, W.F32), (W.MXFP4, W.MXFP4), (W.BF16, W.F32), (W.BF16, W.BF16)])
 def test_product_extreme_values(hip, dev, fmt, xdtype, n):
@@ -409,7 +449,21 @@ def test_refusals_of_handles(hip, dev):
         call(xd=W.MXFP4, x=A + 8, xs=A, h=e)
     with pytest.raises(hip.TinyoaiError, match="invalid MXFP4 rows"):
         call(xd=W.MXFP4, h=e)
+    with pytest.raises(hip.TinyoaiError, match="exceeds what one call takes"):  # 2^25 rows' 64 bytes are 2 GiB
+        call(xd=W.MXFP4, xs=A, xr=(1 << 25) + 1, n=1 << 20, h=e)
     e.close()
+    raw, _ = matrices(rng, W.MXFP4, 1, 130, 64)
+    e = hip.Experts(W.MXFP4, 1, 130, 64, raw)  # 2^31 / 32 times 2 tiles of 256 threads
+    with pytest.raises(hip.TinyoaiError, match="exceeds what one call takes"):
+        call(xr=(1 << 31) - 1, n=(1 << 31) - 1, ldo=130, h=e)
+    e.close()
+    w = hip.Weight(W.Tensor(W.MXFP4, 130, 64, raw))
+    with pytest.raises(hip.TinyoaiError, match="exceeds what one call takes"):
+        w.mul_device(A, (1 << 31) - 1, A)
+    with pytest.raises(hip.TinyoaiError, match="exceeds what one call takes"):
+        w.mul_mxfp4_device(A, A, (1 << 31) - 1, A)
+    w.close()
+    raw, _ = matrices(rng, W.MXFP4, 1, 8, 64)
     q8 = hip.Weight(W.synthetic_q8_0(8, 64, rng))
     with pytest.raises(hip.TinyoaiError, match="need an MXFP4 weight"):
         q8.mul_mxfp4_device(A, A, 1, A)

@@ -2458,6 +2458,7 @@ int tinyoai_weight_mul_device(tinyoai_weight *w, const float *x_dev, int32_t n, 
   hipStream_t st = stream ? (hipStream_t)stream : w->stream;
   if (w->mx.d.codes) {
     const MxProduct p = mx_weight_product(w, x_dev, n, out_dev);
+    if (int rc = check_product(p)) return rc;
     return w->scratch.run(st, mx_scratch(p), [&](void *scratch) { return launch_mx_product(p, scratch, st); });
   }
   const Matrix &m = w->m.desc;
@@ -2483,6 +2484,7 @@ int tinyoai_weight_mul_mxfp4_device(tinyoai_weight *w, const uint8_t *codes_dev,
   p.xdtype = FMT_MXFP4;
   p.x = codes_dev;
   p.xscales = scales_dev;
+  if (int rc = check_product(p)) return rc;
   return w->scratch.run(st, mx_scratch(p), [&](void *scratch) { return launch_mx_product(p, scratch, st); });
 } catch (const std::exception &e) {
   return fail(TINYOAI_ENOMEM, "product: %s", e.what());
@@ -2565,6 +2567,8 @@ int tinyoai_weight_mul_device_noalloc(tinyoai_weight *w, const float *x_dev, int
   const bool order = cap == hipStreamCaptureStatusNone;
   const bool mx = w->mx.d.codes != nullptr;
   const MxProduct mp = mx ? mx_weight_product(w, x_dev, n, out_dev) : MxProduct{};
+  if (mx)
+    if (int rc = check_product(mp)) return rc;
   const Product p = mx ? Product{} : plan_product(m, x_dev, n);
   if ((mx ? mx_scratch(mp) : p.bytes()) > sizeof(scratch))
     return fail(TINYOAI_EINVAL, "product of %d x %d needs more than the no-allocation limit of %zu bytes", n, cols,

@@ -11,12 +11,12 @@
 #include "tinyoai_hip.h"
 
 // ---------------------------------------------------------------- products
-static bool on_tiles(const MxProduct &p) { return !mx_few_supported(p) && mx_tiles_supported(p); }
+bool mx_supported(const MxProduct &p) { return mx_few_supported(p) || mx_tiles_supported(p); }
 
-size_t mx_scratch(const MxProduct &p) { return on_tiles(p) ? mx_tiles_scratch(p) : 0; }
+size_t mx_scratch(const MxProduct &p) { return mx_few_supported(p) ? 0 : mx_tiles_scratch(p); }
 
 hipError_t launch_mx_product(const MxProduct &p, void *scratch, hipStream_t st) {
-  return on_tiles(p) ? launch_mx_tiles(p, scratch, st) : launch_mx_few(p, st);
+  return mx_few_supported(p) ? launch_mx_few(p, st) : launch_mx_tiles(p, scratch, st);
 }
 
 namespace tinyoai {
@@ -94,17 +94,23 @@ ExpertMatrix::~ExpertMatrix() {
   if (mem) hipFree(mem);
 }
 
-int ExpertMatrix::upload(int32_t dtype, int32_t experts, int64_t rows, int64_t cols, const void *data, const void *up,
-                         uint64_t nbytes, hipStream_t st) {
-  if (experts <= 0 || rows <= 0 || cols <= 0 || rows > (1 << 28) || cols > (1 << 28))
-    return fail(TINYOAI_EINVAL, "invalid matrix shape [%lld, %lld]", (long long)rows, (long long)cols);
+int check_matrices(int32_t dtype, int32_t experts, int64_t rows, int64_t cols, uint64_t nbytes, int64_t *each) {
+  if (experts <= 0 || experts > kMxExperts || rows <= 0 || rows > (1 << 28) || cols <= 0 || cols > kMxCols)
+    return fail(TINYOAI_EINVAL, "invalid matrix shape [%lld, %lld] of %d", (long long)rows, (long long)cols, experts);
   if (dtype != FMT_BF16 && dtype != FMT_MXFP4) return fail(TINYOAI_EINVAL, "unsupported expert tensor type %d", dtype);
   if (dtype == FMT_MXFP4 && cols % 32)
     return fail(TINYOAI_EINVAL, "rows of type %d must hold whole quant blocks (%lld values)", dtype, (long long)cols);
-  const int64_t each = dtype == FMT_MXFP4 ? rows * (cols / 32) * 17 : rows * cols * 2;
-  if (nbytes != (uint64_t)each * experts)
-    return fail(TINYOAI_EINVAL, "%d tensors [%lld, %lld] of type %d need %lld bytes, got %llu", experts, (long long)rows,
-                (long long)cols, dtype, (long long)each * experts, (unsigned long long)nbytes);
+  *each = dtype == FMT_MXFP4 ? rows * (cols / 32) * 17 : rows * cols * 2;
+  if (*each > INT64_MAX / experts || nbytes != (uint64_t)*each * experts)
+    return fail(TINYOAI_EINVAL, "%d tensors [%lld, %lld] of type %d need %llu bytes, got %llu", experts, (long long)rows,
+                (long long)cols, dtype, (unsigned long long)*each * experts, (unsigned long long)nbytes);
+  return TINYOAI_OK;
+}
+
+int ExpertMatrix::upload(int32_t dtype, int32_t experts, int64_t rows, int64_t cols, const void *data, const void *up,
+                         uint64_t nbytes, hipStream_t st) {
+  int64_t each = 0;
+  if (int rc = check_matrices(dtype, experts, rows, cols, nbytes, &each)) return rc;
   MxMat m{};
   m.fmt = dtype;
   m.experts = experts;
@@ -150,6 +156,11 @@ int check_mxfp4_rows(const void *codes, const void *scales) {
   return TINYOAI_OK;
 }
 
+int check_product(const MxProduct &p) {
+  if (mx_supported(p)) return TINYOAI_OK;
+  return fail(TINYOAI_EINVAL, "product of %d rows (of %d) by %d outputs exceeds what one call takes", p.n, p.x_rows, p.w.rows);
+}
+
 // A row-major [n][cols] buffer of F32, F16 or BF16 values.
 static int check_rows(const char *what, int32_t dtype, const void *p, int64_t ld, int64_t cols) {
   if (dtype != FMT_F32 && dtype != FMT_F16 && dtype != FMT_BF16)
@@ -163,8 +174,6 @@ static int check_rows(const char *what, int32_t dtype, const void *p, int64_t ld
 }  // namespace tinyoai
 
 using namespace tinyoai;
-
-static constexpr int64_t kMostCols = 1 << 22;  // of MXFP4 rows
 
 struct tinyoai_experts {
   ExpertMatrix m;
@@ -180,7 +189,7 @@ extern "C" {
 
 int tinyoai_mxfp4_quantize_device(int32_t dtype, const void *x_dev, int64_t ldx, int64_t n, int64_t cols,
                                   uint8_t *codes_dev, uint8_t *scales_dev, void *stream) {
-  if (n <= 0 || cols <= 0 || cols % 32 || n > INT32_MAX || cols > kMostCols)
+  if (n <= 0 || cols <= 0 || cols % 32 || n > INT32_MAX || cols > kMxCols)
     return fail(TINYOAI_EINVAL, "invalid MXFP4 shape [%lld, %lld]", (long long)n, (long long)cols);
   if (int rc = check_rows("x", dtype, x_dev, ldx, cols)) return rc;
   if (!codes_dev || !scales_dev) return fail(TINYOAI_EINVAL, "invalid MXFP4 rows");
@@ -191,7 +200,7 @@ int tinyoai_mxfp4_quantize_device(int32_t dtype, const void *x_dev, int64_t ldx,
 
 int tinyoai_mxfp4_dequantize_device(const uint8_t *codes_dev, const uint8_t *scales_dev, int64_t n, int64_t cols,
                                     int32_t dtype, void *out_dev, int64_t ldo, void *stream) {
-  if (n <= 0 || cols <= 0 || cols % 32 || n > INT32_MAX || cols > kMostCols)
+  if (n <= 0 || cols <= 0 || cols % 32 || n > INT32_MAX || cols > kMxCols)
     return fail(TINYOAI_EINVAL, "invalid MXFP4 shape [%lld, %lld]", (long long)n, (long long)cols);
   if (int rc = check_rows("out", dtype, out_dev, ldo, cols)) return rc;
   if (!codes_dev || !scales_dev) return fail(TINYOAI_EINVAL, "invalid MXFP4 rows");
@@ -234,6 +243,8 @@ int tinyoai_experts_upload(int32_t dtype, int32_t experts, int64_t rows, int64_t
                            uint64_t nbytes, tinyoai_experts **out) {
   if (!out || !data) return fail(TINYOAI_EINVAL, "invalid expert upload arguments");
   *out = nullptr;
+  int64_t each = 0;
+  if (int rc = check_matrices(dtype, experts, rows, cols, nbytes, &each)) return rc;
   auto x = std::make_unique<tinyoai_experts>();
   hipError_t e = hipGetDevice(&x->device);
   if (e != hipSuccess) return hip_fail(e, "hipGetDevice");
@@ -263,6 +274,7 @@ int tinyoai_experts_mul_device(tinyoai_experts *x, int32_t x_dtype, const void *
   if (int rc = check_device(x->device, "experts")) return rc;
   hipStream_t st = stream ? (hipStream_t)stream : x->stream;
   const MxProduct p{m, x_dtype, x_dev, x_scales_dev, ldx, x_rows, offsets_dev, index_dev, n, out_dtype, out_dev, ldo};
+  if (int rc = check_product(p)) return rc;
   return x->scratch.run(st, mx_scratch(p), [&](void *scratch) { return launch_mx_product(p, scratch, st); });
 } catch (const std::exception &e) {
   return fail(TINYOAI_ENOMEM, "product: %s", e.what());

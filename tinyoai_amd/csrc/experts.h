@@ -20,8 +20,11 @@ struct ExpertMatrix {
              uint64_t nbytes, hipStream_t st);
 };
 
-// Refusals: another current device than the handle's; misaligned code or
+// Refusals: a shape, type or size that no matrices have (`each`: bytes of one
+// of them); a product past what the kernels address; another current device than the handle's; misaligned code or
 // scale rows.
+int check_matrices(int32_t dtype, int32_t experts, int64_t rows, int64_t cols, uint64_t nbytes, int64_t *each);
+int check_product(const MxProduct &p);
 int check_device(int device, const char *what);
 int check_mxfp4_rows(const void *codes, const void *scales);
 

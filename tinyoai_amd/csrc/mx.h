@@ -34,6 +34,9 @@
 
 enum : int32_t { FMT_MXFP4 = 39 };
 
+constexpr int64_t kMxCols = 1 << 22;  // of a matrix or MXFP4 row, at most
+constexpr int kMxExperts = 65535;     // (blocks of a grid's second dimension)
+
 struct MxMat {
   const uint8_t *codes, *scales;
   int32_t fmt;              // FMT_MXFP4 or FMT_BF16
@@ -145,7 +148,9 @@ hipError_t launch_mx_quantize(int dtype, const void *x, int64_t ldx, int64_t n, 
                               uint8_t *scales, hipStream_t st);
 hipError_t launch_mx_dequantize(const uint8_t *codes, const uint8_t *scales, int64_t n, int64_t cols, int dtype, void *out,
                                 int64_t ldo, hipStream_t st);
-// The product, with mx_scratch bytes of scratch.
+// The product, with mx_scratch bytes of scratch; mx_supported: within what the
+// kernels address.
+bool mx_supported(const MxProduct &p);
 size_t mx_scratch(const MxProduct &p);
 hipError_t launch_mx_product(const MxProduct &p, void *scratch, hipStream_t st);
 // A few rows (or a few for each expert) on the streaming kernel.

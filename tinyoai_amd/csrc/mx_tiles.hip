@@ -35,14 +35,18 @@ namespace {
 using namespace tinyoai_mx;
 
 constexpr int kBand = 8;
-constexpr uint32_t kNone = 0x80000000u, kPast = 0x40000000u;
+// Offsets within a buffer are below 2^31; kNone and what is added to it, and
+// kPast and what it is added to, are past it. (Their sum is 0: the load takes
+// the buffer's first bytes, for a step that is not multiplied.)
+constexpr uint32_t kNone = 0x80000000u, kPast = 0x80000000u;
+constexpr int64_t kExtent = (int64_t)1 << 31;
 
 struct TileArgs {
   MxProduct p;
   const uint16_t *planes;  // XM > 0: bf16 planes of X, plane_stride values apart, rows of ldp values
   int64_t plane_stride;
   int64_t ldp;
-  int mtiles;  // row tiles there can be
+  const int32_t *index;    // X's row in `planes` (MXFP4: in x) of each output row; null: rows as they come
 };
 
 template <int WF, int XM, int BM, int BN, int WAVES>
@@ -144,18 +148,15 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 ? 2 : 1) void tile_kernel(Ti
 
   // Buffers: X from its first row (no index: from the tile's), the matrix from
   // the block's first tile; past them reads zeros.
-  const int64_t xrow = p.index ? 0 : r0;
+  // (MXFP4 rows: a step's columns of all rows lie together, and each step has
+  // a buffer of its own)
+  const int64_t xrow = g.index ? 0 : r0;
   const int64_t xld = Q ? 64 : g.ldp * 2;  // bytes
-  const int64_t xunit = Q ? (int64_t)p.x_rows * 64 : 128;  // from one step's columns to the next
-  const int64_t xrows = p.index ? p.x_rows : min(BM, p.x_rows - r0);
+  const int64_t xrows = g.index ? p.x_rows : min(BM, r1 - r0);
   __amdgpu_buffer_rsrc_t rx[P];
 #pragma unroll
   for (int i = 0; i < P; i++)
-    rx[i] = plane_rsrc(Q ? static_cast<const uint8_t *>(p.x) + xrow * xld
-                         : reinterpret_cast<const uint8_t *>(g.planes + i * g.plane_stride) + xrow * xld,
-                       Q ? (steps - 1) * xunit + xrows * 64 : xrows * xld);
-  const __amdgpu_buffer_rsrc_t rxs =
-      plane_rsrc(Q ? p.xscales + xrow * 4 : p.w.codes, Q ? (int64_t)(steps - 1) * p.x_rows * 4 + xrows * 4 : 0);
+    rx[i] = plane_rsrc(reinterpret_cast<const uint8_t *>(g.planes + i * g.plane_stride) + xrow * xld, Q ? 0 : xrows * xld);
   const int gt = mx_group_tiles(p.w, t0), tg = t0 & 15, wtiles = min(BN / 16, gt - tg);
   const __amdgpu_buffer_rsrc_t rw =
       plane_rsrc(p.w.codes + e * mx_code_bytes(p.w) + mx_tile_at(p.w, t0, 0), ((int64_t)(p.w.chunks - 1) * gt + wtiles) * CB);
@@ -167,8 +168,8 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 ? 2 : 1) void tile_kernel(Ti
   auto source = [&](int row) -> uint32_t {  // of X's row in the buffer, in rows; kNone: no row
     const int r = r0 + row;
     if (row >= BM || r >= r1) return kNone;
-    if (!p.index) return (uint32_t)row;
-    const int src = p.index[r];
+    if (!g.index) return (uint32_t)row;
+    const int src = g.index[r];
     return src >= 0 && src < p.x_rows ? (uint32_t)src : kNone;
   };
   uint32_t xoff[S::NX], woff[S::NW], xsoff = kNone, wsoff = kNone;
@@ -197,12 +198,19 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 ? 2 : 1) void tile_kernel(Ti
   auto issue = [&](int kb, int slot) {
     const bool in = kb < steps;
     const uint32_t base = lds0 + slot * S::kStage;
-    const uint32_t kx = in ? (uint32_t)kb * (uint32_t)xunit : kPast;
+    if constexpr (Q) {
+      const int64_t first = in ? (int64_t)kb * p.x_rows + xrow : 0;  // row, of the step's
+      const auto xc = plane_rsrc(static_cast<const uint8_t *>(p.x) + first * 64, in ? xrows * 64 : 0);
 #pragma unroll
-    for (int i = 0; i < P; i++)
+      for (int j = 0; j < S::NX; j++) lds_dma16(xc, xoff[j], base + (wave + WAVES * j) % S::LX * 1024);
+      lds_dma4(plane_rsrc(p.xscales + first * 4, in ? xrows * 4 : 0), xsoff, base + kXS0 + wave % S::LXS * 256);
+    } else {
+      const uint32_t kx = in ? (uint32_t)kb * 128 : kPast;
 #pragma unroll
-      for (int j = 0; j < S::NX; j++) lds_dma16(rx[i], xoff[j] + kx, base + i * S::kX + (wave + WAVES * j) % S::LX * 1024);
-    if constexpr (Q) lds_dma4(rxs, xsoff + (in ? (uint32_t)kb * (uint32_t)(p.x_rows * 4) : kPast), base + kXS0 + wave % S::LXS * 256);
+      for (int i = 0; i < P; i++)
+#pragma unroll
+        for (int j = 0; j < S::NX; j++) lds_dma16(rx[i], xoff[j] + kx, base + i * S::kX + (wave + WAVES * j) % S::LX * 1024);
+    }
     constexpr bool kHalf = WF == FMT_MXFP4 && !Q;  // a step is half a chunk
     const uint32_t chunk = kHalf ? kb >> 1 : kb;
     const uint32_t kw = in ? chunk * (uint32_t)(gt * CB) + (kHalf ? (kb & 1) * 512 : 0) : kPast;
@@ -409,25 +417,38 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 ? 2 : 1) void tile_kernel(Ti
   }
 }
 
-// X's rows as planes of bf16, columns past `cols` zeros up to ldp.
+// X's rows (those that the index names, in order) as planes of bf16, columns
+// past `cols` zeros up to ldp.
 template <int XT>
-__global__ __launch_bounds__(256) void planes_kernel(MxProduct p, uint16_t *planes, int64_t plane_stride, int64_t ldp) {
-  const int64_t per = ldp / 8, total = per * p.x_rows;
+__global__ __launch_bounds__(256) void planes_kernel(MxProduct p, const int32_t *index, int rows, uint16_t *planes,
+                                                     int64_t plane_stride, int64_t ldp) {
+  const int64_t per = ldp / 8, total = per * rows;
   for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
     const int64_t r = i / per, c = i - r * per;
     constexpr int P = XT == FMT_F32 ? 3 : XT == FMT_F16 ? 2 : 1;
+    const int64_t src = index ? index[r] : r;
+    if (src < 0 || src >= p.x_rows) continue;  // (the product's outputs of such a row are zeros)
     uint4 h[P];
-    planes8<XT>(load_x8<XT>(p, r, (int)c * 8), h);
+    planes8<XT>(load_x8<XT>(p, src, (int)c * 8), h);
 #pragma unroll
     for (int j = 0; j < P; j++) *reinterpret_cast<uint4 *>(planes + j * plane_stride + r * ldp + c * 8) = h[j];
   }
 }
 
 int64_t padded_cols(const MxProduct &p) { return (p.w.cols + 63) / 64 * 64; }
-// bf16 rows that the tiles can read where they are.
+// bf16 rows that the tiles can read where they are (of an index, any of them
+// from one buffer).
 bool direct(const MxProduct &p) {
-  return p.xdtype == FMT_BF16 && p.w.cols % 64 == 0 && p.ldx % 8 == 0 && reinterpret_cast<uintptr_t>(p.x) % 16 == 0;
+  return p.xdtype == FMT_BF16 && p.w.cols % 64 == 0 && p.ldx % 8 == 0 && reinterpret_cast<uintptr_t>(p.x) % 16 == 0 &&
+         (p.index ? p.x_rows : 256) * p.ldx * 2 <= kExtent;
 }
+// Else the planes are of X's rows, or of the rows that the index names where
+// those are fewer or X's would not be one buffer.
+bool gathered(const MxProduct &p) {
+  return p.index && (p.n < p.x_rows || p.x_rows * padded_cols(p) * 2 > kExtent);
+}
+// (without an index, X may have more rows than are multiplied)
+int plane_rows(const MxProduct &p) { return !p.index || gathered(p) ? p.n : p.x_rows; }
 
 template <int WF, int XM, int BM, int BN, int WAVES, int WM, int STAGES>
 hipError_t launch(TileArgs &g, hipStream_t st) {
@@ -436,13 +457,9 @@ hipError_t launch(TileArgs &g, hipStream_t st) {
   constexpr int rows = WAVES * 32 * (BN / (WAVES / WM) + 4) * 4;  // the waves' outputs
   constexpr int bytes = STAGES * S::kStage > rows ? STAGES * S::kStage : rows;
   static_assert(bytes <= 160 * 1024, "LDS of a CU");
-  static bool set = false;
   const auto kernel = &tile_kernel<WF, XM, BM, BN, WAVES, WM, STAGES>;
-  if (!set) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e != hipSuccess) return e;
-    set = true;
-  }
+  static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (attr != hipSuccess) return attr;
   // row tiles there can be: one more for each group than its rows fill
   const int64_t groups = p.offsets ? std::min(p.w.experts, p.n) : 1;
   const int64_t mtiles = p.offsets ? (p.n + groups * (BM - 1)) / BM : (p.n + BM - 1) / BM;
@@ -455,20 +472,21 @@ hipError_t launch(TileArgs &g, hipStream_t st) {
 
 size_t mx_tiles_scratch(const MxProduct &p) {
   if (p.xdtype == FMT_MXFP4 || direct(p)) return 0;
-  return (size_t)mx_planes(p.xdtype) * p.x_rows * padded_cols(p) * 2;
+  return (size_t)mx_planes(p.xdtype) * plane_rows(p) * padded_cols(p) * 2;
 }
 
-// Offsets within a buffer stay below 2^30 bytes: MXFP4 rows, and X where an
-// index may name any of its rows (else the tile's rows alone); a block's 256
-// matrix rows.
+// A step's columns of MXFP4 rows are one buffer, as a block's 256 matrix rows
+// are (kMxCols columns at most); the threads of a launch number below 2^32, with
+// the smallest tiles too.
 bool mx_tiles_supported(const MxProduct &p) {
-  const bool mx = p.xdtype == FMT_MXFP4;
-  const int64_t ld = mx ? (int64_t)p.w.chunks * 64 : direct(p) ? p.ldx * 2 : padded_cols(p) * 2;
-  return (p.index || mx ? p.x_rows : 256) * ld < kPast && (int64_t)p.w.chunks * mx_chunk_bytes(p.w.fmt) * 16 < kPast;
+  const int64_t groups = p.offsets ? std::min(p.w.experts, p.n) : 1;
+  return (p.xdtype != FMT_MXFP4 || (int64_t)p.x_rows * 64 <= kExtent) &&
+         (p.n + groups * 31) / 32 * (((int64_t)p.w.tiles * 16 + 127) / 128) < (int64_t)1 << 24;
 }
 
 hipError_t launch_mx_tiles(const MxProduct &p, void *scratch, hipStream_t st) {
   TileArgs g{p};
+  g.index = p.index;
   if (p.xdtype != FMT_MXFP4) {
     if (direct(p)) {
       g.planes = static_cast<const uint16_t *>(p.x);
@@ -476,11 +494,14 @@ hipError_t launch_mx_tiles(const MxProduct &p, void *scratch, hipStream_t st) {
     } else {
       g.planes = static_cast<const uint16_t *>(scratch);
       g.ldp = padded_cols(p);
-      g.plane_stride = p.x_rows * g.ldp;
-      const int64_t items = p.x_rows * g.ldp / 8;
+      const int rows = plane_rows(p);
+      const int32_t *index = gathered(p) ? p.index : nullptr;
+      if (index) g.index = nullptr;
+      g.plane_stride = rows * g.ldp;
+      const int64_t items = rows * g.ldp / 8;
       const dim3 grid((unsigned)std::min<int64_t>((items + 255) / 256, 1 << 16));
       auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, p, static_cast<uint16_t *>(scratch), g.plane_stride, g.ldp);
+        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, p, index, rows, static_cast<uint16_t *>(scratch), g.plane_stride, g.ldp);
       };
       if (p.xdtype == FMT_F32) go(planes_kernel<FMT_F32>);
       else if (p.xdtype == FMT_F16) go(planes_kernel<FMT_F16>);
@@ -517,7 +538,7 @@ hipError_t launch_mx_tiles(const MxProduct &p, void *scratch, hipStream_t st) {
     if constexpr (B)
       if (rows >= 96 && fills(128, 256)) return launch<WF, XM, 128, 256, 8, 2, XM == 1 ? 3 : 2>(g, st);
     if (!low && fills(64, 256)) return launch<WF, XM, 64, 256, 4, 1, Q ? 3 : 2>(g, st);
-    if (!low && fills(64, 128)) return launch<WF, XM, 64, 128, 4, 2, Q || XM == 1 && !B ? 6 : XM == 3 ? 2 : 3>(g, st);
+    if (!low && fills(64, 128)) return launch<WF, XM, 64, 128, 4, 2, Q || (XM == 1 && !B) ? 6 : XM == 3 ? 2 : 3>(g, st);
     return launch<WF, XM, 32, 128, 4, 1, Q ? 6 : B ? 5 - XM : XM == 1 ? 8 : 4>(g, st);
   };
   using std::integral_constant;
