@@ -565,6 +565,18 @@ def test_combine(hip, dev, dtype, odtype, n, k, cols, pad):
     assert np.array_equal(raw[:, cols:], fresh[:, cols:])
 
 
+def test_combine_many_tokens(hip, dev):
+    """More tokens than a launch has blocks."""
+    rng = np.random.default_rng(8)
+    n, rows = (1 << 24) + 3, 50
+    y = rng.standard_normal(rows).astype(np.float32)
+    pos, w = rng.integers(-1, rows + 1, n).astype(np.int32), rng.random(n, np.float32)
+    out = dev.put(np.full(n, 7, np.float32))
+    hip.combine(W.F32, dev.put(y), 1, rows, dev.put(pos), dev.put(w), n, 1, 1, W.F32, out, 1)
+    want = np.where((pos >= 0) & (pos < rows), y[np.clip(pos, 0, rows - 1)] * w, np.float32(0))
+    assert np.array_equal(dev.get(out, n), want)
+
+
 def test_combine_without_rows(hip, dev):
     """No row at all, and infinities in rows that no position names."""
     y = np.full((4, 8), np.inf, np.float32)
