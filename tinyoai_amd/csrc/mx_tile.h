@@ -80,9 +80,12 @@ __device__ __forceinline__ Raw8<XT> load_x8(const MxProduct &p, int64_t src, int
   using V = std::conditional_t<XT == FMT_F32, uint32_t, uint16_t>;
   const V *s = static_cast<const V *>(p.x) + src * p.ldx + k;
   Raw8<XT> r;
-  if (k + 8 <= p.w.cols && (reinterpret_cast<uintptr_t>(s) & 15) == 0) {
-    r.a[0] = reinterpret_cast<const uint4 *>(s)[0];
-    if constexpr (XT == FMT_F32) r.a[1] = reinterpret_cast<const uint4 *>(s)[1];
+  if (k + 8 <= p.w.cols) {
+#pragma unroll
+    for (int j = 0; j < (XT == FMT_F32 ? 2 : 1); j++) {
+      const u32x4_any v = reinterpret_cast<const u32x4_any *>(s)[j];
+      r.a[j] = make_uint4(v.x, v.y, v.z, v.w);
+    }
   } else {
     V v[8];
 #pragma unroll

@@ -357,7 +357,6 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 ? 2 : 1) void tile_kernel(Ti
   float *outs = reinterpret_cast<float *>(lds) + wave * (32 * (NF * 32 + 4));
   const bool wide = p.odtype == FMT_F32;
   const int V = wide ? 4 : 8, lanes = C / V, at = lane % lanes * V;  // outputs of a lane, lanes of a row
-  const bool vec = p.ldo % V == 0 && reinterpret_cast<uintptr_t>(p.out) % 16 == 0;
   const int o = (p.w.gate ? (t0 + wn * NF * 2) / 2 : t0 + wn * NF * 2) * 16 + at;
 #pragma unroll
   for (int f = 0; f < MF; f++) {
@@ -396,14 +395,14 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 ? 2 : 1) void tile_kernel(Ti
         for (int k = 0; k < 4; k++) v[j + k] = zero ? 0.f : a[k];
       }
       const int64_t to = r * p.ldo + o;
-      if (vec && o + V <= p.w.rows) {
+      if (o + V <= p.w.rows) {
         if (wide) {
-          __builtin_nontemporal_store(f32x4{v[0], v[1], v[2], v[3]}, reinterpret_cast<f32x4 *>(static_cast<float *>(p.out) + to));
+          __builtin_nontemporal_store(f32x4_any{v[0], v[1], v[2], v[3]}, reinterpret_cast<f32x4_any *>(static_cast<float *>(p.out) + to));
         } else {
           uint32_t w[4];
 #pragma unroll
           for (int k = 0; k < 4; k++) w[k] = mx_narrow(p.odtype, v[2 * k]) | (uint32_t)mx_narrow(p.odtype, v[2 * k + 1]) << 16;
-          __builtin_nontemporal_store(u32x4{w[0], w[1], w[2], w[3]}, reinterpret_cast<u32x4 *>(static_cast<uint16_t *>(p.out) + to));
+          __builtin_nontemporal_store(u32x4_any{w[0], w[1], w[2], w[3]}, reinterpret_cast<u32x4_any *>(static_cast<uint16_t *>(p.out) + to));
         }
       } else {
 #pragma unroll

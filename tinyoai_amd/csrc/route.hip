@@ -327,18 +327,18 @@ void launch(const RouteArgs &a, hipStream_t st) {
 // ---------------------------------------------------------------- combine
 // out[t] = sum over j of weights[t][j] * y[positions[t][j]], j in order, in
 // fp32; positions outside [0, y_rows) add nothing. Bound: HBM (each row of y
-// once). A thread forms V consecutive columns, the loads of four choices in
-// flight.
+// once). A thread forms V consecutive columns (16 bytes of y; those of a row's
+// last thread one by one), the loads of four choices in flight.
 template <int D, int V>
-__device__ __forceinline__ void load_row(const void *y, int64_t i, float (&v)[V]) {
-  if constexpr (V == 1) {
-    v[0] = mx_load(D, y, i);
+__device__ __forceinline__ void load_row(const void *y, int64_t i, int n, float (&v)[V]) {
+  if (n < V) {
+#pragma unroll
+    for (int q = 0; q < V; q++) v[q] = q < n ? mx_load(D, y, i + q) : 0.f;
   } else if constexpr (D == FMT_F32) {
-    const float4 a = *reinterpret_cast<const float4 *>(static_cast<const float *>(y) + i);
+    const f32x4_any a = *reinterpret_cast<const f32x4_any *>(static_cast<const float *>(y) + i);
     v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
   } else {
-    const uint4 a = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(y) + i);
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+    const u32x4_any w = *reinterpret_cast<const u32x4_any *>(static_cast<const uint16_t *>(y) + i);
 #pragma unroll
     for (int j = 0; j < 8; j++) {
       const uint16_t h = (uint16_t)(w[j / 2] >> (16 * (j & 1)));
@@ -347,11 +347,13 @@ __device__ __forceinline__ void load_row(const void *y, int64_t i, float (&v)[V]
   }
 }
 
-template <int D, int V>
+template <int D>
 __global__ __launch_bounds__(256) void combine_kernel(CombineArgs a, int per) {
+  constexpr int V = D == FMT_F32 ? 4 : 8;
   const int t = blockIdx.x / per;  // per: blocks of a token
   const int64_t c = ((int64_t)(blockIdx.x - t * per) * 256 + threadIdx.x) * V;
   if (c >= a.cols) return;
+  const int n = (int)min(a.cols - c, (int64_t)V);
   float sum[V] = {};
   for (int j0 = 0; j0 < a.k; j0 += 4) {
     float v[4][V], w[4];
@@ -362,7 +364,7 @@ __global__ __launch_bounds__(256) void combine_kernel(CombineArgs a, int per) {
       const int p = a.positions[slot];
       w[j] = a.weights[slot];
       ok[j] = j0 + j < a.k && p >= 0 && p < a.y_rows;
-      if (ok[j]) load_row<D, V>(a.y, p * a.ldy + c, v[j]);
+      if (ok[j]) load_row<D, V>(a.y, p * a.ldy + c, n, v[j]);
     }
 #pragma unroll
     for (int j = 0; j < 4; j++)
@@ -371,18 +373,20 @@ __global__ __launch_bounds__(256) void combine_kernel(CombineArgs a, int per) {
         if (ok[j]) sum[q] = fmaf(w[j], v[j][q], sum[q]);
   }
   const int64_t o = t * a.ldo + c;
-  if constexpr (V == 1) {
-    mx_store(a.odtype, a.out, o, sum[0]);
+  if (n < V) {
+#pragma unroll
+    for (int q = 0; q < V; q++)
+      if (q < n) mx_store(a.odtype, a.out, o + q, sum[q]);
   } else if (a.odtype == FMT_F32) {
 #pragma unroll
     for (int q = 0; q < V; q += 4)
-      *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + o + q) = make_float4(sum[q], sum[q + 1], sum[q + 2], sum[q + 3]);
+      *reinterpret_cast<f32x4_any *>(static_cast<float *>(a.out) + o + q) = f32x4_any{sum[q], sum[q + 1], sum[q + 2], sum[q + 3]};
   } else {
     uint32_t h[V / 2];
 #pragma unroll
     for (int q = 0; q < V / 2; q++) h[q] = mx_narrow(a.odtype, sum[2 * q]) | (uint32_t)mx_narrow(a.odtype, sum[2 * q + 1]) << 16;
-    if constexpr (V == 8) *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.out) + o) = make_uint4(h[0], h[1], h[2], h[3]);
-    else *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + o) = make_uint2(h[0], h[1]);
+    if constexpr (V == 8) *reinterpret_cast<u32x4_any *>(static_cast<uint16_t *>(a.out) + o) = u32x4_any{h[0], h[1], h[2], h[3]};
+    else *reinterpret_cast<u32x2_any *>(static_cast<uint16_t *>(a.out) + o) = u32x2_any{h[0], h[1]};
   }
 }
 
@@ -398,13 +402,7 @@ hipError_t launch_route(const RouteArgs &a, hipStream_t st) {
 }
 
 hipError_t launch_combine(const CombineArgs &a, hipStream_t st) {
-  // whole 16-byte pieces of y: V columns a thread
-  const int V = a.dtype == FMT_F32 ? 4 : 8;
-  auto pieces = [&](const void *p, int64_t ld, int dtype) {
-    return reinterpret_cast<uintptr_t>(p) % (dtype == FMT_F32 ? 16 : V * 2) == 0 && ld % V == 0;
-  };
-  const bool vec = a.cols % V == 0 && pieces(a.y, a.ldy, a.dtype) && pieces(a.out, a.ldo, a.odtype);
-  const int64_t threads = vec ? a.cols / V : a.cols;
+  const int64_t threads = a.dtype == FMT_F32 ? (a.cols + 3) / 4 : (a.cols + 7) / 8;
   const int per = (int)((threads + 255) / 256);  // at most 2^23
   // A launch's threads number below 2^32: many tokens in several. (Blocks that
   // take several parts in turn cost more, since positions and weights no longer
@@ -422,8 +420,8 @@ hipError_t launch_combine(const CombineArgs &a, hipStream_t st) {
     return launch_combine(part, st);
   }
   auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)(per * a.n)), dim3(256), 0, st, a, per); };
-  if (a.dtype == FMT_F32) vec ? go(combine_kernel<FMT_F32, 4>) : go(combine_kernel<FMT_F32, 1>);
-  else if (a.dtype == FMT_F16) vec ? go(combine_kernel<FMT_F16, 8>) : go(combine_kernel<FMT_F16, 1>);
-  else vec ? go(combine_kernel<FMT_BF16, 8>) : go(combine_kernel<FMT_BF16, 1>);
+  if (a.dtype == FMT_F32) go(combine_kernel<FMT_F32>);
+  else if (a.dtype == FMT_F16) go(combine_kernel<FMT_F16>);
+  else go(combine_kernel<FMT_BF16>);
   return hipGetLastError();
 }
