@@ -137,7 +137,8 @@ def _close(got, want, tol, odtype):
 
 
 SHAPES = [(1, 1, 32), (3, 2, 96), (2, 15, 128), (16, 16, 160), (17, 33, 256), (31, 64, 512), (40, 300, 1024), (5, 70, 2560),
-          (129, 257, 288), (300, 130, 672), (1000, 20, 64), (2, 6912, 2560), (1, 2560, 6912)]
+          (129, 257, 288), (300, 130, 672), (1000, 20, 64), (2, 6912, 2560), (1, 2560, 6912), (48, 260, 2560), (33, 1001, 4160),
+          (12, 130, 6912), (200, 90, 4096), (65, 7, 12800)]
 
 
 @pytest.mark.parametrize("quantised", [False, True])
@@ -418,6 +419,89 @@ def test_captured_and_concurrent_products(hip, dev, fmt, xdtype, n):
         for st in streams:
             rt.hipStreamDestroy(st)
         e.close()
+
+
+@pytest.mark.parametrize("quantised", [False, True])
+def test_captured_weight_product(hip, dev, quantised):
+    """A product that is cut over its columns: two captured calls on two streams and eager calls between the replays."""
+    rng = np.random.default_rng(4)
+    n, rows, cols, rt = 40, 300, 4096, dev.rt
+    raw, _ = matrices(rng, W.MXFP4, 1, rows, cols)
+    w = hip.Weight(W.Tensor(W.MXFP4, rows, cols, raw))
+    xs = [_x_rows(rng, dev, W.MXFP4 if quantised else W.F32, n, cols)[:2] for _ in range(3)]
+    y = [dev.put(np.zeros((n, rows), np.float32)) for _ in range(3)]
+    streams, execs = [C.c_void_p() for _ in range(2)], []
+
+    def call(i, out, stream=0):
+        w.mul_mxfp4_device(*xs[i], n, out, stream) if quantised else w.mul_device(xs[i][0], n, out, stream)
+
+    try:
+        for i, st in enumerate(streams):
+            graph, ex = C.c_void_p(), C.c_void_p()
+            assert rt.hipStreamCreateWithFlags(C.byref(st), 1) == 0
+            assert rt.hipStreamBeginCapture(st, 0) == 0
+            call(i, y[i], st.value)
+            assert rt.hipStreamEndCapture(st, C.byref(graph)) == 0
+            assert rt.hipGraphInstantiate(C.byref(ex), graph, None, None, C.c_size_t(0)) == 0
+            rt.hipGraphDestroy(graph)
+            execs.append(ex)
+        want = []
+        for i in range(3):
+            call(i, y[2])
+            want.append(dev.get(y[2], (n, rows)).copy())
+        assert np.abs(want[0]).max() > 0
+        for _ in range(3):
+            for i in range(3):
+                dev.fill(y[i], np.zeros((n, rows), np.float32))
+            for _ in range(3):
+                for i in range(2):
+                    assert rt.hipGraphLaunch(execs[i], streams[i]) == 0
+                call(2, y[2])
+            for i in range(3):
+                assert np.array_equal(dev.get(y[i], (n, rows)), want[i]), i
+    finally:
+        for ex in execs:
+            rt.hipGraphExecDestroy(ex)
+        for st in streams:
+            rt.hipStreamDestroy(st)
+        w.close()
+
+
+def test_two_threads(hip, dev):
+    """Calls of two threads on one handle, each on its own stream: every call's bits are an idle handle's."""
+    import threading
+    rng = np.random.default_rng(6)
+    rows, cols, experts, n = 100, 256, 4, 120
+    raw, _ = matrices(rng, W.MXFP4, experts, rows, cols)
+    e = hip.Experts(W.MXFP4, experts, rows, cols, raw)
+    po = dev.put(np.linspace(0, n, experts + 1).astype(np.int32))
+    xs = [_x_rows(rng, dev, W.F32, n, cols)[0] for _ in range(2)]
+    y = [[dev.put(np.zeros((n, rows), np.float32)) for _ in range(10)] for _ in range(2)]
+    streams, errors = [C.c_void_p() for _ in range(2)], []
+    for st in streams:
+        assert dev.rt.hipStreamCreateWithFlags(C.byref(st), 1) == 0
+
+    def work(i):
+        try:
+            for out in y[i]:
+                e.mul_device(W.F32, xs[i], 0, cols, n, po, 0, n, W.F32, out, rows, streams[i].value)
+        except Exception as err:
+            errors.append(err)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    got = [[dev.get(out, (n, rows)).copy() for out in outs] for outs in y]
+    for i in range(2):
+        e.mul_device(W.F32, xs[i], 0, cols, n, po, 0, n, W.F32, y[i][0], rows)
+        want = dev.get(y[i][0], (n, rows))
+        assert np.abs(want).max() > 0 and all(np.array_equal(g, want) for g in got[i])
+    for st in streams:
+        dev.rt.hipStreamDestroy(st)
+    e.close()
 
 
 def test_refusals_of_handles(hip, dev):

@@ -43,6 +43,8 @@ constexpr int64_t kExtent = (int64_t)1 << 31;
 
 struct TileArgs {
   MxProduct p;
+  int ks;                  // parts of the columns; part i's sums go to p.out + i * part_stride
+  int64_t part_stride;
   const uint16_t *planes;  // XM > 0: bf16 planes of X, plane_stride values apart, rows of ldp values
   int64_t plane_stride;
   int64_t ldp;
@@ -144,6 +146,11 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 ? 2 : 1) void tile_kernel(Ti
   r1 = __builtin_amdgcn_readfirstlane(r1);
   nt = __builtin_amdgcn_readfirstlane(nt);
   const int t0 = nt * (BN / 16), steps = (p.w.cols + S::kCols - 1) / S::kCols;
+  // (products cut over the columns take the smallest tiles; the others' range of
+  // steps stays plain: 1999 fp32 rows times 6912 x 2560 193 us, 199 otherwise)
+  constexpr bool kParts = BM == 32;
+  const int part = kParts ? blockIdx.y : 0;
+  const int first_step = kParts ? steps * part / g.ks : 0, end_step = kParts ? steps * (part + 1) / g.ks : steps;
   constexpr int CB = WF == FMT_MXFP4 ? 1024 : 2048;
 
   // Buffers: X from its first row (no index: from the tile's), the matrix from
@@ -196,7 +203,7 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 ? 2 : 1) void tile_kernel(Ti
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void *)lds;
   constexpr uint32_t kXS0 = P * S::kX, kW0 = kXS0 + S::kXS, kWS0 = kW0 + S::kW;
   auto issue = [&](int kb, int slot) {
-    const bool in = kb < steps;
+    const bool in = kb < end_step;
     const uint32_t base = lds0 + slot * S::kStage;
     if constexpr (Q) {
       const int64_t first = in ? (int64_t)kb * p.x_rows + xrow : 0;  // row, of the step's
@@ -325,13 +332,13 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 ? 2 : 1) void tile_kernel(Ti
   };
 
 #pragma unroll
-  for (int i = 0; i < STAGES - 1; i++) issue(i, i);
+  for (int i = 0; i < STAGES - 1; i++) issue(first_step + i, i);
   wait_vmcnt<S::kLoads *(STAGES - 2)>();
   __syncthreads();
   Half A, B;
-  read(A, 0, 0, 0);
-  issue(STAGES - 1, STAGES - 1);
-  for (int kb = 0, slot = 0; kb < steps; kb++) {
+  read(A, first_step, 0, 0);
+  issue(first_step + STAGES - 1, STAGES - 1);
+  for (int kb = first_step, slot = 0; kb < end_step; kb++) {
     const int next = slot + 1 == STAGES ? 0 : slot + 1;
     read(B, kb, slot, 1);
     multiply(A, std::integral_constant<int, 0>());
@@ -394,7 +401,7 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 ? 2 : 1) void tile_kernel(Ti
 #pragma unroll
         for (int k = 0; k < 4; k++) v[j + k] = zero ? 0.f : a[k];
       }
-      const int64_t to = r * p.ldo + o;
+      const int64_t to = part * g.part_stride + r * p.ldo + o;
       if (o + V <= p.w.rows) {
         if (wide) {
           __builtin_nontemporal_store(f32x4_any{v[0], v[1], v[2], v[3]}, reinterpret_cast<f32x4_any *>(static_cast<float *>(p.out) + to));
@@ -434,6 +441,24 @@ __global__ __launch_bounds__(256) void planes_kernel(MxProduct p, const int32_t 
   }
 }
 
+// The sums of the parts, in order.
+__global__ __launch_bounds__(256) void join_kernel(const float *parts, int ks, int64_t values, float *out) {
+  const int64_t i = (blockIdx.x * (int64_t)256 + threadIdx.x) * 4;
+  if (i >= values) return;
+  f32x4_any sum = {0.f, 0.f, 0.f, 0.f};
+  if (i + 4 <= values) {
+#pragma unroll 8
+    for (int k = 0; k < ks; k++) sum += *reinterpret_cast<const f32x4_any *>(parts + k * values + i);
+    *reinterpret_cast<f32x4_any *>(out + i) = sum;
+  } else {
+    for (int64_t j = i; j < values; j++) {
+      float s = 0.f;
+      for (int k = 0; k < ks; k++) s += parts[k * values + j];
+      out[j] = s;
+    }
+  }
+}
+
 int64_t padded_cols(const MxProduct &p) { return (p.w.cols + 63) / 64 * 64; }
 // bf16 rows that the tiles can read where they are (of an index, any of them
 // from one buffer).
@@ -463,15 +488,33 @@ hipError_t launch(TileArgs &g, hipStream_t st) {
   const int64_t groups = p.offsets ? std::min(p.w.experts, p.n) : 1;
   const int64_t mtiles = p.offsets ? (p.n + groups * (BM - 1)) / BM : (p.n + BM - 1) / BM;
   const int64_t blocks = (mtiles * ((p.w.tiles * 16 + BN - 1) / BN) + 7) / 8 * 8;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(WAVES * 64), bytes, st, g);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks, BM == 32 ? g.ks : 1), dim3(WAVES * 64), bytes, st, g);
   return hipGetLastError();
 }
 
 }  // namespace
 
-size_t mx_tiles_scratch(const MxProduct &p) {
+// A weight's product whose smallest tiles leave half of the CUs without a block
+// is cut over the columns, into parts of 8 steps at least, for a block a CU; the
+// parts' sums are added by a launch of their own, which a short K does not repay
+// (whole and in parts: fp32 rows, 128 x 1000, K = 4096, 33 and 17.6 us; 12 x 4096,
+// K = 6912, 46 and 16; 48 x 2560, K = 2560, 22 and 16; 64 x 1024, K = 1024, 12.5
+// and 12.7; MXFP4 rows, 100 x 500, K = 6912, 19 and 13.5; 400 x 1024, K = 2560,
+// 11.3 and 13.1). The sums take 4 MiB at most.
+static int parts_of(const MxProduct &p) {
+  const int cols = p.xdtype == FMT_MXFP4 ? 128 : 64, steps = (p.w.cols + cols - 1) / cols;
+  if (p.offsets || p.w.gate || p.odtype != FMT_F32 || p.ldo != p.w.rows || steps < 32) return 1;
+  const int64_t blocks = (int64_t)((p.n + 31) / 32) * ((p.w.tiles * 16 + 127) / 128);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(device_cu_count() / blocks, steps / 8));
+}
+static size_t planes_bytes(const MxProduct &p) {
   if (p.xdtype == FMT_MXFP4 || direct(p)) return 0;
-  return (size_t)mx_planes(p.xdtype) * plane_rows(p) * padded_cols(p) * 2;
+  return (size_t)mx_planes(p.xdtype) * plane_rows(p) * padded_cols(p) * 2;  // (a multiple of 128)
+}
+
+size_t mx_tiles_scratch(const MxProduct &p) {
+  const int ks = parts_of(p);
+  return planes_bytes(p) + (ks > 1 ? (size_t)ks * p.n * p.w.rows * 4 : 0);
 }
 
 // A step's columns of MXFP4 rows are one buffer, as a block's 256 matrix rows
@@ -486,6 +529,11 @@ bool mx_tiles_supported(const MxProduct &p) {
 hipError_t launch_mx_tiles(const MxProduct &p, void *scratch, hipStream_t st) {
   TileArgs g{p};
   g.index = p.index;
+  g.ks = parts_of(p);
+  if (g.ks > 1) {
+    g.p.out = static_cast<uint8_t *>(scratch) + planes_bytes(p);
+    g.part_stride = (int64_t)p.n * p.w.rows;
+  }
   if (p.xdtype != FMT_MXFP4) {
     if (direct(p)) {
       g.planes = static_cast<const uint16_t *>(p.x);
@@ -541,15 +589,21 @@ hipError_t launch_mx_tiles(const MxProduct &p, void *scratch, hipStream_t st) {
     return launch<WF, XM, 32, 128, 4, 1, Q ? 6 : B ? 5 - XM : XM == 1 ? 8 : 4>(g, st);
   };
   using std::integral_constant;
+  hipError_t e;
   if (bf16) {
     const integral_constant<int, FMT_BF16> wf;
-    return planes == 1 ? go(wf, integral_constant<int, 1>())
-           : planes == 2 ? go(wf, integral_constant<int, 2>())
-                         : go(wf, integral_constant<int, 3>());
+    e = planes == 1   ? go(wf, integral_constant<int, 1>())
+        : planes == 2 ? go(wf, integral_constant<int, 2>())
+                      : go(wf, integral_constant<int, 3>());
+  } else {
+    const integral_constant<int, FMT_MXFP4> wf;
+    e = mx            ? go(wf, integral_constant<int, 0>())
+        : planes == 1 ? go(wf, integral_constant<int, 1>())
+        : planes == 2 ? go(wf, integral_constant<int, 2>())
+                      : go(wf, integral_constant<int, 3>());
   }
-  const integral_constant<int, FMT_MXFP4> wf;
-  return mx            ? go(wf, integral_constant<int, 0>())
-         : planes == 1 ? go(wf, integral_constant<int, 1>())
-         : planes == 2 ? go(wf, integral_constant<int, 2>())
-                       : go(wf, integral_constant<int, 3>());
+  if (e != hipSuccess || g.ks == 1) return e;
+  hipLaunchKernelGGL(join_kernel, dim3((unsigned)((g.part_stride + 1023) / 1024)), dim3(256), 0, st,
+                     static_cast<const float *>(g.p.out), g.ks, g.part_stride, static_cast<float *>(p.out));
+  return hipGetLastError();
 }
