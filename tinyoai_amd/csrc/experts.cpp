@@ -240,7 +240,7 @@ int tinyoai_combine_device(int32_t dtype, const void *y_dev, int64_t ldy, int32_
 }
 
 int tinyoai_experts_upload(int32_t dtype, int32_t experts, int64_t rows, int64_t cols, const void *data, const void *up,
-                           uint64_t nbytes, tinyoai_experts **out) {
+                           uint64_t nbytes, tinyoai_experts **out) try {
   if (!out || !data) return fail(TINYOAI_EINVAL, "invalid expert upload arguments");
   *out = nullptr;
   int64_t each = 0;
@@ -253,6 +253,8 @@ int tinyoai_experts_upload(int32_t dtype, int32_t experts, int64_t rows, int64_t
   if (int rc = x->m.upload(dtype, experts, rows, cols, data, up, nbytes, x->stream)) return rc;
   *out = x.release();
   return TINYOAI_OK;
+} catch (const std::exception &e) {
+  return fail(TINYOAI_ENOMEM, "expert upload: %s", e.what());
 }
 
 int tinyoai_experts_mul_device(tinyoai_experts *x, int32_t x_dtype, const void *x_dev, const uint8_t *x_scales_dev,
@@ -273,6 +275,8 @@ int tinyoai_experts_mul_device(tinyoai_experts *x, int32_t x_dtype, const void *
   if (!index_dev && x_rows < n) return fail(TINYOAI_EINVAL, "%d rows of x for %d rows without an index", x_rows, n);
   if (int rc = check_device(x->device, "experts")) return rc;
   hipStream_t st = stream ? (hipStream_t)stream : x->stream;
+  // (without an index, rows past n do not count; an MXFP4 buffer's layout has them)
+  if (!index_dev && x_dtype != FMT_MXFP4) x_rows = n;
   const MxProduct p{m, x_dtype, x_dev, x_scales_dev, ldx, x_rows, offsets_dev, index_dev, n, out_dtype, out_dev, ldo};
   if (int rc = check_product(p)) return rc;
   return x->scratch.run(st, mx_scratch(p), [&](void *scratch) { return launch_mx_product(p, scratch, st); });
