@@ -5,17 +5,20 @@
 // columns: a wave holds its columns of X in registers, as operands of the
 // matrix cores, and streams its columns of one tile of 16 matrix rows after
 // another (pairs: of two), each chunk's registers loaded again for the next
-// tile once it is multiplied; a load takes 1 KB of a tile as it is stored. So nothing but sums goes through LDS: the
-// waves' parts of a tile meet there. (With X in LDS, every wave whole tiles of
-// its own, a block had to stage the rows in parts, and eight waves fitted a CU:
-// 16 tokens' gate and up of 32 experts, 1728 x 2560, took 43 us.)
+// tile once it is multiplied; a load takes 1 KB of a tile as it is stored. So
+// nothing but sums goes through LDS: the waves' parts of a tile meet there.
+// (With X in LDS, every wave whole tiles of its own, a block had to stage the
+// rows in parts, and eight waves fitted a CU: 16 tokens' gate and up of 32
+// experts, 1728 x 2560, took 43 us; now 38, 131 MB at 3.5 TB/s, 31 where the
+// matrices were read just before. One fp32 row times 6912 x 2560: 5.6 us, 1.7
+// TB/s, most of it the launch's ramp.)
 //
-// fp32 and fp16 rows keep all their bits: a value is the exact sum of three
-// (fp16: two) bf16 planes, truncations of what is left, and each plane is an
-// operand column of its own, so P planes of m rows fill m * P of the 16
-// columns that v_mfma_f32_16x16x32_bf16 multiplies anyway; the planes' sums
-// are added at the end. MXFP4 codes times their block's scale are exact in
-// bf16. MXFP4 rows take v_mfma_scale_f32_16x16x128_f8f6f4, both operands as
+// fp32 and fp16 rows keep all their bits: a value is the sum of three (fp16:
+// two) bf16 planes, truncations of what is left (exact but for what lies below
+// bf16's smallest, 2^-133), and each plane is an operand column of its own, so P
+// planes of m rows fill m * P of the 16 columns that v_mfma_f32_16x16x32_bf16
+// multiplies anyway; the planes' sums are added at the end. MXFP4 codes times
+// their block's scale are exact in bf16 (past its range infinite). MXFP4 rows take v_mfma_scale_f32_16x16x128_f8f6f4, both operands as
 // they are stored.
 #include <algorithm>
 

@@ -45,7 +45,8 @@ __device__ __forceinline__ uint4 fp4_bf16(uint32_t c, float s) {
 }
 
 // A value's planes as fp32 bit patterns whose low halves are zero: what is
-// left after a plane has eight bits fewer, and the difference is exact. An
+// left after a plane has eight bits fewer, and the difference is exact (but a
+// plane's bits below 2^-133, bf16's smallest, are lost). An
 // infinity or NaN is all in the first plane.
 template <int P>
 __device__ __forceinline__ void planes_of(float v, uint32_t (&h)[P]) {

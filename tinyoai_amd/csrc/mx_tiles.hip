@@ -1,15 +1,24 @@
 // Products of many rows with expert matrices (mx.h) on LDS tiles.
 //
-// A block forms BM rows of one group times BN = 256 stored matrix rows; both
+// A block forms BM rows of one group times BN stored matrix rows; both
 // operands go straight to LDS (buffer loads to LDS, rows picked by the index
 // on the way), a ring of stages ahead of the products, and each wave holds MF x
-// NF tiles of 32 x 32 sums. What bounds it: the matrix cores, and at a short K
-// the output's stores. The matrix is the first operand, so a lane ends with
+// NF tiles of 32 x 32 sums. The matrix is the first operand, so a lane ends with
 // four runs of four outputs of a row, and of a pair with both halves; the sums
 // go through LDS so that whole rows of a wave's outputs are stored together
-// (as they are, a store would take 16-byte pieces of 32 rows).
-// (v_mfma of 16 x 16 x 4 k at the same rate on paper: alone on its SIMD a wave
-// keeps it at half of that, and at 0.9 of the 32 x 32 one.)
+// (as they are, a store would take 16-byte pieces of 32 rows). (16 x 16 sums
+// reach the same rate on paper; a wave alone on its SIMD kept them at half of it,
+// these at 0.9.)
+//
+// What bounds it, by measurement: 1999 fp32 rows times 6912 x 2560 MXFP4, 181 us,
+// the matrix cores, busy 78% of the time (212 GFLOP of plane products, 1.17
+// PFLOP/s; a large library bf16 product reaches 1.22). 8192 MXFP4 rows times 13824
+// x 2560, 200 us, 2.9 PFLOP/s: cores busy 40%; the 453 MB of fp32 outputs alone
+// take 66 us at the rate of a fill, and only the CU's other block hides them
+// (one 256 x 256 block a CU of the same wave tiles 235 us, of larger ones 258).
+// 16384 MXFP4 rows of 64 experts' pairs, 1728 x 2560, 145 us: cores busy 33%, groups'
+// last row tiles and the gate on top. 4096 bf16 rows, 8 BF16 experts of 2560 x
+// 1728, 55 us: cores busy 48%, 0.66 PFLOP/s, three rounds of blocks at most.
 //
 //   planes of X (1, 2 or 3, bf16; mx_tile.h) times BF16, or times MXFP4 codes
 //   that become bf16 times their scale as a wave reads them (exact): 64

@@ -16,7 +16,8 @@
 // expert in `tokens`; the next launch sums the blocks before each, places the
 // block's slots and writes `positions`, and a third one writes `tokens` from
 // them (16384 tokens to 8 of 128 experts: 53 us with a block for each expert,
-// each over all slots, 23 us so).
+// each over all slots, 23 us so, 14 of them the choices' lane moves).
+// 16 tokens to 4 of 64 experts: 5.9 us.
 #include <algorithm>
 
 #include "mx.h"
@@ -327,8 +328,9 @@ void launch(const RouteArgs &a, hipStream_t st) {
 // ---------------------------------------------------------------- combine
 // out[t] = sum over j of weights[t][j] * y[positions[t][j]], j in order, in
 // fp32; positions outside [0, y_rows) add nothing. Bound: HBM (each row of y
-// once). A thread forms V consecutive columns (16 bytes of y; those of a row's
-// last thread one by one), the loads of four choices in flight.
+// once: 8192 tokens of 8 bf16 rows of 2560 columns, 378 MB, in 79 us, 4.8 TB/s).
+// A thread forms V consecutive columns (16 bytes of y; those of a row's last
+// thread one by one), the loads of four choices in flight.
 template <int D, int V>
 __device__ __forceinline__ void load_row(const void *y, int64_t i, int n, float (&v)[V]) {
   if (n < V) {
