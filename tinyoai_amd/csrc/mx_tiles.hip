@@ -354,8 +354,12 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 ? 2 : 1) void tile_kernel(Ti
     __builtin_amdgcn_sched_barrier(0);
     wait_vmcnt<S::kLoads *(STAGES - 2)>();  // this wave's loads of kb + 1 (later steps' may be in flight)
     __syncthreads();                        // every wave's; and all are past their reads of kb
+    // (past the last step: zeros. One bf16 plane and BF16 values: the next loads
+    // after the reads, 2% faster; otherwise before, 2 to 3%)
+    constexpr bool kReadFirst = WF == FMT_BF16 && XM == 1;
+    if constexpr (kReadFirst) read(A, kb + 1, next, 0);
     issue(kb + STAGES, slot);
-    read(A, kb + 1, next, 0);  // (past the last step: zeros)
+    if constexpr (!kReadFirst) read(A, kb + 1, next, 0);
     multiply(B, std::integral_constant<int, 1>());
     __builtin_amdgcn_sched_barrier(0);
     slot = next;
