@@ -627,7 +627,7 @@ def test_route(hip, dev, dtype, n, experts, k, over_all, pad):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("odtype", TYPES)
 @pytest.mark.parametrize("n,k,cols,pad", [(1, 1, 1, 0), (3, 2, 64, 0), (16, 4, 2560, 0), (9, 8, 100, 4), (5, 3, 37, 1),
-                                          (700, 5, 260, 0)])
+                                          (700, 5, 260, 0), (6, 3, 515, 0), (4, 2, 259, 2)])
 def test_combine(hip, dev, dtype, odtype, n, k, cols, pad):
     rng = np.random.default_rng(n * cols)
     y_rows = max(1, n * k - 1)
