@@ -269,6 +269,37 @@ def test_grouped_product_offsets(hip, dev, fmt, xdtype):
     e.close()
 
 
+@pytest.mark.parametrize("fmt,xdtype", [(W.BF16, W.BF16), (W.BF16, W.F32), (W.MXFP4, W.MXFP4), (W.MXFP4, W.F16)])
+def test_longest_rows(hip, dev, fmt, xdtype):
+    """Rows of 2^22 columns, the longest taken: a few hundred small whole numbers in zeros, so every sum is exact."""
+    rng = np.random.default_rng(2)
+    rows, cols, n, offsets = 17, 1 << 22, 3, [0, 2, 3]
+    at = np.unique(np.concatenate([[0, 1, 127, 128, cols // 2, cols - 1, cols - 65], rng.integers(0, cols, 200)]))
+    codes = np.zeros((2, rows, cols), np.uint8)
+    codes[..., at] = rng.choice([0, 2, 4, 5, 6, 7, 10, 12], (2, rows, at.size))  # 0, 1, 2, 3, 4, 6, -1, -2
+    table = np.array([0, .5, 1, 1.5, 2, 3, 4, 6, -0., -.5, -1, -1.5, -2, -3, -4, -6])
+    if fmt == W.MXFP4:
+        raw = np.concatenate([W.encode_mxfp4(c, np.full((rows, cols // 32), 127, np.uint8)) for c in codes])
+    else:
+        raw = (table.astype(np.float32).view(np.uint32) >> 16).astype(np.uint16)[codes].reshape(-1).view(np.uint8)
+    xc = np.zeros((n, cols), np.uint8)
+    xc[:, at] = rng.choice([0, 2, 4, 5, 6, 7, 10, 12], (n, at.size))
+    ps = 0
+    if xdtype == W.MXFP4:
+        c, s = mx_rows(xc, np.full((n, cols // 32), 127, np.uint8))
+        px, ps = dev.put(c), dev.put(s)
+    else:
+        px = dev.put(encode(xdtype, table)[0][xc])
+    e = hip.Experts(fmt, 2, rows, cols, raw)
+    out = dev.put(np.full((n, rows), np.nan, np.float32))
+    e.mul_device(xdtype, px, ps, cols, n, dev.put(np.array(offsets, np.int32)), 0, n, W.F32, out, rows)
+    got = dev.get(out, (n, rows))
+    e.close()
+    for i in range(2):
+        r = slice(offsets[i], offsets[i + 1])
+        assert np.array_equal(got[r], table[xc[r]][:, at] @ table[codes[i][:, at]].T)
+
+
 @pytest.mark.parametrize("counts", [[1, 0, 4], [40, 0, 90, 33]])
 @pytest.mark.parametrize("fmt,xdtype", PAIRS)
 def test_gathered_from_many_rows(hip, dev, fmt, xdtype, counts):
