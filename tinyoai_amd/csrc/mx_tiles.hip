@@ -50,6 +50,20 @@ constexpr int kBand = 8;
 constexpr uint32_t kNone = 0x80000000u, kPast = 0x80000000u;
 constexpr int64_t kExtent = (int64_t)1 << 31;
 
+// A chain of sums on the matrix cores rounds at every 16 columns of each plane
+// (MXFP4 rows: 64), and its error grows with the root of its length: relative to
+// float64, in the norm, fp32 rows times MXFP4 4.5e-7 at 2560 columns, 1.2e-6
+// at 16384, 2.3e-6 at 65536. Long rows (chain_cols) go to totals a run of
+// columns at a time: 2.8, 3.1 and 3.4e-7. Totals take as many registers as the
+// sums, which costs the short rows 1 to 6%, and 21% where it leaves a CU fewer blocks
+// (64 experts' pairs of MXFP4, bf16 rows).
+constexpr int kRunBf16 = 1024, kRunMx = 8192;
+// Columns of one chain, at most: for fp32 rows what keeps the error near that of
+// fp32 sums of 512 columns (5e-7); bf16 rows' inputs are rounded to eight bits already.
+constexpr int chain_cols(int planes) { return planes == 0 ? 65536 : planes == 1 ? 16384 : 8192 / planes; }
+// Past these the totals' own chain counts: the smallest tiles, whose totals are doubles.
+constexpr int kFloatTotals = 1 << 18;
+
 struct TileArgs {
   MxProduct p;
   int ks;                  // parts of the columns; part i's sums go to p.out + i * part_stride
@@ -136,7 +150,7 @@ __device__ __forceinline__ bool find_tile(const MxProduct &p, int lane, int ntil
   return false;
 }
 
-template <int WF, int XM, int BM, int BN, int WAVES, int WM, int STAGES>
+template <int WF, int XM, int BM, int BN, int WAVES, int WM, int STAGES, bool RUNS>
 __global__ __launch_bounds__(WAVES * 64, WAVES == 4 ? 2 : 1) void tile_kernel(TileArgs g) {
   using S = Shape<WF, XM, BM, BN, WAVES>;
   constexpr bool Q = S::Q;
@@ -161,6 +175,7 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 ? 2 : 1) void tile_kernel(Ti
   const int part = kParts ? blockIdx.y : 0;
   const int first_step = kParts ? steps * part / g.ks : 0, end_step = kParts ? steps * (part + 1) / g.ks : steps;
   constexpr int CB = WF == FMT_MXFP4 ? 1024 : 2048;
+  constexpr int kRun = (Q ? kRunMx : kRunBf16) / S::kCols;  // steps
 
   // Buffers: X from its first row (no index: from the tile's), the matrix from
   // the block's first tile; past them reads zeros.
@@ -236,19 +251,41 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 ? 2 : 1) void tile_kernel(Ti
       lds_dma4(rws, wsoff + (in ? chunk * (uint32_t)(gt * 64) : kPast), base + kWS0 + wave % S::LWS * 256);
   };
 
-  // (a single tile has four sums, added at the end: each product would wait
+  // (a single tile has four sums, added at a run's end: each product would wait
   // for the one before)
   constexpr int NA = MF * NF == 1 ? 4 : 1;
   f32x16 acc[MF][NF], more[NA];
+  std::conditional_t<BM == 32, double, float> total[RUNS ? MF : 1][RUNS ? NF : 1][16];
 #pragma unroll
   for (int v = 0; v < 16; v++) {
 #pragma unroll
     for (int f = 0; f < MF; f++)
 #pragma unroll
-      for (int n = 0; n < NF; n++) acc[f][n][v] = 0.f;
+      for (int n = 0; n < NF; n++) {
+        acc[f][n][v] = 0.f;
+        if constexpr (RUNS) total[f][n][v] = 0;
+      }
 #pragma unroll
     for (int a = 0; a < NA; a++) more[a][v] = 0.f;
   }
+  auto joined = [&](int f, int n, int v) {
+    if constexpr (NA > 1) return (more[0][v] + more[1][v]) + (more[2][v] + more[3][v]);
+    else return acc[f][n][v];
+  };
+  auto end_run = [&] {  // the run's sums to the totals
+#pragma unroll
+    for (int v = 0; v < 16; v++) {
+#pragma unroll
+      for (int f = 0; f < MF; f++)
+#pragma unroll
+        for (int n = 0; n < NF; n++) {
+          total[f][n][v] += joined(f, n, v);
+          acc[f][n][v] = 0.f;
+        }
+#pragma unroll
+      for (int a = 0; a < NA; a++) more[a][v] = 0.f;
+    }
+  };
   const int xr = wm * MF * 32 + l32;            // this lane's row of the wave's first row tile
   const int wt = (lane & 31) >> 4, l16 = lane & 15;  // its matrix row: of the pair's tile wt, row l16
   const int mine = 8 * wt + (NF == 1 ? 16 * (wn & 1) : 0);  // where a scale word has the byte of this lane's row in tile 0
@@ -362,11 +399,22 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 ? 2 : 1) void tile_kernel(Ti
     if constexpr (!kReadFirst) read(A, kb + 1, next, 0);
     multiply(B, std::integral_constant<int, 1>());
     __builtin_amdgcn_sched_barrier(0);
+    if constexpr (RUNS)
+      if ((kb + 1) % kRun == 0) end_run();
     slot = next;
   }
-  if constexpr (NA > 1)
+  if constexpr (RUNS) {
+    end_run();
 #pragma unroll
-    for (int v = 0; v < 16; v++) acc[0][0][v] = (more[0][v] + more[1][v]) + (more[2][v] + more[3][v]);
+    for (int v = 0; v < 16; v++)
+#pragma unroll
+      for (int f = 0; f < MF; f++)
+#pragma unroll
+        for (int n = 0; n < NF; n++) acc[f][n][v] = (float)total[f][n][v];
+  } else if constexpr (NA > 1) {
+#pragma unroll
+    for (int v = 0; v < 16; v++) acc[0][0][v] = joined(0, 0, v);
+  }
   wait_vmcnt<0>();  // nothing may land in LDS any more
   __syncthreads();
 
@@ -487,14 +535,14 @@ bool gathered(const MxProduct &p) {
 // (without an index, X may have more rows than are multiplied)
 int plane_rows(const MxProduct &p) { return !p.index || gathered(p) ? p.n : p.x_rows; }
 
-template <int WF, int XM, int BM, int BN, int WAVES, int WM, int STAGES>
+template <int WF, int XM, int BM, int BN, int WAVES, int WM, int STAGES, bool RUNS = false>
 hipError_t launch(TileArgs &g, hipStream_t st) {
   using S = Shape<WF, XM, BM, BN, WAVES>;
   const MxProduct &p = g.p;
   constexpr int rows = WAVES * 32 * (BN / (WAVES / WM) + 4) * 4;  // the waves' outputs
   constexpr int bytes = STAGES * S::kStage > rows ? STAGES * S::kStage : rows;
   static_assert(bytes <= 160 * 1024, "LDS of a CU");
-  const auto kernel = &tile_kernel<WF, XM, BM, BN, WAVES, WM, STAGES>;
+  const auto kernel = &tile_kernel<WF, XM, BM, BN, WAVES, WM, STAGES, RUNS>;
   static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (attr != hipSuccess) return attr;
   // row tiles there can be: one more for each group than its rows fill
@@ -588,18 +636,28 @@ hipError_t launch_mx_tiles(const MxProduct &p, void *scratch, hipStream_t st) {
   const bool mx = p.xdtype == FMT_MXFP4, bf16 = p.w.fmt == FMT_BF16;
   const int planes = mx_planes(p.xdtype);
   const bool low = p.offsets && planes > 1 && rows <= 24;  // (one plane: the matrix's loads count for more)
+  const int cols = p.w.cols, chain = chain_cols(mx ? 0 : planes);
   auto go = [&](auto wf, auto xm) {
     constexpr int WF = decltype(wf)::value, XM = decltype(xm)::value;
     constexpr bool B = WF == FMT_BF16, Q = XM == 0;
-    if constexpr (B && XM == 1)
-      if (rows >= 384 && fills(256, 256)) return launch<WF, XM, 256, 256, 8, 4, 2>(g, st);
-    if constexpr (Q)
-      if (rows >= 128 && fills(128, 256)) return launch<WF, XM, 128, 256, 4, 2, 3>(g, st);
-    if constexpr (B)
-      if (rows >= 96 && fills(128, 256)) return launch<WF, XM, 128, 256, 8, 2, XM == 1 ? 3 : 2>(g, st);
-    if (!low && fills(64, 256)) return launch<WF, XM, 64, 256, 4, 1, Q ? 3 : 2>(g, st);
-    if (!low && fills(64, 128)) return launch<WF, XM, 64, 128, 4, 2, Q || (XM == 1 && !B) ? 6 : XM == 3 ? 2 : 3>(g, st);
-    return launch<WF, XM, 32, 128, 4, 1, Q ? 6 : B ? 5 - XM : XM == 1 ? 8 : 4>(g, st);
+    auto tiles = [&](auto runs) {
+      constexpr bool R = decltype(runs)::value;
+      if constexpr (!R) {  // (no registers for totals)
+        if constexpr (B && XM == 1)
+          if (rows >= 384 && fills(256, 256)) return launch<WF, XM, 256, 256, 8, 4, 2>(g, st);
+        if constexpr (Q)
+          if (rows >= 128 && fills(128, 256)) return launch<WF, XM, 128, 256, 4, 2, 3>(g, st);
+      }
+      if constexpr (B)
+        if (rows >= 96 && fills(128, 256)) return launch<WF, XM, 128, 256, 8, 2, XM == 1 ? 3 : 2, R>(g, st);
+      if (!low && fills(64, 256)) return launch<WF, XM, 64, 256, 4, 1, Q ? 3 : 2, R>(g, st);
+      return launch<WF, XM, 64, 128, 4, 2, Q || (XM == 1 && !B) ? 6 : XM == 3 ? 2 : 3, R>(g, st);
+    };
+    if (cols <= kFloatTotals && !low && (fills(64, 256) || fills(64, 128)))
+      return cols > chain ? tiles(std::true_type()) : tiles(std::false_type());
+    // (a wave has four chains of sums, two of MXFP4 rows)
+    constexpr int kStages = Q ? 6 : B ? 5 - XM : XM == 1 ? 8 : 4;
+    return cols / g.ks > chain * (Q ? 2 : 4) ? launch<WF, XM, 32, 128, 4, 1, kStages, true>(g, st) : launch<WF, XM, 32, 128, 4, 1, kStages>(g, st);
   };
   using std::integral_constant;
   hipError_t e;
