@@ -377,8 +377,9 @@ int tinyoai_experts_upload(int32_t dtype, int32_t experts, int64_t rows, int64_t
  * tinyoai_route_device lists them; index NULL: x[r]. Other rows of out stay as
  * they are. x: F32, F16 or BF16 [x_rows][ldx], or MXFP4 rows (x_scales_dev their
  * scales, ldx = cols; MXFP4 experts, x_rows at most 2^25). Sums are fp32: F32
- * and F16 rows count with all their bits (an infinity in the matrix makes their
- * products with it NaN). An index outside [0, x_rows) gives a row of zeros.
+ * and F16 rows count with all their bits (down to 2^-133, where values below 2^-117
+ * lose some); infinities and NaN give what fp32 products and sums give. An
+ * index outside [0, x_rows) gives a row of zeros.
  * Offsets that leave [0, n] count as the nearest that do not; they must not
  * fall (rows of such groups may be left out; nothing outside `out` is touched).
  * n / 32 times rows / 128 (pairs: rows / 64) must stay below 2^24.

@@ -97,3 +97,96 @@ def test_long_rows(hip, dev, fmt, xdtype, n, rows, cols):
         g.mul_device(px, n, out) if not ps else g.mul_mxfp4_device(px, ps, n, out)
         check()
         g.close()
+
+
+def _kind(got, want):
+    """NaN where want is, infinities where want has them and of their sign; finite elsewhere."""
+    inf = np.isinf(want)
+    return (np.array_equal(np.isnan(got), np.isnan(want)) and np.array_equal(np.isinf(got), inf) and
+            np.array_equal(np.sign(got[inf]), np.sign(want[inf])))
+
+
+@pytest.mark.parametrize("xdtype", [W.F32, W.F16, W.BF16])
+@pytest.mark.parametrize("fmt", [W.MXFP4, W.BF16])
+@pytest.mark.parametrize("n,gate", [(3, False), (3, True), (300, False), (300, True)])
+def test_infinities_in_the_matrix(hip, dev, fmt, xdtype, n, gate):
+    """Infinities in a matrix (MXFP4: values past fp32's) give what fp32 products and sums give: infinities of either
+    sign, NaN from two of them or from zeros of x; other outputs, unnamed rows and other groups' rows are as without."""
+    rng = np.random.default_rng(n)
+    experts, rows, cols = 3, 70, 160
+    raws, ws = [], []
+    for phase in range(2 if gate else 1):
+        if fmt == W.MXFP4:
+            codes, scales = random_mx(rng, experts * rows, cols)
+            for r, block, s, c in ((5, 0, 254, 7), (5 + rows, 1, 254, 12), (9 + rows, 4, 253, 6), (11, 2, 254, 4), (20, 0, 254, 7)):
+                r += phase  # a pair's gate and up rows beside each other
+                scales[r, block] = s
+                codes[r, block * 32:block * 32 + 32] = 0
+                codes[r, block * 32 + 7] = c
+            codes[20 + phase, 8] = 15  # -6 beside 6
+            scales[30, 1], codes[30, 32:64] = 253, 5  # 3 * 2^126 is finite
+            codes[30, 33:64] = 0
+            raws.append(W.encode_mxfp4(codes, scales))
+            w = mx_values(codes, scales)
+        else:
+            bits, w = encode(W.BF16, rng.standard_normal((experts * rows, cols)) * 0.02)
+            for r, k, v in ((5, 7, np.inf), (5 + rows, 39, -np.inf), (9 + rows, 135, np.inf), (20, 7, np.inf), (20, 8, -np.inf)):
+                w[r + phase, k] = v
+                bits[r + phase, k] = 0x7f80 if v > 0 else 0xff80
+            raws.append(bits.reshape(-1).view(np.uint8))
+        with np.errstate(over="ignore"):
+            ws.append(w.astype(np.float32).astype(np.float64).reshape(experts, rows, cols))
+    x = rng.standard_normal((n, cols))
+    x[0, 7] = 0  # times an infinity: NaN
+    if n > 2:
+        x[2, 39] = -0.0
+    bits, x = encode(xdtype, x)
+    counts = [1, 0, 2] if n == 3 else [120, 90, 80]
+    m = sum(counts)
+    offsets = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+    index = rng.permutation(n).astype(np.int32)
+    index[m - 1] = -1
+    e = hip.Experts(fmt, experts, rows, cols, *raws)
+    out = dev.put(np.full((n, rows), 7, np.float32))
+    e.mul_device(xdtype, dev.put(bits), 0, cols, n, dev.put(offsets), dev.put(index), n, W.F32, out, rows)
+    got = dev.get(out, (n, rows))
+    e.close()
+    assert (got[m:] == 7).all() and (got[m - 1] == 0).all()
+    with np.errstate(all="ignore"):
+        for i in range(experts):
+            for r in range(offsets[i], min(offsets[i + 1], m - 1)):
+                # (the sums are fp32: those past its range are infinities before the gate sees them)
+                y = [(x[index[r]] * w[i]).sum(1) for w in ws]
+                y = [np.where(np.abs(v) > 3.41e38, np.sign(v) * np.inf, v) for v in y]
+                want = silu(y[0]) * y[1] if gate else y[0]
+                want = np.where(np.abs(want) > 3.41e38, np.sign(want) * np.inf, want)
+                assert _kind(got[r], want), (i, r)
+                ok = np.isfinite(want)
+                if gate:
+                    assert np.all(np.abs(got[r] - want)[ok] <= 1e-4 * (np.abs(want[ok]) + np.abs(y[1][ok])) + 1e-4)
+                else:
+                    tol = (cols + 128) * 2.0 ** -24 * (np.abs(x[index[r]]) * np.abs(ws[0][i])).sum(1)
+                    assert np.all((np.abs(got[r] - want) <= tol)[ok])
+
+
+@pytest.mark.parametrize("n", [4, 200])
+@pytest.mark.parametrize("fmt", [W.MXFP4, W.BF16])
+def test_smallest_values(hip, dev, fmt, n):
+    """fp32 rows down to subnormal values keep their bits from 2^-133 up (bf16's smallest number, of their last plane)."""
+    rng = np.random.default_rng(n)
+    rows, cols = 40, 256
+    if fmt == W.MXFP4:
+        codes, scales = random_mx(rng, rows, cols, 215, 225)
+        raw, w = W.encode_mxfp4(codes, scales), mx_values(codes, scales)
+    else:
+        bits, w = encode(W.BF16, rng.standard_normal((rows, cols)) * 2.0 ** 95)
+        raw = bits.reshape(-1).view(np.uint8)
+    x = (rng.standard_normal((n, cols)) * 2.0 ** -rng.integers(105, 135, (n, 1))).astype(np.float32)
+    e = hip.Experts(fmt, 1, rows, cols, raw)
+    out = dev.put(np.zeros((n, rows), np.float32))
+    e.mul_device(W.F32, dev.put(x), 0, cols, n, dev.put(np.array([0, n], np.int32)), 0, n, W.F32, out, rows)
+    got = dev.get(out, (n, rows))
+    e.close()
+    x = x.astype(np.float64)
+    tol = (cols + 128) * 2.0 ** -24 * (np.abs(x) @ np.abs(w).T) + 2.0 ** -133 * np.abs(w).sum(1)
+    assert np.all(np.abs(got - x @ w.T) <= tol)

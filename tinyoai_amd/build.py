@@ -24,7 +24,7 @@ ARCH = os.environ.get("TINYOAI_OFFLOAD_ARCH", "gfx950")
 MATVEC_FORMATS = ["q8_0", "bf16", "f32", "f16", "q5_1", "q4_k", "q5_k", "q6_k"]
 SOURCES = ["decode.hip", "api.cpp", "llama.cpp", "prefill.hip", "weights.hip", "gemm.hip", "gemm_q8.hip",
            "flash.hip", "logprobs.hip", "kq_rows.hip", "few_rows.hip", "gemm_exact.hip", "llama_tiny.hip",
-           "experts.cpp", "mx_quant.hip", "mx_few.hip", "mx_tiles.hip", "route.hip"] + [f"matvec_{f}.hip" for f in MATVEC_FORMATS]
+           "experts.cpp", "mx_quant.hip", "mx_few.hip", "mx_tiles.hip", "mx_infinite.hip", "route.hip"] + [f"matvec_{f}.hip" for f in MATVEC_FORMATS]
 FLAGS = ["-O3", "-std=c++17", "-fPIC", "-x", "hip", f"--offload-arch={ARCH}", "-ffp-contract=off",
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
          "-Wall", "-Wno-unused-function", "-Wno-unused-variable", "-Wno-unused-value", "-Wno-unused-result",

@@ -2317,7 +2317,7 @@ int tinyoai_stablelm_profile_read(tinyoai_model *m, double *ms, int64_t *counts,
 }
 
 int tinyoai_weight_upload(int32_t dtype, int64_t rows, int64_t cols, const void *data, uint64_t nbytes,
-                          tinyoai_weight **out) {
+                          tinyoai_weight **out) try {
   if (!out || !data) return fail(TINYOAI_EINVAL, "invalid weight upload arguments");
   *out = nullptr;
   auto w = std::make_unique<tinyoai_weight>();
@@ -2332,6 +2332,8 @@ int tinyoai_weight_upload(int32_t dtype, int64_t rows, int64_t cols, const void 
   if (e != hipSuccess) return hip_fail(e, "weight upload");
   *out = w.release();
   return TINYOAI_OK;
+} catch (const std::exception &e) {
+  return fail(TINYOAI_ENOMEM, "weight upload: %s", e.what());
 }
 
 int tinyoai_weight_read_values(tinyoai_weight *w, int64_t offset, int64_t n, float *out) {

@@ -2,10 +2,12 @@
 // products grouped by expert and the weighted sum of the experts' rows.
 #include "experts.h"
 
+#include <algorithm>
 #include <atomic>
 #include <climits>
 #include <exception>
 #include <memory>
+#include <vector>
 
 #include "stream_scratch.h"
 #include "tinyoai_hip.h"
@@ -16,7 +18,9 @@ bool mx_supported(const MxProduct &p) { return mx_few_supported(p) || mx_tiles_s
 size_t mx_scratch(const MxProduct &p) { return mx_few_supported(p) ? 0 : mx_tiles_scratch(p); }
 
 hipError_t launch_mx_product(const MxProduct &p, void *scratch, hipStream_t st) {
-  return mx_few_supported(p) ? launch_mx_few(p, st) : launch_mx_tiles(p, scratch, st);
+  const hipError_t e = mx_few_supported(p) ? launch_mx_few(p, st) : launch_mx_tiles(p, scratch, st);
+  if (e != hipSuccess || !p.w.infinite_rows || (p.xdtype != FMT_F32 && p.xdtype != FMT_F16)) return e;
+  return launch_mx_infinite_rows(p, st);
 }
 
 namespace tinyoai {
@@ -92,6 +96,7 @@ int StreamScratch::take(hipStream_t st, size_t bytes, ScratchPool::Lease *lease)
 // ---------------------------------------------------------------- matrices
 ExpertMatrix::~ExpertMatrix() {
   if (mem) hipFree(mem);
+  if (infinite) hipFree(infinite);
 }
 
 int check_matrices(int32_t dtype, int32_t experts, int64_t rows, int64_t cols, uint64_t nbytes, int64_t *each) {
@@ -125,18 +130,60 @@ int ExpertMatrix::upload(int32_t dtype, int32_t experts, int64_t rows, int64_t c
   m.codes = (const uint8_t *)mem;
   m.scales = (const uint8_t *)mem + codes;
   void *raw = nullptr;
-  e = device_alloc(&raw, each);
-  if (e != hipSuccess) return fail(TINYOAI_ENOMEM, "hipMalloc(%lld): %s", (long long)each, hipGetErrorString(e));
+  // behind the room for one matrix, a word for each: whether it holds an infinity
+  const size_t at = ((size_t)each + 3) / 4 * 4, phases = m.gate + 1;
+  std::vector<uint32_t> any(experts * phases);
+  const size_t raw_bytes = at + any.size() * 4;
+  e = device_alloc(&raw, raw_bytes);
+  if (e != hipSuccess) return fail(TINYOAI_ENOMEM, "hipMalloc(%zu): %s", raw_bytes, hipGetErrorString(e));
+  const std::unique_ptr<void, hipError_t (*)(void *)> free_raw(raw, hipFree);
+  uint8_t *matrix = (uint8_t *)raw;
+  uint32_t *any_dev = (uint32_t *)(matrix + at);
+  auto copy = [&](size_t i) {  // (of pairs, expert after expert, both)
+    return hipMemcpyAsync(raw, (const uint8_t *)(i % phases ? up : data) + i / phases * each, each, hipMemcpyHostToDevice, st);
+  };
+  auto fetch = [&](void *to, const void *from, size_t n) {
+    const hipError_t f = hipMemcpyAsync(to, from, n, hipMemcpyDeviceToHost, st);
+    return f == hipSuccess ? hipStreamSynchronize(st) : f;
+  };
   e = hipMemsetAsync(mem, 0, bytes, st);  // rows and columns past the matrix are zeros
-  for (int i = 0; i < experts; i++)
-    for (int phase = 0; phase <= m.gate; phase++) {
-      const uint8_t *src = (const uint8_t *)(phase ? up : data) + (size_t)i * each;
-      if (e == hipSuccess) e = hipMemcpyAsync(raw, src, each, hipMemcpyHostToDevice, st);
-      if (e == hipSuccess) e = launch_mx_place(m, (const uint8_t *)raw, i, phase, st);
-      if (e == hipSuccess) e = hipStreamSynchronize(st);  // the next copy takes the same buffer
-    }
-  hipFree(raw);
+  if (e == hipSuccess) e = hipMemsetAsync(any_dev, 0, any.size() * 4, st);
+  for (size_t i = 0; i < any.size(); i++) {
+    if (e == hipSuccess) e = copy(i);
+    if (e == hipSuccess) e = launch_mx_place(m, matrix, (int)(i / phases), (int)(i % phases), any_dev + i, st);
+    if (e == hipSuccess) e = hipStreamSynchronize(st);  // the next copy takes the same buffer
+  }
+  if (e == hipSuccess) e = fetch(any.data(), any_dev, any.size() * 4);
   if (e != hipSuccess) return hip_fail(e, "expert upload");
+  std::vector<int32_t> found;  // (expert, row) with an infinity
+  for (size_t i = 0; i < any.size(); i += phases) {
+    if (std::none_of(&any[i], &any[i] + phases, [](uint32_t v) { return v != 0; })) continue;
+    std::vector<uint8_t> flags(rows);
+    void *flags_dev = nullptr;
+    e = device_alloc(&flags_dev, rows);
+    if (e != hipSuccess) return fail(TINYOAI_ENOMEM, "hipMalloc(%lld): %s", (long long)rows, hipGetErrorString(e));
+    e = hipMemsetAsync(flags_dev, 0, rows, st);
+    for (size_t j = i; j < i + phases; j++) {
+      if (e == hipSuccess) e = copy(j);
+      if (e == hipSuccess) e = launch_mx_infinite(dtype, matrix, rows, cols, (uint8_t *)flags_dev, st);
+      if (e == hipSuccess) e = hipStreamSynchronize(st);
+    }
+    if (e == hipSuccess) e = fetch(flags.data(), flags_dev, rows);
+    hipFree(flags_dev);
+    if (e != hipSuccess) return hip_fail(e, "expert upload");
+    for (int64_t r = 0; r < rows; r++)
+      if (flags[r]) found.insert(found.end(), {(int32_t)(i / phases), (int32_t)r});
+  }
+  if (!found.empty()) {
+    if (found.size() / 2 > INT32_MAX) return fail(TINYOAI_EINVAL, "%zu rows with infinities", found.size() / 2);
+    e = device_alloc(&infinite, found.size() * 4);
+    if (e != hipSuccess) return fail(TINYOAI_ENOMEM, "hipMalloc(%zu): %s", found.size() * 4, hipGetErrorString(e));
+    e = hipMemcpyAsync(infinite, found.data(), found.size() * 4, hipMemcpyHostToDevice, st);
+    if (e == hipSuccess) e = hipStreamSynchronize(st);
+    if (e != hipSuccess) return hip_fail(e, "expert upload");
+    m.infinite = (const int32_t *)infinite;
+    m.infinite_rows = (int32_t)(found.size() / 2);
+  }
   d = m;
   return TINYOAI_OK;
 }

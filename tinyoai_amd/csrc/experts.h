@@ -9,7 +9,7 @@ namespace tinyoai {
 // `experts` matrices (or (gate, up) pairs) of one shape in the tiles of mx.h.
 struct ExpertMatrix {
   MxMat d{};
-  void *mem = nullptr;
+  void *mem = nullptr, *infinite = nullptr;
   ExpertMatrix() = default;
   ExpertMatrix(const ExpertMatrix &) = delete;
   ExpertMatrix &operator=(const ExpertMatrix &) = delete;

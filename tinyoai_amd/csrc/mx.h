@@ -44,6 +44,8 @@ struct MxMat {
   int32_t gate;             // (gate, up) pairs
   int32_t tiles;            // row tiles of an expert, a multiple of four
   int32_t chunks;           // column chunks
+  int32_t infinite_rows;    // (expert, output row) with an infinity in the matrix (of a pair, in either)
+  const int32_t *infinite;  // [infinite_rows][2]
 };
 
 __host__ __device__ inline int mx_chunk_cols(int fmt) { return fmt == FMT_MXFP4 ? 128 : 64; }
@@ -87,6 +89,16 @@ __device__ __forceinline__ float mx_code(uint32_t c) {
   const uint32_t m = c & 7;
   const float v = m < 2 ? 0.5f * (float)m : __uint_as_float(((m >> 1) + 126) << 23 | (m & 1) << 22);
   return c & 8 ? -v : v;
+}
+// Whether a raw bf16 value, or one of a raw MXFP4 block's, is an infinity in
+// fp32: codes 4 and 6 (2 and 4) times 2^127, 6 times 2^126.
+__device__ __forceinline__ bool mx_infinite(uint16_t bf16) { return (bf16 & 0x7fff) == 0x7f80; }
+__device__ __forceinline__ bool mx_infinite(const uint8_t *block) {
+  const uint32_t s = block[0], least = s == 254 ? 4 : 6;
+  bool inf = false;
+  if (s == 254 || s == 253)
+    for (int j = 1; j <= 16; j++) inf |= (block[j] & 7u) >= least || (block[j] >> 4 & 7u) >= least;
+  return inf;
 }
 // Value (row of the stored tiles, column) of expert e.
 __device__ __forceinline__ float mx_value(const MxMat &m, int e, int row, int col) {
@@ -153,8 +165,12 @@ struct MxProduct {
 };
 
 // Rows of one expert's GGUF tensor (raw, on the device) into its tiles; phase
-// 1: the up rows of pairs.
-hipError_t launch_mx_place(const MxMat &m, const uint8_t *raw, int expert, int phase, hipStream_t st);
+// 1: the up rows of pairs. *any becomes 1 if one of its values is an infinity.
+hipError_t launch_mx_place(const MxMat &m, const uint8_t *raw, int expert, int phase, uint32_t *any, hipStream_t st);
+// flags[row] = 1 for the rows of a raw matrix with an infinity.
+hipError_t launch_mx_infinite(int fmt, const uint8_t *raw, int64_t rows, int64_t cols, uint8_t *flags, hipStream_t st);
+// The outputs of the rows p.w.infinite, after the product of fp32 or fp16 rows.
+hipError_t launch_mx_infinite_rows(const MxProduct &p, hipStream_t st);
 // Values [offset, offset + n) of a single matrix, row-major.
 hipError_t launch_mx_read(const MxMat &m, int64_t offset, int64_t n, float *out, hipStream_t st);
 hipError_t launch_mx_quantize(int dtype, const void *x, int64_t ldx, int64_t n, int64_t cols, uint8_t *codes,

@@ -106,7 +106,7 @@ __global__ __launch_bounds__(kT) void dequantize_kernel(const uint32_t *codes, c
 // GGUF rows -> tiles. MXFP4 blocks are {scale, 16 bytes}, byte j the codes of
 // values j (low) and j + 16; BF16 rows are plain values.
 __global__ __launch_bounds__(kT) void place_mxfp4_kernel(MxMat m, uint8_t *codes, uint8_t *scales, const uint8_t *raw,
-                                                         int phase) {
+                                                         int phase, uint32_t *any) {
   const int64_t nb = m.cols / 32, total = m.rows * nb;
   for (int64_t i = blockIdx.x * (int64_t)kT + threadIdx.x; i < total; i += (int64_t)gridDim.x * kT) {
     const int row = mx_stored_row(m, (int)(i / nb), phase), col = (int)(i % nb) * 32;
@@ -118,13 +118,15 @@ __global__ __launch_bounds__(kT) void place_mxfp4_kernel(MxMat m, uint8_t *codes
       dst[j + 8] = (uint8_t)((a >> 4) | (b >> 4) << 4);
     }
     scales[mx_scale_at(m, row, col)] = src[0];
+    if (mx_infinite(src)) *any = 1;
   }
 }
-__global__ __launch_bounds__(kT) void place_bf16_kernel(MxMat m, uint8_t *codes, const uint16_t *raw, int phase) {
+__global__ __launch_bounds__(kT) void place_bf16_kernel(MxMat m, uint8_t *codes, const uint16_t *raw, int phase, uint32_t *any) {
   const int64_t total = (int64_t)m.rows * m.cols;
   for (int64_t i = blockIdx.x * (int64_t)kT + threadIdx.x; i < total; i += (int64_t)gridDim.x * kT) {
     const int row = mx_stored_row(m, (int)(i / m.cols), phase), col = (int)(i % m.cols);
     *reinterpret_cast<uint16_t *>(codes + mx_code_at(m, row, col)) = raw[i];
+    if (mx_infinite(raw[i])) *any = 1;
   }
 }
 
@@ -169,15 +171,15 @@ hipError_t launch_mx_dequantize(const uint8_t *codes, const uint8_t *scales, int
   return hipGetLastError();
 }
 
-hipError_t launch_mx_place(const MxMat &m, const uint8_t *raw, int expert, int phase, hipStream_t st) {
+hipError_t launch_mx_place(const MxMat &m, const uint8_t *raw, int expert, int phase, uint32_t *any, hipStream_t st) {
   uint8_t *codes = const_cast<uint8_t *>(m.codes) + expert * mx_code_bytes(m);
   uint8_t *scales = const_cast<uint8_t *>(m.scales) + expert * mx_scale_bytes(m);
   if (m.fmt == FMT_MXFP4)
     hipLaunchKernelGGL(place_mxfp4_kernel, dim3(blocks_for((int64_t)m.rows * m.cols / 32)), dim3(kT), 0, st, m, codes,
-                       scales, raw, phase);
+                       scales, raw, phase, any);
   else
     hipLaunchKernelGGL(place_bf16_kernel, dim3(blocks_for((int64_t)m.rows * m.cols)), dim3(kT), 0, st, m, codes,
-                       reinterpret_cast<const uint16_t *>(raw), phase);
+                       reinterpret_cast<const uint16_t *>(raw), phase, any);
   return hipGetLastError();
 }
 
