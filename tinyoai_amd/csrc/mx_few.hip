@@ -41,8 +41,6 @@ __device__ __forceinline__ uint4 load16(__amdgpu_buffer_rsrc_t r, uint32_t at) {
   return make_uint4(v.x, v.y, v.z, v.w);
 }
 
-constexpr int kMostChunks = 4;  // of a wave
-
 struct FewArgs {
   MxProduct p;
   int units;  // tiles (pairs: of both) of an expert
@@ -281,8 +279,6 @@ __global__ __launch_bounds__(kWaves * 64) void few_kernel(FewArgs g) {
   }
 }
 
-int groups(const MxProduct &p) { return p.offsets ? std::min(p.w.experts, p.n) : 1; }
-
 int64_t x_bytes(const MxProduct &p) {
   if (p.xdtype == FMT_MXFP4) return (int64_t)p.x_rows * p.w.chunks * 64;
   return ((int64_t)(p.x_rows - 1) * p.ldx + p.w.cols) * (int64_t)mx_width(p.xdtype);
@@ -297,7 +293,7 @@ hipError_t launch(FewArgs &g, hipStream_t st) {
   // rows of groups, which cost little and are uneven (16 tokens' gate and up of
   // 32 experts 21.9 us instead of 23.6).
   const int64_t blocks = (int64_t)device_cu_count() * (XM == 0 && p.offsets ? 2 : 1);
-  g.per = (int)std::max<int64_t>(1, ((int64_t)groups(p) * g.units + blocks - 1) / blocks);
+  g.per = (int)std::max<int64_t>(1, (tinyoai_rule::groups(mx_sizes(p)) * g.units + blocks - 1) / blocks);
   // a group's rows past the first kRows have blocks of their own
   const int rows = 16 * CT / (XM == 0 ? 1 : XM);
   const dim3 grid((g.units + g.per - 1) / g.per, p.offsets ? p.w.experts : 1, std::min((p.n + rows - 1) / rows, p.offsets ? 4 : 1));
@@ -307,23 +303,19 @@ hipError_t launch(FewArgs &g, hipStream_t st) {
 
 }  // namespace
 
-// Whether the few-row kernel takes the product: its rows fill one or two
-// column tiles (one, with sixteen waves), its columns no more than four chunks
-// of sixteen waves (pairs and planes: of eight, or registers spill), X comes in
-// whole 16-byte pieces, and offsets within X and a matrix fit 31 bits.
+// Whether the few-row kernel takes the product: by its sizes (mx_rule.h), and X
+// comes in whole 16-byte pieces, and offsets within X and a matrix fit 31 bits.
 bool mx_few_supported(const MxProduct &p) {
   const bool pieces = p.xdtype == FMT_MXFP4 || (p.w.cols % 8 == 0 && p.ldx * mx_width(p.xdtype) % 16 == 0 &&
                                                 reinterpret_cast<uintptr_t>(p.x) % 16 == 0);
-  const int waves = p.w.gate && p.xdtype != FMT_MXFP4 ? 8 : 16;
-  return p.w.chunks <= waves * kMostChunks && pieces && x_bytes(p) < kNone && mx_code_bytes(p.w) < kNone &&
-         (int64_t)p.n * mx_planes(p.xdtype) <= (int64_t)groups(p) * (p.w.chunks <= 8 * kMostChunks ? 32 : 16);
+  return pieces && x_bytes(p) < kNone && mx_code_bytes(p.w) < kNone && tinyoai_rule::few_rows(mx_sizes(p));
 }
 
 hipError_t launch_mx_few(const MxProduct &p, hipStream_t st) {
   FewArgs g{p};
   g.x_bytes = x_bytes(p);
-  // column tiles: one for a dense product of few rows; groups are uneven
-  const bool two = (int64_t)p.n * mx_planes(p.xdtype) > (p.offsets ? 4 : 16) * (int64_t)groups(p);
+  const tinyoai_rule::Few form = tinyoai_rule::few_form(mx_sizes(p));
+  const bool two = form.column_tiles == 2;
   using std::integral_constant;
   auto go = [&](auto wf, auto xm) {
     constexpr int WF = decltype(wf)::value, XM = decltype(xm)::value;
@@ -338,8 +330,8 @@ hipError_t launch_mx_few(const MxProduct &p, hipStream_t st) {
     const integral_constant<int, 3> three;
     const integral_constant<int, 4> four;
     const integral_constant<int, 8> eight;
-    if (p.w.chunks > 8 * 4) return gated(integral_constant<int, 16>(), one, four);
-    if (p.w.chunks > 8 * 3) return two ? gated(eight, both, four) : gated(eight, one, four);
+    if (form.waves == 16) return gated(integral_constant<int, 16>(), one, four);
+    if (form.wave_chunks == 4) return two ? gated(eight, both, four) : gated(eight, one, four);
     return two ? gated(eight, both, three) : gated(eight, one, three);
   };
   const int xm = p.xdtype == FMT_MXFP4 ? 0 : mx_planes(p.xdtype);

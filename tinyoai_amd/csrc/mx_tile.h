@@ -5,9 +5,16 @@
 #include <type_traits>
 
 #include "mx.h"
+#include "mx_rule.h"
 
 // bf16 planes that hold a type's values exactly (MXFP4: none).
 __host__ __device__ inline int mx_planes(int dtype) { return dtype == FMT_F32 ? 3 : dtype == FMT_F16 ? 2 : 1; }
+
+// What the rules see of a product.
+inline tinyoai_rule::Sizes mx_sizes(const MxProduct &p) {
+  return {p.w.fmt == FMT_BF16, p.xdtype == FMT_MXFP4 ? 0 : mx_planes(p.xdtype), p.w.gate != 0, p.offsets != nullptr,
+          p.w.experts, p.n, p.w.rows, p.w.cols};
+}
 
 namespace tinyoai_mx {
 

@@ -42,6 +42,7 @@
 namespace {
 
 using namespace tinyoai_mx;
+using namespace tinyoai_rule;
 
 constexpr int kBand = 8;
 // Offsets within a buffer are below 2^31; kNone and what is added to it, and
@@ -49,20 +50,6 @@ constexpr int kBand = 8;
 // the buffer's first bytes, for a step that is not multiplied.)
 constexpr uint32_t kNone = 0x80000000u, kPast = 0x80000000u;
 constexpr int64_t kExtent = (int64_t)1 << 31;
-
-// A chain of sums on the matrix cores rounds at every 16 columns of each plane
-// (MXFP4 rows: 64), and its error grows with the root of its length: relative to
-// float64, in the norm, fp32 rows times MXFP4 4.5e-7 at 2560 columns, 1.2e-6
-// at 16384, 2.3e-6 at 65536. Long rows (chain_cols) go to totals a run of
-// columns at a time: 2.8, 3.1 and 3.4e-7. Totals take as many registers as the
-// sums, which costs the short rows 1 to 6%, and 21% where it leaves a CU fewer blocks
-// (64 experts' pairs of MXFP4, bf16 rows).
-constexpr int kRunBf16 = 1024, kRunMx = 8192;
-// Columns of one chain, at most: for fp32 rows what keeps the error near that of
-// fp32 sums of 512 columns (5e-7); bf16 rows' inputs are rounded to eight bits already.
-constexpr int chain_cols(int planes) { return planes == 0 ? 65536 : planes == 1 ? 16384 : 8192 / planes; }
-// Past these the totals' own chain counts: the smallest tiles, whose totals are doubles.
-constexpr int kFloatTotals = 1 << 18;
 
 struct TileArgs {
   MxProduct p;
@@ -546,7 +533,7 @@ hipError_t launch(TileArgs &g, hipStream_t st) {
   static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (attr != hipSuccess) return attr;
   // row tiles there can be: one more for each group than its rows fill
-  const int64_t groups = p.offsets ? std::min(p.w.experts, p.n) : 1;
+  const int64_t groups = tinyoai_rule::groups(mx_sizes(p));
   const int64_t mtiles = p.offsets ? (p.n + groups * (BM - 1)) / BM : (p.n + BM - 1) / BM;
   const int64_t blocks = (mtiles * ((p.w.tiles * 16 + BN - 1) / BN) + 7) / 8 * 8;
   hipLaunchKernelGGL(kernel, dim3((unsigned)blocks, BM == 32 ? g.ks : 1), dim3(WAVES * 64), bytes, st, g);
@@ -555,18 +542,8 @@ hipError_t launch(TileArgs &g, hipStream_t st) {
 
 }  // namespace
 
-// A weight's product whose smallest tiles leave half of the CUs without a block
-// is cut over the columns, into parts of 8 steps at least, for a block a CU; the
-// parts' sums are added by a launch of their own, which a short K does not repay
-// (whole and in parts: fp32 rows, 128 x 1000, K = 4096, 33 and 17.6 us; 12 x 4096,
-// K = 6912, 46 and 16; 48 x 2560, K = 2560, 22 and 16; 64 x 1024, K = 1024, 12.5
-// and 12.7; MXFP4 rows, 100 x 500, K = 6912, 19 and 13.5; 400 x 1024, K = 2560,
-// 11.3 and 13.1). The sums take 4 MiB at most.
 static int parts_of(const MxProduct &p) {
-  const int cols = p.xdtype == FMT_MXFP4 ? 128 : 64, steps = (p.w.cols + cols - 1) / cols;
-  if (p.offsets || p.w.gate || p.odtype != FMT_F32 || p.ldo != p.w.rows || steps < 32) return 1;
-  const int64_t blocks = (int64_t)((p.n + 31) / 32) * ((p.w.tiles * 16 + 127) / 128);
-  return (int)std::max<int64_t>(1, std::min<int64_t>(device_cu_count() / blocks, steps / 8));
+  return p.odtype == FMT_F32 && p.ldo == p.w.rows ? parts(mx_sizes(p), device_cu_count()) : 1;
 }
 static size_t planes_bytes(const MxProduct &p) {
   if (p.xdtype == FMT_MXFP4 || direct(p)) return 0;
@@ -582,7 +559,7 @@ size_t mx_tiles_scratch(const MxProduct &p) {
 // are (kMxCols columns at most); the threads of a launch number below 2^32, with
 // the smallest tiles too.
 bool mx_tiles_supported(const MxProduct &p) {
-  const int64_t groups = p.offsets ? std::min(p.w.experts, p.n) : 1;
+  const int64_t groups = tinyoai_rule::groups(mx_sizes(p));
   return (p.xdtype != FMT_MXFP4 || (int64_t)p.x_rows * 64 <= kExtent) &&
          (p.n + groups * 31) / 32 * (((int64_t)p.w.tiles * 16 + 127) / 128) < (int64_t)1 << 24;
 }
@@ -618,57 +595,35 @@ hipError_t launch_mx_tiles(const MxProduct &p, void *scratch, hipStream_t st) {
       if (e != hipSuccess) return e;
     }
   }
-  // The largest tiles that give most CUs a block, and of groups no taller than
-  // their rows need (BM x BN, measured at K = 2560; "rows" of each group on
-  // average):
-  //   6912 outputs, MXFP4 rows: 64 rows 8.1 us with 32 x 128, 12.3 with 64 x
-  //   256; 256 rows 10.3 with 64 x 128, 11.7 and 12.9; 1024 rows 19.5 with 64 x
-  //   256, 24.7 with 64 x 128; fp32 rows 25 and 47, 39 and 52, 98 and 112;
-  //   64 pairs of 1728: fp32, 16 rows: 124 with 32 x 128, 152 with 64 x 256,
-  //   64 rows: 270 and 248; MXFP4, 64 rows: 79 with 64 x 256, 78 with 128 x 256,
-  //   256 rows: 181 and 163;
-  //   BF16, 32 pairs: 32 rows 110 with 64 x 256, 113 with 128 x 256, 128 rows: 180
-  //   and 151; 8 experts of 2560 x 1728, 512 rows: 60 and 51 with 256 x 256.
-  const int64_t groups = p.offsets ? std::min(p.w.experts, p.n) : 1, rows = p.n / groups;
-  const int64_t cus = device_cu_count(), stored = p.w.tiles * 16;
-  auto blocks = [&](int bm, int bn) { return groups * ((rows + bm - 1) / bm) * ((stored + bn - 1) / bn); };
-  auto fills = [&](int bm, int bn) { return blocks(bm, bn) * 4 >= cus * 3; };
-  const bool mx = p.xdtype == FMT_MXFP4, bf16 = p.w.fmt == FMT_BF16;
-  const int planes = mx_planes(p.xdtype);
-  const bool low = p.offsets && planes > 1 && rows <= 24;  // (one plane: the matrix's loads count for more)
-  const int cols = p.w.cols, chain = chain_cols(mx ? 0 : planes);
+  const int planes = p.xdtype == FMT_MXFP4 ? 0 : mx_planes(p.xdtype);
+  const Tile t = tile(mx_sizes(p), g.ks, device_cu_count());
   auto go = [&](auto wf, auto xm) {
     constexpr int WF = decltype(wf)::value, XM = decltype(xm)::value;
     constexpr bool B = WF == FMT_BF16, Q = XM == 0;
-    auto tiles = [&](auto runs) {
+    if constexpr (B && XM == 1)
+      if (t.bm == 256) return launch<WF, XM, 256, 256, 8, 4, 2>(g, st);
+    if constexpr (Q)
+      if (t.bm == 128) return launch<WF, XM, 128, 256, 4, 2, 3>(g, st);
+    auto of = [&](auto runs) {
       constexpr bool R = decltype(runs)::value;
-      if constexpr (!R) {  // (no registers for totals)
-        if constexpr (B && XM == 1)
-          if (rows >= 384 && fills(256, 256)) return launch<WF, XM, 256, 256, 8, 4, 2>(g, st);
-        if constexpr (Q)
-          if (rows >= 128 && fills(128, 256)) return launch<WF, XM, 128, 256, 4, 2, 3>(g, st);
-      }
       if constexpr (B)
-        if (rows >= 96 && fills(128, 256)) return launch<WF, XM, 128, 256, 8, 2, XM == 1 ? 3 : 2, R>(g, st);
-      if (!low && fills(64, 256)) return launch<WF, XM, 64, 256, 4, 1, Q ? 3 : 2, R>(g, st);
-      return launch<WF, XM, 64, 128, 4, 2, Q || (XM == 1 && !B) ? 6 : XM == 3 ? 2 : 3, R>(g, st);
+        if (t.bm == 128) return launch<WF, XM, 128, 256, 8, 2, XM == 1 ? 3 : 2, R>(g, st);
+      if (t.bm == 64 && t.bn == 256) return launch<WF, XM, 64, 256, 4, 1, Q ? 3 : 2, R>(g, st);
+      if (t.bm == 64) return launch<WF, XM, 64, 128, 4, 2, Q || (XM == 1 && !B) ? 6 : XM == 3 ? 2 : 3, R>(g, st);
+      return launch<WF, XM, 32, 128, 4, 1, Q ? 6 : B ? 5 - XM : XM == 1 ? 8 : 4, R>(g, st);
     };
-    if (cols <= kFloatTotals && !low && (fills(64, 256) || fills(64, 128)))
-      return cols > chain ? tiles(std::true_type()) : tiles(std::false_type());
-    // (a wave has four chains of sums, two of MXFP4 rows)
-    constexpr int kStages = Q ? 6 : B ? 5 - XM : XM == 1 ? 8 : 4;
-    return cols / g.ks > chain * (Q ? 2 : 4) ? launch<WF, XM, 32, 128, 4, 1, kStages, true>(g, st) : launch<WF, XM, 32, 128, 4, 1, kStages>(g, st);
+    return t.runs ? of(std::true_type()) : of(std::false_type());
   };
   using std::integral_constant;
   hipError_t e;
-  if (bf16) {
+  if (p.w.fmt == FMT_BF16) {
     const integral_constant<int, FMT_BF16> wf;
     e = planes == 1   ? go(wf, integral_constant<int, 1>())
         : planes == 2 ? go(wf, integral_constant<int, 2>())
                       : go(wf, integral_constant<int, 3>());
   } else {
     const integral_constant<int, FMT_MXFP4> wf;
-    e = mx            ? go(wf, integral_constant<int, 0>())
+    e = planes == 0   ? go(wf, integral_constant<int, 0>())
         : planes == 1 ? go(wf, integral_constant<int, 1>())
         : planes == 2 ? go(wf, integral_constant<int, 2>())
                       : go(wf, integral_constant<int, 3>());

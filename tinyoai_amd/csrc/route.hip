@@ -21,8 +21,11 @@
 #include <algorithm>
 
 #include "mx.h"
+#include "mx_rule.h"
 
 namespace {
+
+using namespace tinyoai_rule;
 
 // The order of logits as unsigned numbers; 0: never chosen.
 __device__ __forceinline__ uint32_t rank_of(float v) {
@@ -103,7 +106,8 @@ __global__ __launch_bounds__(256) void choose_kernel(RouteArgs a) {
 }
 
 // Block e: offsets[e + 1] and expert e's rows.
-constexpr int kSortT = 1024, kSortWaves = kSortT / 64, kSortSlots = kSortT * 8;  // a round of loads
+constexpr int kSortT = 1024, kSortWaves = kSortT / 64;
+static_assert(kSortSlots == kSortT * 8, "a round of loads");
 __global__ __launch_bounds__(kSortT) void sort_kernel(RouteArgs a) {
   __shared__ uint32_t counts[3][kSortWaves];
   const int e = blockIdx.x, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -267,7 +271,6 @@ __global__ __launch_bounds__(256) void tokens_kernel(RouteArgs a) {
 }
 
 // A few tokens: both steps in one block.
-constexpr int kFewSlots = 256, kFewTokens = 32;
 template <int EI>
 __global__ __launch_bounds__(1024) void route_few_kernel(RouteArgs a) {
   __shared__ __align__(16) int32_t ids[kFewSlots];
@@ -307,12 +310,13 @@ __global__ __launch_bounds__(1024) void route_few_kernel(RouteArgs a) {
 
 template <int EI>
 void launch(const RouteArgs &a, hipStream_t st) {
-  if (a.n <= kFewTokens && a.n * a.k <= kFewSlots) {
+  const Sort path = sort_path(a.n, a.k);
+  if (path == Sort::one_block) {
     hipLaunchKernelGGL(route_few_kernel<EI>, dim3(1), dim3(1024), 0, st, a);
     return;
   }
   const int slots = a.n * a.k;
-  if (slots <= kSortSlots) {
+  if (path == Sort::by_expert) {
     hipLaunchKernelGGL(choose_kernel<EI>, dim3((a.n + 3) / 4), dim3(256), 0, st, a);
     hipLaunchKernelGGL(sort_kernel, dim3(a.experts), dim3(kSortT), 0, st, a);
     return;
@@ -395,11 +399,13 @@ __global__ __launch_bounds__(256) void combine_kernel(CombineArgs a, int per) {
 }  // namespace
 
 hipError_t launch_route(const RouteArgs &a, hipStream_t st) {
-  if (a.experts <= 64) launch<1>(a, st);
-  else if (a.experts <= 128) launch<2>(a, st);
-  else if (a.experts <= 256) launch<4>(a, st);
-  else if (a.experts <= 512) launch<8>(a, st);
-  else launch<16>(a, st);
+  switch (lane_experts(a.experts)) {
+    case 1: launch<1>(a, st); break;
+    case 2: launch<2>(a, st); break;
+    case 4: launch<4>(a, st); break;
+    case 8: launch<8>(a, st); break;
+    default: launch<16>(a, st);
+  }
   return hipGetLastError();
 }
 
