@@ -4,6 +4,7 @@
 #pragma once
 
 #include <algorithm>
+#include <cmath>
 #include <cstdint>
 
 namespace tinyoai_rule {
@@ -85,7 +86,15 @@ struct Tile {
 //   64 rows: 270 and 248; MXFP4, 64 rows: 79 with 64 x 256, 78 with 128 x 256,
 //   256 rows: 181 and 163;
 //   BF16, 32 pairs: 32 rows 110 with 64 x 256, 113 with 128 x 256, 128 rows: 180
-//   and 151; 8 experts of 2560 x 1728, 512 rows: 60 and 51 with 256 x 256.
+//   and 151.
+// BF16 matrices and rows, 256 x 256 against 128 x 256: one block of either fills
+// a CU, and the larger one takes 0.87 of the smaller's time for a product, so it
+// is taken where its rounds of blocks are no more than half as many (groups have
+// half a tile more on average). us, experts x rows of each:
+//   rounds 1 and 2: 8 x 512 of 2560 x 1728, 49 and 57; 8 x 256 of 3584 x 4096, 89 and 102;
+//     one of 4096, 4096 x 4096, 118 and 130; 4 and 8: 8 x 2048 of 3584 x 2560, 284 and 318;
+//   rounds 2 and 3: 8 x 1024 of 2560 x 1728, 96 and 92; 8 x 400 of 5120 x 2560, 124 and 113;
+//     2 and 2: 8 x 512 of 3584 x 2560, 123 and 90; 1 and 1: 4 x 1024 of 1792 x 4096, 84 and 64.
 inline Tile tile(const Sizes &s, int ks, int cus) {
   const int64_t g = groups(s), rows = s.n / g, stored = stored_rows(s);
   auto fills = [&](int bm, int bn) { return g * ((rows + bm - 1) / bm) * ((stored + bn - 1) / bn) * 4 >= cus * 3; };
@@ -94,7 +103,11 @@ inline Tile tile(const Sizes &s, int ks, int cus) {
   if (s.cols <= kFloatTotals && !low && (fills(64, 256) || fills(64, 128))) {
     const bool runs = s.cols > chain;
     if (!runs) {  // (no registers for totals)
-      if (s.bf16 && s.planes == 1 && rows >= 384 && fills(256, 256)) return {256, 256, false};
+      auto rounds = [&](int bm) {
+        const double tiles = g == 1 ? (double)((rows + bm - 1) / bm) : (double)rows / bm + 0.5;
+        return std::ceil(g * tiles * (double)((stored + 255) / 256) / cus);
+      };
+      if (s.bf16 && s.planes == 1 && rows >= 256 && 2 * rounds(256) <= rounds(128)) return {256, 256, false};
       if (s.planes == 0 && rows >= 128 && fills(128, 256)) return {128, 256, false};
     }
     if (s.bf16 && rows >= 96 && fills(128, 256)) return {128, 256, runs};
