@@ -190,3 +190,20 @@ def test_smallest_values(hip, dev, fmt, n):
     x = x.astype(np.float64)
     tol = (cols + 128) * 2.0 ** -24 * (np.abs(x) @ np.abs(w).T) + 2.0 ** -133 * np.abs(w).sum(1)
     assert np.all(np.abs(got - x @ w.T) <= tol)
+
+
+@pytest.mark.parametrize("n,rows,cols", [(131072, 40, 32), (2080, 100, 2016), (32767, 20, 128), (43690, 36, 96)])
+def test_largest_products_without_allocation(hip, dev, n, rows, cols):
+    """MXFP4 weights with as many rows as the no-allocation array holds (n * cols up to 2^22; at 32 columns the planes
+    fill it, at 2016 the parts' sums lie behind them): the same bits as with allocation."""
+    rng = np.random.default_rng(cols)
+    raw, _ = matrices(rng, W.MXFP4, 1, rows, cols)
+    w = hip.Weight(W.Tensor(W.MXFP4, rows, cols, raw))
+    x, out = dev.put(rng.standard_normal((n, cols)).astype(np.float32)), dev.put(np.full((n, rows), np.nan, np.float32))
+    w.mul_device(x, n, out)
+    want = dev.get(out, (n, rows)).copy()
+    assert np.isfinite(want).all() and want.std() > 0
+    dev.fill(out, np.full((n, rows), np.nan, np.float32))
+    w.mul_device_noalloc(x, n, out)
+    assert np.array_equal(dev.get(out, (n, rows)), want)
+    w.close()

@@ -2503,9 +2503,13 @@ int tinyoai_weight_mul_mxfp4_device(tinyoai_weight *w, const uint8_t *codes_dev,
 constexpr size_t kScratchValues = (size_t)4 << 20;  // activation values per call (n * cols)
 // operand planes (two of 16 bits: 16 MiB; fp16 planes of rows that are no
 // multiple of 32 columns up to 24), then the K-split partials in what is left,
-// at most 32 MiB
+// at most 32 MiB. MXFP4 weights: three planes of rows padded to 64 columns, 24 MiB, at 32
+// columns all 48; products in parts, of 2016 columns and more (parts of csrc/mx_rule.h),
+// at most 24.4 and their sums' 4.
 static __device__ __align__(256) uint16_t scratch[kProductScratchBytes / 2];
 static_assert(2 * kScratchValues * 2 + kProductPartialBytes <= kProductScratchBytes, "planes, then partials");
+static_assert(3 * 2 * (2 * kScratchValues) <= kProductScratchBytes, "three planes of rows twice as long");
+static_assert(3 * 2 * (kScratchValues / 2016 * 2048) + (4 << 20) <= kProductScratchBytes, "three planes and the parts' sums");
 
 namespace {
 constexpr int kMaxDevices = 64;
