@@ -82,3 +82,14 @@ def test_every_routing_form(rule):
     got = rule([f"r {n} {experts} {k}" for _, n, experts, k in F.ROUTES])
     assert got == [form for form, *_ in F.ROUTES]
     assert {form for form, *_ in F.ROUTES} == {(p, e) for p in ("one_block", "by_expert", "by_tokens") for e in (1, 2, 4, 8, 16)}
+
+
+def test_many_experts_leave_the_streaming_kernel(rule):
+    """32 experts and more of large matrices at half of the rows: their groups may be uneven."""
+    def form(experts, n, rows=1728, cols=2560, xd=W.BF16):
+        return rule([_line(W.MXFP4, xd, True, True, experts, n, rows, cols)])[0][0]
+
+    assert [form(64, 16 * 64), form(64, 16 * 64 + 1), form(64, 32 * 64)] == ["few", "tile", "tile"]
+    assert [form(64, 16 * 64 // 3, xd=W.F32), form(64, 16 * 64 // 3 + 1, xd=W.F32)] == ["few", "tile"]
+    assert [form(8, 32 * 8), form(8, 32 * 8 + 1)] == ["few", "tile"]
+    assert [form(32, 32 * 32, 256, 1024), form(32, 32 * 32 + 1, 256, 1024)] == ["few", "tile"]

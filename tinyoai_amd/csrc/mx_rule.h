@@ -28,10 +28,21 @@ constexpr int kMostChunks = 4;  // of a wave
 // Whether the rows fill one or two column tiles (one, with sixteen waves), and
 // the columns are no more than four chunks of sixteen waves (pairs and planes:
 // of eight, or registers spill).
+// 32 experts and more of large matrices: half of that on average. A group with more
+// rows than the tiles hold is streamed again for each, by the few blocks that one
+// expert has, so uneven groups cost much here, and little on the tiles of many rows.
+// us, streamed and tiled, with 20 and with 32 operand columns a group (rows times
+// planes), at random / of a popularity as 1 / i^1.5:
+//   64 pairs of 1728 x 2560, MXFP4, fp32: 92 104 / 202 95, 100 112 / 319 115; bf16: 66 78 / 216 72,
+//     93 81 / 345 95; MXFP4 rows: 54 54 / 120 51, 77 56 / 177 67;
+//   128 of 512 x 512, MXFP4, fp32: 36 25 / 160 22, 42 26 / 256 27; BF16, bf16: 29 25 / 156 33, 46 27 / 241 36;
+//   16 of 2560 x 1728, MXFP4, bf16: 14 20 / 24 20, 23 20 / 34 20; 8 pairs of 1728 x 2560, fp32: 18 24 / 25 24,
+//     27 25 / 29 25; small, 32 of 256 x 1024, fp32: 10 14 / 14 14, 11 14 / 22 15.
 inline bool few_rows(const Sizes &s) {
   const int waves = s.gate && s.planes ? 8 : 16;
+  const bool large = groups(s) >= 32 && groups(s) * stored_rows(s) * s.cols > 1 << 25;
   return chunks(s) <= waves * kMostChunks &&
-         s.n * std::max(s.planes, 1) <= groups(s) * (chunks(s) <= 8 * kMostChunks ? 32 : 16);
+         s.n * std::max(s.planes, 1) <= groups(s) * (chunks(s) > 8 * kMostChunks || large ? 16 : 32);
 }
 struct Few {
   int waves, column_tiles, wave_chunks;
