@@ -123,17 +123,17 @@ __device__ __forceinline__ void mx_store(int dtype, void *p, int64_t i, float v)
 // place at most where the gate is a normal number: e^x is 2^t (1 + r ln 2), t the rounded x log2 e
 // and r what it lacks, by the hardware's 2^t and reciprocal, one unit each (64
 // experts' pairs times 16384 MXFP4 rows, K = 2560, 167 us with expf and a
-// division, 156 so). The hardware's reciprocal is zero where it would be
+// division, 155 so). The hardware's reciprocal is zero where it would be
 // subnormal, from 1 + e^x = 2^126 on: past t = 64 both terms are taken 2^-64
 // times as large, and the quotient with them. |x| is held at 200, where that
 // e^x is infinite or zero too.
 __device__ __forceinline__ float mx_gate(float g, float u) {
   const float x = fminf(fmaxf(-g, -200.f), 200.f), t = x * 1.44269502f;
-  const float r = fmaf(x, 1.44269502f, -t) + x * 1.92596303e-8f;  // log2 e = 1.44269502 + 1.93e-8
+  const float r = fmaf(x, 1.92596303e-8f, fmaf(x, 1.44269502f, -t));  // log2 e = 1.44269502 + 1.93e-8
   const bool far = t > 64.f;
   const float one = far ? 0x1p-64f : 1.f;
-  const float e = __builtin_amdgcn_exp2f(far ? t - 64.f : t) * fmaf(r, 0.693147182f, 1.f);
-  return g * __builtin_amdgcn_rcpf(one + e) * one * u;
+  const float e = __builtin_amdgcn_exp2f(far ? t - 64.f : t);
+  return g * __builtin_amdgcn_rcpf(fmaf(e, fmaf(r, 0.693147182f, 1.f), one)) * one * u;
 }
 
 // Sixteen (eight) bytes at an address of a value's alignment alone: the card
