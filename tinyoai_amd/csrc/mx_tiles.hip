@@ -18,7 +18,9 @@
 // (one 256 x 256 block a CU of the same wave tiles 235 us, of larger ones 258).
 // 16384 MXFP4 rows of 64 experts' pairs, 1728 x 2560, 145 us: cores busy 33%, groups'
 // last row tiles and the gate on top. 4096 bf16 rows, 8 BF16 experts of 2560 x
-// 1728, 55 us: cores busy 48%, 0.66 PFLOP/s, three rounds of blocks at most.
+// 1728, 48 us: cores busy 60%, 0.76 PFLOP/s, one round of 160 blocks for 256 CUs.
+//
+// Long rows: the sums of runs of columns go to totals (RUNS; mx_rule.h).
 //
 //   planes of X (1, 2 or 3, bf16; mx_tile.h) times BF16, or times MXFP4 codes
 //   that become bf16 times their scale as a wave reads them (exact): 64
