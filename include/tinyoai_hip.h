@@ -389,6 +389,99 @@ int tinyoai_experts_mul_device(tinyoai_experts *e, int32_t x_dtype, const void *
                                int32_t n, int32_t out_dtype, void *out_dev, int64_t ldo, void *stream);
 int tinyoai_experts_free(tinyoai_experts *e);
 
+/* ---------------- attention for serving programs (no counterpart in the reference) ----------------
+ *
+ * For a program that walks a model's layers itself and serves many requests:
+ * rotary positions, a cache of pages that requests share, the attention of one
+ * new token of each over them, and that of packed prompts. Device buffers
+ * throughout; every call but the opens and closes enqueues on `stream` (a
+ * hipStream_t) without synchronizing and may be captured. NULL is the handle's
+ * own stream, or without a handle the current device's default stream. The
+ * current device must be the handle's. Types are TINYOAI_F32, TINYOAI_F16 and
+ * TINYOAI_BF16. A buffer's row holds its heads one after another and rows are
+ * `ld` values apart (at most 2^22); a buffer starts at a multiple of its type's
+ * size. Heads have a multiple of 8 values, at most 256. A call with no rows
+ * (n, nq = 0) does nothing. Handles may be used by several threads at once;
+ * what is still enqueued must have ended before a close. */
+
+#define TINYOAI_ROPE_HALF 0        /* value i of a head turns with i + rot / 2 */
+#define TINYOAI_ROPE_INTERLEAVED 1 /* value 2 i with 2 i + 1 */
+#define TINYOAI_ROPE_NONE 0
+#define TINYOAI_ROPE_LINEAR 1 /* all angles over `factor` */
+#define TINYOAI_ROPE_BANDS 2  /* pairs that turn `high` times or more in `context` positions keep their angle, those that
+                               * turn `low` times or fewer have it over `factor`, those between a mix, linear in the turns */
+#define TINYOAI_ROPE_YARN 3   /* the same with a mix linear in the pair's index, between the pairs (floor, ceiling) that turn
+                               * `high` and `low` times; sines and cosines times 0.1 ln(factor) + 1 */
+typedef struct {
+  int32_t head_dim, rot; /* values of a head, and how many of them turn (even): the first ones */
+  int32_t layout, scaling;
+  double theta;          /* pair i turns by position * theta^(-2 i / rot) radians, unscaled; theta > 1 */
+  double factor;         /* >= 1 (read where there is a scaling) */
+  int32_t context;       /* positions (bands, yarn) */
+  double low, high;      /* turns, 0 < low < high (bands, yarn) */
+} tinyoai_rope_config;
+typedef struct tinyoai_rope tinyoai_rope;
+int tinyoai_rope_open(const tinyoai_rope_config *config, tinyoai_rope **out);
+/* out[r][h] = x[r][h] turned by positions[r], for n rows of `heads` heads (of
+ * queries, keys or both where they lie together). Angles are formed in 64 bits,
+ * the rest in fp32, rounded once. out may be x itself (same type and distance);
+ * otherwise they must not overlap. */
+int tinyoai_rope_device(tinyoai_rope *r, int32_t dtype, const void *x_dev, int64_t ldx, int32_t n, int32_t heads,
+                        const int32_t *positions_dev, int32_t out_dtype, void *out_dev, int64_t ldo, void *stream);
+int tinyoai_rope_close(tinyoai_rope *r);
+
+/* A cache of `pages` pages of `page` positions (a power of two, at most 1024;
+ * page * pages at most 2^30) for each of `layers` layers, allocated at once and
+ * zeroed; slot s is position s % page of page s / page. Types F32, F16, BF16
+ * and Q8_0: blocks of 32 values of a head (the last one may be shorter) as whole
+ * numbers times a scale: d = the largest magnitude over 127, rounded to fp32 and
+ * then to fp16 (at most 65504), and the fp32 quotients x / d to the nearest
+ * whole number, halfway ones to the even one, within -127 .. 127. A block with an
+ * infinity or NaN becomes NaN. */
+typedef struct tinyoai_kv_pages tinyoai_kv_pages;
+int tinyoai_kv_pages_open(int32_t type, int32_t layers, int32_t kv_heads, int32_t head_dim, int32_t page, int32_t pages,
+                          tinyoai_kv_pages **out);
+/* n rows of keys and of values to their slots, rounded to the nearest in the
+ * cache's type. Rows whose slot is outside [0, page * pages) are left out; a
+ * slot named twice holds parts of either row. */
+int tinyoai_kv_pages_write_device(tinyoai_kv_pages *c, int32_t layer, int32_t dtype, const void *k_dev, int64_t ldk,
+                                  const void *v_dev, int64_t ldv, const int32_t *slots_dev, int32_t n, void *stream);
+/* The values that n slots stand for, rounded to the nearest (exact but for 8-bit
+ * and wider types read as narrower ones); zeros for slots outside the cache. */
+int tinyoai_kv_pages_read_device(tinyoai_kv_pages *c, int32_t layer, int32_t dtype, void *k_dev, int64_t ldk, void *v_dev,
+                                 int64_t ldv, const int32_t *slots_dev, int32_t n, void *stream);
+/* out[i][h] = sum over j < lengths[i] of softmax_j(scale * q[i][h] . k_j) v_j for
+ * one new token i of each of n sequences, query head h over key head h /
+ * (heads / kv_heads); position j of sequence i lies in page table[i][j / page].
+ * Lengths beyond width * page (at most 2^30) count as that; positions of entries
+ * outside [0, pages) are left out, entries past the length are not read, and
+ * a sequence without positions gets zeros. The new token's own key and value are
+ * written first (they count as any other). Scores, softmax and sums are fp32, of
+ * the values that the cache stands for; the result is rounded once. n * heads is
+ * at most 2^22. Long sequences are cut into ranges whose sums are joined in
+ * order, in scratch as tinyoai_weight_mul_device's. */
+int tinyoai_kv_pages_attend_device(tinyoai_kv_pages *c, int32_t layer, int32_t dtype, const void *q_dev, int64_t ldq,
+                                   int32_t heads, float scale, const int32_t *table_dev, int32_t width,
+                                   const int32_t *lengths_dev, int32_t n, void *out_dev, int64_t ldo, void *stream);
+int tinyoai_kv_pages_close(tinyoai_kv_pages *c);
+
+/* Attention of packed sequences: sequence s has the query rows q_offsets[s] ..
+ * q_offsets[s + 1] - 1 of nq and the key and value rows k_offsets[s] ..
+ * k_offsets[s + 1] - 1 of nk. Query i of a sequence's m sees, with causal
+ * nonzero, its keys j <= i + (keys - m) (the last query sees every key: a
+ * chunk of a prompt behind what is cached of it), else all of them; one that
+ * sees none gets zeros. Masked keys and values have no effect, whatever they
+ * hold. q, k, v and out have one type; sums are fp32, and for 16-bit types the
+ * softmax weights are rounded to that type. Rows outside the sequences stay as
+ * they are. Offsets that leave [0, nq] or [0, nk] count as the nearest that do
+ * not; they must not fall (rows of such sequences may be left out; nothing
+ * outside `out` is touched). nq and nk are at most 2^30, and (nq / 128 +
+ * sequences) * heads must stay below 2^24. */
+int tinyoai_attention_device(int32_t dtype, const void *q_dev, int64_t ldq, int32_t heads, const void *k_dev, int64_t ldk,
+                             const void *v_dev, int64_t ldv, int32_t kv_heads, int32_t head_dim, float scale, int32_t causal,
+                             const int32_t *q_offsets_dev, const int32_t *k_offsets_dev, int32_t sequences, int32_t nq,
+                             int32_t nk, void *out_dev, int64_t ldo, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -32,6 +32,9 @@ EXPORTS = [
     "tinyoai_mxfp4_quantize_device", "tinyoai_mxfp4_dequantize_device", "tinyoai_weight_mul_mxfp4_device",
     "tinyoai_route_device", "tinyoai_combine_device", "tinyoai_experts_upload", "tinyoai_experts_mul_device",
     "tinyoai_experts_free",
+    "tinyoai_rope_open", "tinyoai_rope_device", "tinyoai_rope_close", "tinyoai_kv_pages_open",
+    "tinyoai_kv_pages_write_device", "tinyoai_kv_pages_read_device", "tinyoai_kv_pages_attend_device",
+    "tinyoai_kv_pages_close", "tinyoai_attention_device",
 ]
 
 
@@ -55,6 +58,12 @@ class StableLMConfig(C.Structure):
 class LlamaConfig(C.Structure):
     _fields_ = [("dim", C.c_int32), ("hidden_dim", C.c_int32), ("n_layers", C.c_int32), ("n_heads", C.c_int32),
                 ("n_kv_heads", C.c_int32), ("vocab_size", C.c_int32), ("seq_len", C.c_int32)]
+
+
+class RopeConfig(C.Structure):
+    _fields_ = [("head_dim", C.c_int32), ("rot", C.c_int32), ("layout", C.c_int32), ("scaling", C.c_int32),
+                ("theta", C.c_double), ("factor", C.c_double), ("context", C.c_int32), ("low", C.c_double),
+                ("high", C.c_double)]
 
 
 _lib = None
@@ -113,6 +122,16 @@ def lib():
         L.tinyoai_experts_upload.argtypes = [i32, i32, i64, i64, P, P, C.c_uint64, C.POINTER(P)]
         L.tinyoai_experts_mul_device.argtypes = [P, i32, P, P, i64, i32, P, P, i32, i32, P, i64, P]
         L.tinyoai_experts_free.argtypes = [P]
+        f32 = C.c_float
+        L.tinyoai_rope_open.argtypes = [C.POINTER(RopeConfig), C.POINTER(P)]
+        L.tinyoai_rope_device.argtypes = [P, i32, P, i64, i32, i32, P, i32, P, i64, P]
+        L.tinyoai_rope_close.argtypes = [P]
+        L.tinyoai_kv_pages_open.argtypes = [i32, i32, i32, i32, i32, i32, C.POINTER(P)]
+        L.tinyoai_kv_pages_write_device.argtypes = [P, i32, i32, P, i64, P, i64, P, i32, P]
+        L.tinyoai_kv_pages_read_device.argtypes = [P, i32, i32, P, i64, P, i64, P, i32, P]
+        L.tinyoai_kv_pages_attend_device.argtypes = [P, i32, i32, P, i64, i32, f32, P, i32, P, i32, P, i64, P]
+        L.tinyoai_kv_pages_close.argtypes = [P]
+        L.tinyoai_attention_device.argtypes = [i32, P, i64, i32, P, i64, P, i64, i32, i32, f32, i32, P, P, i32, i32, i32, P, i64, P]
         _lib = L
     return _lib
 
@@ -221,6 +240,93 @@ class Experts:
             self.close()
         except Exception:
             pass
+
+
+# ---------------------------------------------------------------- attention for serving programs
+# Buffers, streams and types as above.
+class Rope:
+    """Rotary positions of heads of `head_dim` values whose first `rot` turn;
+    layout "half" or "interleaved". Scalings: "none", "linear" (factor),
+    "bands" and "yarn" (factor, context, low and high turns)."""
+
+    LAYOUTS = {"half": 0, "interleaved": 1}
+    SCALINGS = {"none": 0, "linear": 1, "bands": 2, "yarn": 3}
+
+    def __init__(self, head_dim: int, rot: int, layout: str = "half", theta: float = 10000.0, scaling: str = "none",
+                 factor: float = 1.0, context: int = 0, low: float = 0.0, high: float = 0.0):
+        self.h = None
+        c = RopeConfig(head_dim, rot, self.LAYOUTS[layout], self.SCALINGS[scaling], theta, factor, context, low, high)
+        h = C.c_void_p()
+        check(lib().tinyoai_rope_open(C.byref(c), C.byref(h)))
+        self.h = h
+
+    def rotate(self, dtype: int, x_ptr: int, ldx: int, n: int, heads: int, positions_ptr: int, out_dtype: int,
+               out_ptr: int, ldo: int, stream: int = 0) -> None:
+        """n rows of `heads` heads turned by their positions (int32); out may be x."""
+        check(lib().tinyoai_rope_device(self.h, dtype, x_ptr, ldx, n, heads, positions_ptr, out_dtype, out_ptr, ldo,
+                                        stream or None))
+
+    def close(self):
+        if self.h:
+            lib().tinyoai_rope_close(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class KVPages:
+    """Keys and values of `layers` layers in `pages` pages of `page`
+    positions, held as F32, F16, BF16 or Q8_0."""
+
+    def __init__(self, dtype: int, layers: int, kv_heads: int, head_dim: int, page: int, pages: int):
+        self.dtype, self.layers, self.kv_heads, self.head_dim = dtype, layers, kv_heads, head_dim
+        self.page, self.pages = page, pages
+        self.h = None
+        h = C.c_void_p()
+        check(lib().tinyoai_kv_pages_open(dtype, layers, kv_heads, head_dim, page, pages, C.byref(h)))
+        self.h = h
+
+    def write(self, layer: int, dtype: int, k_ptr: int, ldk: int, v_ptr: int, ldv: int, slots_ptr: int, n: int,
+              stream: int = 0) -> None:
+        """n rows of keys and of values to their slots (int32; others than the cache's: left out)."""
+        check(lib().tinyoai_kv_pages_write_device(self.h, layer, dtype, k_ptr, ldk, v_ptr, ldv, slots_ptr, n, stream or None))
+
+    def read(self, layer: int, dtype: int, k_ptr: int, ldk: int, v_ptr: int, ldv: int, slots_ptr: int, n: int,
+             stream: int = 0) -> None:
+        """The values that n slots stand for (zeros for slots outside the cache)."""
+        check(lib().tinyoai_kv_pages_read_device(self.h, layer, dtype, k_ptr, ldk, v_ptr, ldv, slots_ptr, n, stream or None))
+
+    def attend(self, layer: int, dtype: int, q_ptr: int, ldq: int, heads: int, scale: float, table_ptr: int, width: int,
+               lengths_ptr: int, n: int, out_ptr: int, ldo: int, stream: int = 0) -> None:
+        """The attention of one new token of each of n sequences over its
+        first lengths[i] positions, which lie in the pages table[i][:width]."""
+        check(lib().tinyoai_kv_pages_attend_device(self.h, layer, dtype, q_ptr, ldq, heads, scale, table_ptr, width,
+                                                   lengths_ptr, n, out_ptr, ldo, stream or None))
+
+    def close(self):
+        if self.h:
+            lib().tinyoai_kv_pages_close(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def attention(dtype: int, q_ptr: int, ldq: int, heads: int, k_ptr: int, ldk: int, v_ptr: int, ldv: int, kv_heads: int,
+              head_dim: int, scale: float, causal: bool, q_offsets_ptr: int, k_offsets_ptr: int, sequences: int, nq: int,
+              nk: int, out_ptr: int, ldo: int, stream: int = 0) -> None:
+    """The attention of packed sequences: queries q_offsets[s] .. q_offsets[s + 1] - 1 over keys k_offsets[s] ..
+    k_offsets[s + 1] - 1 (causal: aligned at the end)."""
+    check(lib().tinyoai_attention_device(dtype, q_ptr, ldq, heads, k_ptr, ldk, v_ptr, ldv, kv_heads, head_dim, scale,
+                                         int(causal), q_offsets_ptr, k_offsets_ptr, sequences, nq, nk, out_ptr, ldo,
+                                         stream or None))
 
 
 class Weight:
