@@ -29,9 +29,6 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
-constexpr int kT = 256;     // four waves
-constexpr int kQ = 128;     // queries of a block, 32 a wave
-constexpr int kKeys = 64;   // keys of a tile
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -65,6 +62,29 @@ __device__ __forceinline__ bool not_finite(uint4 w) {
   return bad;
 }
 
+template <int D>
+__device__ __forceinline__ uint4 only_finite(uint4 w) {  // zeros for the others
+  auto one = [](uint32_t u) {
+    if constexpr (D == FMT_F32) return (u & 0x7f800000u) == 0x7f800000u ? 0u : u;
+    constexpr uint32_t e = D == FMT_F16 ? 0x7c00u : 0x7f80u;
+    return ((u & e) == e ? 0u : u & 0xffffu) | ((u >> 16 & e) == e ? 0u : u & 0xffff0000u);
+  };
+  return make_uint4(one(w.x), one(w.y), one(w.z), one(w.w));
+}
+// c plus both halves of a pair.
+template <int D>
+__device__ __forceinline__ float plus2(uint32_t a, float c) {
+  if constexpr (D == FMT_F16)
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, a), f16x2{(_Float16)1.f, (_Float16)1.f}, c, false);
+  else
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, a), bf16x2{(__bf16)1.f, (__bf16)1.f}, c, false);
+}
+// The value of lane l ^ 32.
+__device__ __forceinline__ float other_half(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
+}
+
 // LDS rows of C chunks of 16 bytes; chunk c of row r at place c ^ swizzle, so
 // that the lanes of a read that go together hit distinct banks. K (by rows): 16
 // consecutive rows, one chunk. V (transposed): 4 consecutive rows, 4 chunks
@@ -83,12 +103,13 @@ __device__ __forceinline__ int v_place(int r, int c) {
   else return c;
 }
 
-// The sequence of query tile `tile` (tiles of kQ queries, a sequence's last
+// The sequence of query tile `tile` (tiles of QB queries, a sequence's last
 // ones first), its queries and keys.
 struct Where {
   int tile;            // within the sequence; -1: none
   int q0, nq, k0, nk;  // first rows and numbers
 };
+template <int QB>
 __device__ __forceinline__ Where find(const PromptArgs &a, int tile) {
   const int lane = threadIdx.x & 63;
   int before = 0;
@@ -99,7 +120,7 @@ __device__ __forceinline__ Where find(const PromptArgs &a, int tile) {
       first = min(max(a.q_offsets[s], 0), a.nq);
       n = max(min(a.q_offsets[s + 1], a.nq) - first, 0);
     }
-    const int tiles = (n + kQ - 1) / kQ;
+    const int tiles = (n + QB - 1) / QB;
     int upto = tiles;
 #pragma unroll
     for (int off = 1; off < 64; off *= 2) {
@@ -121,25 +142,47 @@ __device__ __forceinline__ Where find(const PromptArgs &a, int tile) {
   return Where{-1, 0, 0, 0, 0};
 }
 
-// KS: steps of 16 dims. T: the chunks (16 bytes) of a row.
-template <int D, int KS>
-__global__ __launch_bounds__(kT) void prompt_kernel(PromptArgs a) {
-  constexpr bool F32 = D == FMT_F32;
-  constexpr int HD = KS * 16;
-  constexpr int V = F32 ? 4 : 8;          // values of a chunk
-  constexpr int C = HD / V;               // chunks of a row
-  constexpr int DT = (HD + 31) / 32;      // 32-dim tiles of O^T
-  constexpr int KEYS = F32 && KS > 8 ? 32 : kKeys;
-  constexpr int HALVES = KEYS / 32;
-  constexpr int LOADS = (KEYS * C + kT - 1) / kT;
-  constexpr float kLeap = 8.f;            // the reference moves only when a score exceeds it by 2^8
+// The chunk that place `p` of a tile's plane holds: C chunks a row, a row's
+// chunks exchanged by k_place or v_place (both are their own inverse).
+template <int D, int C, bool VT>
+__device__ __forceinline__ int chunk_at(int row, int p) {
+  return !VT ? k_place<C>(row, p) : D == FMT_F32 ? p : v_place<C>(row, p);
+}
+
+// QG * KG waves: QG groups of 32 queries by KG groups of keys, which take the
+// sequence's tiles of KEYS keys in turn and whose sums are joined at the end.
+// KS: steps of 16 dims. DMA: K and V go straight into LDS (rows on 16-byte
+// boundaries), else through registers.
+template <int D, int KS, int QG, int KG, int KEYS, int STAGES, bool DMA>
+struct Prompt {
+  static constexpr bool F32 = D == FMT_F32;
+  static constexpr int HD = KS * 16;
+  static constexpr int T = 64 * QG * KG, QB = 32 * QG;
+  static constexpr int V = F32 ? 4 : 8;              // values of a chunk
+  static constexpr int C = HD / V;                   // chunks of a row
+  static constexpr int DT = (HD + 31) / 32;          // 32-dim tiles of O^T
+  static constexpr int PLANE = KEYS * C;             // chunks of a tile's K or V
+  static constexpr int QS = F32 ? 2 * KS : KS;       // operands of a query
+  static constexpr int SPAN = DT * 32 / V - C;       // chunks past a row that its last transposed read may touch
+  static constexpr int JOIN = KG > 1 ? QG * KG * (DT * 16 + 2) * 16 : 0;  // chunks that the groups' sums take
+  static constexpr int TILES = STAGES * KG * 2 * PLANE + SPAN;
+  static constexpr int LDS = TILES > JOIN ? TILES : JOIN;
+  static_assert(LDS * 16 <= 160 * 1024, "LDS of a CU");
   typedef std::conditional_t<F32, float, uint16_t> Value;
-  // (the transposed reads of a row's last tile may go past the row)
-  __shared__ __align__(16) uint4 ks[KEYS * C];
-  __shared__ __align__(16) uint4 vs[KEYS * C + DT * 32 / V - C];
+};
+
+template <int D, int KS, int QG, int KG, int KEYS, int STAGES, bool DMA>
+__global__ __launch_bounds__(64 * QG * KG) __attribute__((amdgpu_waves_per_eu(D != FMT_F32 && KS <= 8 ? 2 : 1)))
+void prompt_kernel(PromptArgs a) {
+  using P = Prompt<D, KS, QG, KG, KEYS, STAGES, DMA>;
+  using Value = typename P::Value;
+  constexpr bool F32 = P::F32;
+  constexpr int V = P::V, C = P::C, DT = P::DT, PLANE = P::PLANE, QS = P::QS, HALVES = KEYS / 32;
+  constexpr float kLeap = 8.f;            // the reference moves only when a score exceeds it by 2^8
+  __shared__ __align__(16) uint4 lds[P::LDS];
 
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, g = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), qg = wave % QG, kg = wave / QG;
   // Blocks go over the XCDs in turn: an XCD takes the same heads of every tile,
   // so the blocks it runs share their keys in its L2.
   int head, tile;
@@ -151,29 +194,32 @@ __global__ __launch_bounds__(kT) void prompt_kernel(PromptArgs a) {
     head = blockIdx.x % a.heads;
     tile = blockIdx.x / a.heads;
   }
-  const Where w = find(a, tile);
+  const Where w = find<P::QB>(a, tile);
   if (w.tile < 0) return;
   const int kvh = head / (a.heads / a.kv_heads);
-  const int qb = w.tile * kQ, qw = qb + wave * 32, mine = qw + col;  // within the sequence
+  const int qb = w.tile * P::QB, qw = qb + qg * 32, mine = qw + col;  // within the sequence
   const int shift = w.nk - w.nq;
-  // the last key that this lane's query, the wave's and the block's last ones see
+  // the last key that this lane's query, the wave's and the block's last ones
+  // see, and the first ones'
   const int last = a.causal ? min(mine, w.nq - 1) + shift : w.nk - 1;
   const int last_wave = a.causal ? min(qw + 31, w.nq - 1) + shift : w.nk - 1;
-  const int last_block = a.causal ? min(qb + kQ - 1, w.nq - 1) + shift : w.nk - 1;
-  const int first_wave = a.causal ? qw + shift : w.nk - 1;  // of the wave's first query
+  const int last_block = a.causal ? min(qb + P::QB - 1, w.nq - 1) + shift : w.nk - 1;
+  const int first_wave = a.causal ? qw + shift : w.nk - 1;
+  const int first_block = a.causal ? qb + shift : w.nk - 1;
 
-  // Q^T as B operands: query l % 32, dims 16 step + 8 g .. + 7 (fp32: of a
-  // chunk 8 step + 4 g .. + 3, one value a product).
-  uint4 q[F32 ? 2 * KS : KS];
+  // Q^T as B operands: query l % 32, dims 16 step + 8 g .. + 7 (fp32: a chunk 8
+  // step + 4 g .. + 3, one value a product). A negative scale turns their signs.
+  uint4 q[QS];
   {
     const Value *p = static_cast<const Value *>(a.q) + (w.q0 + min(mine, w.nq - 1)) * a.ldq + (int64_t)head * a.hd;
+    const uint32_t sign = a.scale < 0.f ? F32 ? 0x80000000u : 0x80008000u : 0u;
 #pragma unroll
-    for (int s = 0; s < (F32 ? 2 * KS : KS); s++) {
+    for (int s = 0; s < QS; s++) {
       const int d = (2 * s + g) * V;
       q[s] = make_uint4(0, 0, 0, 0);
       if (d < a.hd) {
         const u32x4_any x = *reinterpret_cast<const u32x4_any *>(p + d);
-        q[s] = make_uint4(x.x, x.y, x.z, x.w);
+        q[s] = make_uint4(x.x ^ sign, x.y ^ sign, x.z ^ sign, x.w ^ sign);
       }
     }
   }
@@ -182,111 +228,148 @@ __global__ __launch_bounds__(kT) void prompt_kernel(PromptArgs a) {
   for (int t = 0; t < DT; t++)
 #pragma unroll
     for (int v = 0; v < 16; v++) o[t][v] = 0.f;
-  float ref = -INFINITY, sum = 0.f;  // of this lane's query; sum: of the lane's own keys
-  const float scale = a.scale * kLog2e;
+  // Softmax weights are 2^(s scale - ref). sum: of the lane's own keys.
+  float ref = -INFINITY, sum = 0.f;
+  const float scale = fmaxf(fabsf(a.scale) * kLog2e, 1e-37f);  // (of zero: all weights alike)
 
+  // ---- staging. A group's QG waves load its tile, K by their first half and V by the other.
+  constexpr int PARTS = QG == 1 ? 1 : QG / 2;              // waves of a plane
+  constexpr int N = PLANE / 64 / PARTS, NS = QG == 1 ? 2 * N : N;  // loads of a wave
+  static_assert(PLANE % (64 * PARTS) == 0, "whole loads");
   const Value *kp = static_cast<const Value *>(a.k) + (int64_t)w.k0 * a.ldk + (int64_t)kvh * a.hd;
   const Value *vp = static_cast<const Value *>(a.v) + (int64_t)w.k0 * a.ldv + (int64_t)kvh * a.hd;
-  const int tiles = last_block / KEYS + 1;  // (last_block < 0: no key, tiles <= 0 or all masked)
-  uint4 kr[LOADS], vr[LOADS];
-  auto load = [&](int t0) {
+  const bool second = QG > 1 && qg >= PARTS;               // (uniform: this wave loads V)
+  const int part = QG == 1 ? 0 : qg % PARTS;
+  constexpr uint32_t kNone = 0x80000000u;
+  uint32_t voff[NS];                                       // bytes from the tile's first row
 #pragma unroll
-    for (int i = 0; i < LOADS; i++) {
-      const int e = tid + kT * i, r = t0 + e / C, d = e % C * V;
-      kr[i] = vr[i] = make_uint4(0, 0, 0, 0);
-      if (e < KEYS * C && r < w.nk && d < a.hd) {
-        const u32x4_any x = *reinterpret_cast<const u32x4_any *>(kp + r * a.ldk + d);
-        const u32x4_any y = *reinterpret_cast<const u32x4_any *>(vp + r * a.ldv + d);
-        kr[i] = make_uint4(x.x, x.y, x.z, x.w);
-        vr[i] = make_uint4(y.x, y.y, y.z, y.w);
-      }
-    }
-  };
-  if (last_block >= 0) load(0);
-  for (int tile_k = 0; last_block >= 0 && tile_k < tiles; tile_k++) {
-    const int t0 = tile_k * KEYS;
-    __syncthreads();
+  for (int j = 0; j < NS; j++) {
+    const bool vt = QG == 1 ? j >= N : second;
+    const int e = (part * N + j % N) * 64 + lane, r = e / C, c = vt ? chunk_at<D, C, true>(r, e % C) : chunk_at<D, C, false>(r, e % C);
+    const int64_t ld = vt ? a.ldv : a.ldk;
+    voff[j] = c * V < a.hd ? (uint32_t)((r * ld + c * V) * (int)sizeof(Value)) : kNone;
+  }
+  uint4 staged[DMA ? 1 : NS];
+  auto load = [&](int t0, int stage) {  // the tile from key t0 on
+    const int left = min(max(w.nk - t0, 0), KEYS);
+    auto plane = [&](const Value *base, int64_t ld, int j0, bool vt) {
+      const Value *at = base + (int64_t)t0 * ld;
+      const uint32_t bytes = left ? (uint32_t)(((left - 1) * ld + a.hd) * (int)sizeof(Value)) : 0u;
+      if constexpr (DMA) {
+        const __amdgpu_buffer_rsrc_t rsrc = plane_rsrc(reinterpret_cast<const uint8_t *>(at), bytes);
+        const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint4 *)(lds) +
+                            (((stage * KG + kg) * 2 + vt) * PLANE + part * N * 64) * 16;
 #pragma unroll
-    for (int i = 0; i < LOADS; i++) {
-      const int e = tid + kT * i, r = e / C, c = e % C;
-      if (KEYS * C % kT == 0 || e < KEYS * C) {
-        ks[r * C + k_place<C>(r, c)] = kr[i];
-        vs[r * C + (F32 ? c : v_place<C>(r, c))] = vr[i];
-      }
-    }
-    if (tile_k + 1 < tiles) load(t0 + KEYS);
-    __syncthreads();
-    if (qw >= w.nq || t0 > last_wave) continue;
-    const bool masked = t0 + KEYS - 1 > first_wave || t0 + KEYS > w.nk;
-
-    f32x16 s[HALVES];
+        for (int j = 0; j < N; j++) lds_dma16(rsrc, voff[j0 + j], __builtin_amdgcn_readfirstlane(to + j * 1024));
+      } else {
 #pragma unroll
-    for (int h = 0; h < HALVES; h++) {
-#pragma unroll
-      for (int v = 0; v < 16; v++) s[h][v] = 0.f;
-      const int r = h * 32 + col;
-#pragma unroll
-      for (int st = 0; st < (F32 ? 2 * KS : KS); st++) {
-        const uint4 x = ks[r * C + k_place<C>(r, 2 * st + g)];
-        if constexpr (F32) {
-          s[h] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(x.x), __uint_as_float(q[st].x), s[h], 0, 0, 0);
-          s[h] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(x.y), __uint_as_float(q[st].y), s[h], 0, 0, 0);
-          s[h] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(x.z), __uint_as_float(q[st].z), s[h], 0, 0, 0);
-          s[h] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(x.w), __uint_as_float(q[st].w), s[h], 0, 0, 0);
-        } else {
-          s[h] = mfma<D>(x, q[st], s[h]);
+        for (int j = 0; j < N; j++) {
+          staged[j0 + j] = make_uint4(0, 0, 0, 0);
+          if (voff[j0 + j] < bytes) {
+            const u32x4_any x = *reinterpret_cast<const u32x4_any *>(reinterpret_cast<const uint8_t *>(at) + voff[j0 + j]);
+            staged[j0 + j] = make_uint4(x.x, x.y, x.z, x.w);
+          }
         }
       }
+    };
+    if constexpr (QG == 1) {
+      plane(kp, a.ldk, 0, false);
+      plane(vp, a.ldv, N, true);
+    } else {
+      plane(second ? vp : kp, second ? a.ldv : a.ldk, 0, second);
     }
-    float top = -INFINITY;
+  };
+  auto store = [&](int stage) {  // (not DMA)
 #pragma unroll
-    for (int h = 0; h < HALVES; h++)
-#pragma unroll
-      for (int v = 0; v < 16; v++) {
-        s[h][v] *= scale;
-        if (masked && t0 + h * 32 + (v >> 2) * 8 + g * 4 + (v & 3) > last) s[h][v] = -INFINITY;
-        top = fmaxf(top, s[h][v]);
-      }
-    top = fmaxf(top, __shfl_xor(top, 32));
-    if (__any(top > ref + kLeap || (ref == -INFINITY && top > ref))) {
-      const float next = fmaxf(ref, top), fade = next == -INFINITY ? 1.f : exp2_hw(ref - next);
-      ref = next;
-      sum *= fade;
-#pragma unroll
-      for (int t = 0; t < DT; t++)
-#pragma unroll
-        for (int v = 0; v < 16; v++) o[t][v] *= fade;
+    for (int j = 0; j < NS; j++) {
+      const bool vt = QG == 1 ? j >= N : second;
+      lds[((stage * KG + kg) * 2 + vt) * PLANE + (part * N + j % N) * 64 + lane] = staged[j];
     }
-    const float base = ref == -INFINITY ? 0.f : ref;
-#pragma unroll
-    for (int h = 0; h < HALVES; h++)
-#pragma unroll
-      for (int v = 0; v < 16; v++) {
-        s[h][v] = exp2_hw(s[h][v] - base);
-        sum += s[h][v];
-      }
-    // A key that some query of the tile does not see: its weight there is 0,
+  };
+
+  const int rounds = last_block < 0 ? 0 : (last_block / KEYS + KG) / KG;
+  bool bad = false;
+  if (rounds) {
+    load(kg * KEYS, 0);
+    if constexpr (!DMA) store(0);
+  }
+  for (int round = 0; round < rounds; round++) {
+    const int t0 = (round * KG + kg) * KEYS, stage = STAGES == 2 ? round & 1 : 0;
+    if constexpr (DMA) wait_vmcnt<0>();
+    __syncthreads();
+    const bool more = round + 1 < rounds;
+    if (STAGES == 2 && more) load(t0 + KG * KEYS, stage ^ 1);
+    const uint4 *ks = lds + (stage * KG + kg) * 2 * PLANE;
+    uint4 *vs = lds + ((stage * KG + kg) * 2 + 1) * PLANE;
+    // A key that some query of the block does not see: its weight there is 0,
     // and 0 times an infinity or NaN would be one too. Such values are left out
-    // of the products and added to the queries that see them.
-    bool bad = false;
-    if (masked && a.causal) {
-      for (int e = lane; e < KEYS * C; e += 64) bad |= not_finite<D>(vs[e]);
-      bad = __any(bad);
+    // of the products here and added to the queries that see them at the end.
+    if (a.causal && ((round + 1) * KG) * KEYS - 1 > first_block) {
+      bool found = false;
+      for (int e = qg * 64 + lane; e < PLANE; e += 64 * QG) {
+        uint4 x = vs[e];
+        if (not_finite<D>(x)) vs[e] = only_finite<D>(x), found = true;
+      }
+      bad |= found;
+      __syncthreads();
     }
-    auto product = [&](auto clean) {
-      constexpr bool CLEAN = decltype(clean)::value;
+    if (qw < w.nq && t0 <= last_wave) {
+      f32x16 s[HALVES];
+#pragma unroll
+      for (int h = 0; h < HALVES; h++) {
+#pragma unroll
+        for (int v = 0; v < 16; v++) s[h][v] = 0.f;
+        const int r = h * 32 + col;
+#pragma unroll
+        for (int st = 0; st < QS; st++) {
+          const uint4 x = ks[r * C + k_place<C>(r, 2 * st + g)];
+          if constexpr (F32) {
+            s[h] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(x.x), __uint_as_float(q[st].x), s[h], 0, 0, 0);
+            s[h] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(x.y), __uint_as_float(q[st].y), s[h], 0, 0, 0);
+            s[h] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(x.z), __uint_as_float(q[st].z), s[h], 0, 0, 0);
+            s[h] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(x.w), __uint_as_float(q[st].w), s[h], 0, 0, 0);
+          } else {
+            s[h] = mfma<D>(x, q[st], s[h]);
+          }
+        }
+      }
+      if (t0 + KEYS - 1 > first_wave) {  // some of the wave's queries do not see the whole tile
+#pragma unroll
+        for (int h = 0; h < HALVES; h++)
+#pragma unroll
+          for (int v = 0; v < 16; v++)
+            if (t0 + h * 32 + (v >> 2) * 8 + g * 4 + (v & 3) > last) s[h][v] = -INFINITY;
+      }
+      float top = s[0][0];
+#pragma unroll
+      for (int h = 0; h < HALVES; h++)
+#pragma unroll
+        for (int v = 0; v < 16; v++) top = fmaxf(top, s[h][v]);
+      top = fmaxf(top, other_half(top)) * scale;
+      if (__any(top > ref + kLeap)) {  // (at first always: -inf + 8 is -inf)
+        const float next = fmaxf(ref, top), fade = next == -INFINITY ? 1.f : exp2_hw(ref - next);
+        ref = next;
+        sum *= fade;
+#pragma unroll
+        for (int t = 0; t < DT; t++)
+#pragma unroll
+          for (int v = 0; v < 16; v++) o[t][v] *= fade;
+      }
+      const float base = ref == -INFINITY ? 0.f : -ref;
+#pragma unroll
+      for (int h = 0; h < HALVES; h++)
+#pragma unroll
+        for (int v = 0; v < 16; v++) s[h][v] = exp2_hw(fmaf(s[h][v], scale, base));
 #pragma unroll
       for (int h = 0; h < HALVES; h++) {
         if constexpr (F32) {
 #pragma unroll
           for (int v = 0; v < 16; v++) {
+            sum += s[h][v];
             const int r = h * 32 + (v >> 2) * 8 + g * 4 + (v & 3);
 #pragma unroll
-            for (int t = 0; t < DT; t++) {
-              float x = reinterpret_cast<const float *>(vs + r * C)[t * 32 + col];
-              if (CLEAN && (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u) x = 0.f;
-              o[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, s[h][v], o[t], 0, 0, 0);
-            }
+            for (int t = 0; t < DT; t++)
+              o[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(reinterpret_cast<const float *>(vs + r * C)[t * 32 + col], s[h][v], o[t], 0, 0, 0);
           }
         } else {
 #pragma unroll
@@ -296,72 +379,126 @@ __global__ __launch_bounds__(kT) void prompt_kernel(PromptArgs a) {
             pw.y = pack2<D>(s[h][8 * st + 2], s[h][8 * st + 3]);
             pw.z = pack2<D>(s[h][8 * st + 4], s[h][8 * st + 5]);
             pw.w = pack2<D>(s[h][8 * st + 6], s[h][8 * st + 7]);
+            sum = plus2<D>(pw.x, plus2<D>(pw.y, plus2<D>(pw.z, plus2<D>(pw.w, sum))));
             const int r0 = h * 32 + st * 16 + g * 4 + (lane & 15) / 4;
 #pragma unroll
             for (int t = 0; t < DT; t++) {
               const int d = t * 32 + (lane >> 4 & 1) * 16 + (lane & 3) * 4;
               auto read = [&](int r) {
                 const uint4 *chunk = vs + (r * C + v_place<C>(r, d / 8));
-                return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(reinterpret_cast<const uint16_t *>(chunk) + d % 8));
+                return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (lds_s16x4 *)(reinterpret_cast<const uint16_t *>(chunk) + d % 8)));
               };
-              const uint2 lo = __builtin_bit_cast(uint2, read(r0)), hi = __builtin_bit_cast(uint2, read(r0 + 8));
-              uint4 x = make_uint4(lo.x, lo.y, hi.x, hi.y);
-              if constexpr (CLEAN) {
-                constexpr uint32_t e = D == FMT_F16 ? 0x7c00u : 0x7f80u;
-                auto finite = [](uint32_t u) {
-                  return ((u & e) == e ? 0u : u & 0xffffu) | ((u >> 16 & e) == e ? 0u : u & 0xffff0000u);
-                };
-                x = make_uint4(finite(x.x), finite(x.y), finite(x.z), finite(x.w));
-              }
-              o[t] = mfma<D>(x, pw, o[t]);
+              const uint2 lo = read(r0), hi = read(r0 + 8);
+              o[t] = mfma<D>(make_uint4(lo.x, lo.y, hi.x, hi.y), pw, o[t]);
             }
           }
         }
       }
-    };
-    if (!bad) {
-      product(std::false_type());
-    } else {
-      product(std::true_type());
-      for (int r = 0; r < KEYS && t0 + r <= last; r++)
-#pragma unroll
-        for (int t = 0; t < DT; t++)
-#pragma unroll
-          for (int v = 0; v < 16; v++) {
-            const int d = t * 32 + (v >> 2) * 8 + g * 4 + (v & 3);
-            if (d >= HD) continue;
-            const Value raw = reinterpret_cast<const Value *>(vs + (r * C + (F32 ? d / V : v_place<C>(r, d / V))))[d % V];
-            float x;
-            if constexpr (F32) x = raw;
-            else x = D == FMT_F16 ? hw_half(raw) : bf16_to_float(raw);
-            if ((__float_as_uint(x) & 0x7f800000u) == 0x7f800000u) o[t][v] += x;
-          }
+    }
+    if constexpr (STAGES == 1) {
+      if (more) {
+        if constexpr (!DMA) load(t0 + KG * KEYS, 0);
+        __syncthreads();
+        if constexpr (DMA) load(t0 + KG * KEYS, 0);
+      }
+    }
+    if constexpr (!DMA) {
+      if (more) store(STAGES == 2 ? stage ^ 1 : 0);
     }
   }
-  sum += __shfl_xor(sum, 32);
-  if (mine >= w.nq) return;
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  bad = __syncthreads_or(bad);
+  sum += other_half(sum);
   Value *out = static_cast<Value *>(a.out) + (w.q0 + mine) * a.ldo + (int64_t)head * a.hd;
-#pragma unroll
-  for (int t = 0; t < DT; t++)
+  auto finish = [&](int t, f32x16 x, float inv) {
+    if (mine >= w.nq) return;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
       const int d = t * 32 + j * 8 + g * 4;
       if (d >= a.hd) continue;
-      const float x = o[t][4 * j] * inv, y = o[t][4 * j + 1] * inv, z = o[t][4 * j + 2] * inv, u = o[t][4 * j + 3] * inv;
-      if constexpr (F32) *reinterpret_cast<f32x4_any *>(out + d) = f32x4_any{x, y, z, u};
-      else *reinterpret_cast<u32x2_any *>(out + d) = u32x2_any{pack2<D>(x, y), pack2<D>(z, u)};
+      float y[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) y[i] = x[4 * j + i] * inv;
+      if (bad)
+        for (int r = max(first_block / (KG * KEYS), 0) * (KG * KEYS); r <= last; r++)
+          for (int i = 0; i < 4; i++) {
+            const float u = mx_load(D, vp, r * a.ldv + d + i);
+            if ((__float_as_uint(u) & 0x7f800000u) == 0x7f800000u) y[i] += u;
+          }
+      if constexpr (F32) *reinterpret_cast<f32x4_any *>(out + d) = f32x4_any{y[0], y[1], y[2], y[3]};
+      else *reinterpret_cast<u32x2_any *>(out + d) = u32x2_any{pack2<D>(y[0], y[1]), pack2<D>(y[2], y[3])};
     }
+  };
+  if constexpr (KG == 1) {
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int t = 0; t < DT; t++) finish(t, o[t], inv);
+  } else {
+    // [wave][reference, sum, values][lane]; a group of keys joins every KG-th tile of its queries'
+    float *f = reinterpret_cast<float *>(lds) + lane;
+    constexpr int W = (DT * 16 + 2) * 64;
+    f[wave * W] = ref;
+    f[wave * W + 64] = sum;
+#pragma unroll
+    for (int t = 0; t < DT; t++)
+#pragma unroll
+      for (int v = 0; v < 16; v++) f[wave * W + (2 + t * 16 + v) * 64] = o[t][v];
+    __syncthreads();
+    float top = -INFINITY, fade[KG], all = 0.f;
+#pragma unroll
+    for (int i = 0; i < KG; i++) top = fmaxf(top, f[(i * QG + qg) * W]);
+#pragma unroll
+    for (int i = 0; i < KG; i++) {
+      fade[i] = top == -INFINITY ? 0.f : exp2_hw(f[(i * QG + qg) * W] - top);
+      all += fade[i] * f[(i * QG + qg) * W + 64];
+    }
+    const float inv = all == 0.f ? 0.f : 1.f / all;
+    for (int t = kg; t < DT; t += KG) {
+      f32x16 x;
+#pragma unroll
+      for (int v = 0; v < 16; v++) {
+        x[v] = 0.f;
+#pragma unroll
+        for (int i = 0; i < KG; i++) x[v] += fade[i] * f[(i * QG + qg) * W + (2 + t * 16 + v) * 64];
+      }
+      finish(t, x, inv);
+    }
+  }
 }
 
 }  // namespace
 
-hipError_t launch_prompt(const PromptArgs &a, hipStream_t st) {
+namespace {
+
+template <int D, int KS, int QG, int KG, int KEYS, int STAGES>
+void launch(const PromptArgs &a, bool dma, hipStream_t st) {
+  constexpr int QB = 32 * QG;
   // at most: every sequence's last tile may be a part
-  const int64_t tiles = a.nq / kQ + std::min<int64_t>(a.sequences, a.nq);
-  const dim3 grid((unsigned)(tiles * a.heads));
+  const int64_t tiles = a.nq / QB + std::min<int64_t>(a.sequences, a.nq);
+  const dim3 grid((unsigned)(tiles * a.heads)), block(64 * QG * KG);
+  if (dma) hipLaunchKernelGGL((prompt_kernel<D, KS, QG, KG, KEYS, STAGES, true>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((prompt_kernel<D, KS, QG, KG, KEYS, STAGES, false>), grid, block, 0, st, a);
+}
+
+bool aligned16(const void *p, int64_t ld, int width) { return (reinterpret_cast<uintptr_t>(p) | (uintptr_t)(ld * width)) % 16 == 0; }
+
+}  // namespace
+
+hipError_t launch_prompt(const PromptArgs &a, hipStream_t st) {
+  const int width = (int)mx_width(a.dtype);
+  const bool dma = aligned16(a.k, a.ldk, width) && aligned16(a.v, a.ldv, width);
+  const int64_t blocks = (a.nq / 128 + std::min<int64_t>(a.sequences, a.nq)) * a.heads;
   auto go = [&](auto d, auto k) {
-    hipLaunchKernelGGL((prompt_kernel<decltype(d)::value, decltype(k)::value>), grid, dim3(kT), 0, st, a);
+    constexpr int D = decltype(d)::value, KS = decltype(k)::value;
+    if constexpr (D == FMT_F32) {
+      constexpr bool wide = KS > 8;
+      if (blocks < 256) launch<D, KS, 1, wide ? 2 : 4, 32, KS <= 4 ? 2 : 1>(a, dma, st);
+      else launch<D, KS, 4, 1, 32, wide ? 1 : 2>(a, dma, st);
+    } else {
+      if (blocks < 256 && a.nq <= 32) launch<D, KS, 1, 4, 32, KS <= 8 ? 2 : 1>(a, dma, st);
+      else if (blocks < 256 && KS <= 8) launch<D, KS, KS <= 8 ? 2 : 4, KS <= 8 ? 4 : 1, 32, 2>(a, dma, st);
+      else launch<D, KS, 4, 1, KS <= 8 ? 64 : 32, 2>(a, dma, st);
+    }
   };
   for_type(a.dtype, [&](auto d) {
     if (a.hd <= 32) go(d, std::integral_constant<int, 2>());
