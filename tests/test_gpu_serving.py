@@ -316,6 +316,8 @@ def test_attend_long(hip, dev, cache):
     _attend_check(hip, dev, rng, cache, dtype, 2, 2, 128, 256, (9000, 1), drop=0.2)
     _attend_check(hip, dev, rng, cache, W.BF16, 3, 1, 80, 8, (4097, 20, 300), pad=1, shift=2, drop=0.5)
     _attend_check(hip, dev, rng, cache, dtype, 16, 2, 128, 64, tuple(rng.integers(0, 900, 40)))
+    _attend_check(hip, dev, rng, cache, dtype, 2, 1, 8, 4, tuple(rng.integers(0, 3, 200)) + (600, 0, 129) + (1,) * 70)
+    _attend_check(hip, dev, rng, cache, dtype, 3, 3, 64, 32, tuple(rng.integers(0, 300, 130)))
 
 
 @pytest.mark.parametrize("cache", CACHES)

@@ -8,7 +8,7 @@
 // block attends to, a head's positions of a page, is then one contiguous run.
 // 8-bit pages (Q8_0) hold a byte a value and, in planes of their own with the
 // same order, the fp16 scales of a row's blocks of 32 values (the last block
-// may be shorter), `nb` of them, a power of two.
+// may be shorter), `nb` of them, a power of two from 2 on.
 #pragma once
 
 #include "mx.h"
@@ -27,6 +27,7 @@ struct KVPagesDev {
   int32_t pitch, nb;            // bytes of a row, its scales (0: none)
   uint8_t *k, *v;               // of the call's layer
   uint16_t *kd, *vd;            // scales
+  const uint8_t *zeros;         // 256 bytes: what positions that do not count read
 };
 
 // The row of (slot, head): of a plane in rows, so `pitch` bytes or `nb` scales each.
@@ -134,4 +135,40 @@ inline void for_type(int dtype, const F &call) {
   if (dtype == FMT_F32) call(std::integral_constant<int, FMT_F32>());
   else if (dtype == FMT_F16) call(std::integral_constant<int, FMT_F16>());
   else call(std::integral_constant<int, FMT_BF16>());
+}
+
+// LDS rows of C chunks of 16 bytes; chunk c of row r at place c ^ swizzle, so
+// that the lanes of a read that go together hit distinct banks. K (by rows): 16
+// consecutive rows, one chunk. V (transposed): 4 consecutive rows, 4 chunks
+// (fp32: one row, consecutive dims: none needed).
+template <int C>
+__device__ __forceinline__ int k_place(int r, int c) {
+  if constexpr (C % 16 == 0) return c ^ (r & 15);
+  else if constexpr (C == 8) return c ^ ((r >> 1) & 7);
+  else if constexpr (C % 4 == 0) return c ^ ((r >> 2) & 3);
+  else return c ^ ((r >> 3) & 1);
+}
+template <int C>
+__device__ __forceinline__ int v_place(int r, int c) {
+  if constexpr (C % 16 == 0) return c ^ ((r & 3) << 2 | ((r >> 2) & 3));
+  else if constexpr (C == 8) return c ^ (((r >> 1) & 1) << 2 | ((r >> 2) & 3));
+  else return c;
+}
+
+// Over lanes l and l ^ 32, and (quarters) l, l ^ 16, l ^ 32 and l ^ 48.
+__device__ __forceinline__ float halves_max(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float halves_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float quarters_max(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return halves_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+__device__ __forceinline__ float quarters_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return halves_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
 }

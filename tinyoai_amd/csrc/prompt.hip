@@ -79,30 +79,6 @@ __device__ __forceinline__ float plus2(uint32_t a, float c) {
   else
     return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, a), bf16x2{(__bf16)1.f, (__bf16)1.f}, c, false);
 }
-// The value of lane l ^ 32.
-__device__ __forceinline__ float other_half(float x) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
-}
-
-// LDS rows of C chunks of 16 bytes; chunk c of row r at place c ^ swizzle, so
-// that the lanes of a read that go together hit distinct banks. K (by rows): 16
-// consecutive rows, one chunk. V (transposed): 4 consecutive rows, 4 chunks
-// (fp32: one row, consecutive dims: none needed).
-template <int C>
-__device__ __forceinline__ int k_place(int r, int c) {
-  if constexpr (C % 16 == 0) return c ^ (r & 15);
-  else if constexpr (C == 8) return c ^ ((r >> 1) & 7);
-  else if constexpr (C % 4 == 0) return c ^ ((r >> 2) & 3);
-  else return c ^ ((r >> 3) & 1);
-}
-template <int C>
-__device__ __forceinline__ int v_place(int r, int c) {
-  if constexpr (C % 16 == 0) return c ^ ((r & 3) << 2 | ((r >> 2) & 3));
-  else if constexpr (C == 8) return c ^ (((r >> 1) & 1) << 2 | ((r >> 2) & 3));
-  else return c;
-}
-
 // The sequence of query tile `tile` (tiles of QB queries, a sequence's last
 // ones first), its queries and keys.
 struct Where {
@@ -345,7 +321,7 @@ void prompt_kernel(PromptArgs a) {
       for (int h = 0; h < HALVES; h++)
 #pragma unroll
         for (int v = 0; v < 16; v++) top = fmaxf(top, s[h][v]);
-      top = fmaxf(top, other_half(top)) * scale;
+      top = halves_max(top) * scale;
       if (__any(top > ref + kLeap)) {  // (at first always: -inf + 8 is -inf)
         const float next = fmaxf(ref, top), fade = next == -INFINITY ? 1.f : exp2_hw(ref - next);
         ref = next;
@@ -408,7 +384,7 @@ void prompt_kernel(PromptArgs a) {
     }
   }
   bad = __syncthreads_or(bad);
-  sum += other_half(sum);
+  sum = halves_sum(sum);
   Value *out = static_cast<Value *>(a.out) + (w.q0 + mine) * a.ldo + (int64_t)head * a.hd;
   auto finish = [&](int t, f32x16 x, float inv) {
     if (mine >= w.nq) return;

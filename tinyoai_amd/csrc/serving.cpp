@@ -197,14 +197,14 @@ int tinyoai_kv_pages_open(int32_t type, int32_t layers, int32_t kv_heads, int32_
   while (1 << c->d.page_log2 < page) c->d.page_log2++;
   c->d.pitch = type == FMT_Q8_0 ? (head_dim + 15) / 16 * 16 : head_dim * (int)mx_width(type);
   if (type == FMT_Q8_0)
-    for (c->d.nb = 1; c->d.nb * 32 < head_dim; c->d.nb *= 2) {}
+    for (c->d.nb = 2; c->d.nb * 32 < head_dim; c->d.nb *= 2) {}
   const int64_t rows = (int64_t)pages * page * kv_heads;  // at most 2^54
   c->plane = rows * c->d.pitch;
   c->scales = (rows * c->d.nb * 2 + 255) / 256 * 256;
   c->plane = (c->plane + 255) / 256 * 256;
   const double bytes = 2.0 * layers * ((double)c->plane + (double)c->scales);
   if (bytes > 1e15) return fail(TINYOAI_ENOMEM, "paged cache of %.3g bytes", bytes);
-  const size_t total = (size_t)layers * 2 * (size_t)(c->plane + c->scales);
+  const size_t total = (size_t)layers * 2 * (size_t)(c->plane + c->scales) + 256;  // (zeros last)
   hipError_t e = hipGetDevice(&c->device);
   if (e != hipSuccess) return hip_fail(e, "hipGetDevice");
   e = hipStreamCreateWithFlags(&c->stream, hipStreamNonBlocking);
@@ -212,6 +212,7 @@ int tinyoai_kv_pages_open(int32_t type, int32_t layers, int32_t kv_heads, int32_
   e = device_alloc(&c->mem, total);
   if (e != hipSuccess) return fail(TINYOAI_ENOMEM, "hipMalloc(%zu): %s", total, hipGetErrorString(e));
   c->d.k = static_cast<uint8_t *>(c->mem);
+  c->d.zeros = c->d.k + (total - 256);
   e = hipMemsetAsync(c->mem, 0, total, c->stream);  // what no call has written reads as zeros
   if (e == hipSuccess) e = hipStreamSynchronize(c->stream);
   if (e != hipSuccess) return hip_fail(e, "paged cache");
