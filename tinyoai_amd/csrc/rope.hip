@@ -7,8 +7,11 @@
 //
 // What bounds it: HBM, each value read and written once. A block takes a few
 // rows, so that their angles' sines and cosines, one a thread, serve all of the
-// rows' heads; a thread then takes eight pairs of a head at a time (both
-// halves, so a row may be turned in place).
+// rows' heads. A thread keeps its place within the head (a unit: sixteen values
+// of eight pairs in the half layout, eight values in a row in the interleaved
+// one, or eight values to copy) and goes through rows and heads, four at a
+// time, whose loads all start before the first is used (at first before the
+// angles are formed). 8192 rows of 40 bf16 heads of 128: FIGURE.
 #include <type_traits>
 
 #include "attend.h"
@@ -21,75 +24,104 @@ struct Turn {
   float c, s;
 };
 
-template <int D, int O>
+template <int D, int O, bool INTER>
 __global__ __launch_bounds__(kT) void rope_kernel(RopeArgs a, int rows, int heads) {
-  __shared__ Turn turn[kT];  // [rows][rot / 2]
+  constexpr int B = 2;                // units of a thread in flight
+  constexpr int P = INTER ? 4 : 8;    // pairs of a unit
+  constexpr int L = INTER ? 1 : 2;    // loads of a unit
+  __shared__ Turn turn[kT];           // [rows][rot / 2]
   const int half = a.rot / 2, r0 = blockIdx.x * rows, h0 = blockIdx.y * heads;
   const int nr = min(rows, a.n - r0), nh = min(heads, a.heads - h0);
+  const int pairs = (half + P - 1) / P, units = pairs + (a.hd - a.rot + 7) / 8;
+  const int side = kT / units;        // heads that the block takes side by side
+  const int unit = threadIdx.x % units, lane_head = threadIdx.x / units;
+  const bool turns = unit < pairs;
+  const int first = turns ? unit * P : 0;                            // the unit's first pair
+  const int at0 = turns ? INTER ? 2 * first : first : a.rot + (unit - pairs) * 8, at1 = at0 + half;
+  // its values at each place, less than eight at the end of a head's part
+  const int count = turns ? min(INTER ? 2 * (half - first) : half - first, 8) : min(a.hd - at0, 8);
+  const bool whole = count == 8;
+  float v[B][L][8];
+  // Of the next B (row, heads side by side): where they are, from row `nr` on none.
+  int row[B], head[B], next_row = 0, next_head = 0;
+  auto load = [&]() {
+#pragma unroll
+    for (int j = 0; j < B; j++) {
+      row[j] = next_row, head[j] = next_head + lane_head;
+      next_head += side;
+      if (next_head >= nh) next_head = 0, next_row++;
+      if (lane_head >= side || head[j] >= nh) head[j] = -1;
+      if (row[j] >= nr || head[j] < 0) continue;
+      const int64_t from = (r0 + row[j]) * a.ldx + (int64_t)(h0 + head[j]) * a.hd;
+      if (whole) {
+        load8<D>(a.x, from + at0, v[j][0]);
+        if (L == 2 && turns) load8<D>(a.x, from + at1, v[j][L - 1]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          v[j][0][e] = e < count ? mx_load(D, a.x, from + at0 + e) : 0.f;
+          if (L == 2) v[j][L - 1][e] = e < count && turns ? mx_load(D, a.x, from + at1 + e) : 0.f;
+        }
+      }
+    }
+  };
+  load();
   for (int i = threadIdx.x; i < nr * half; i += kT) {
     const double angle = (double)a.positions[r0 + i / half] * a.frequencies[i % half];
-    const double turns = rint(angle * 0.15915494309189535);
-    const float t = (float)fma(-turns, 2.4492935982947064e-16, fma(-turns, 6.283185307179586, angle));
+    const double whole_turns = rint(angle * 0.15915494309189535);
+    const float t = (float)fma(-whole_turns, 2.4492935982947064e-16, fma(-whole_turns, 6.283185307179586, angle));
     float s, c;
     sincosf(t, &s, &c);
     turn[i] = Turn{c * a.magnitude, s * a.magnitude};
   }
   __syncthreads();
-  const int pairs = (half + 7) / 8, rest = (a.hd - a.rot + 7) / 8, units = pairs + rest;
-  const int items = nr * nh * units;
-  for (int i = threadIdx.x; i < items; i += kT) {
-    const int u = i % units, rh = i / units, row = rh / nh, head = h0 + rh % nh;
-    const int64_t from = (int64_t)(r0 + row) * a.ldx + (int64_t)head * a.hd, to = (int64_t)(r0 + row) * a.ldo + (int64_t)head * a.hd;
-    if (u >= pairs) {
-      const int c = a.rot + (u - pairs) * 8;
-      if (c + 8 <= a.hd) {
-        float v[8];
-        load8<D>(a.x, from + c, v);
-        store8<O>(a.out, to + c, v);
-      } else {
-        for (int j = c; j < a.hd; j++) mx_store(O, a.out, to + j, mx_load(D, a.x, from + j));
-      }
-      continue;
-    }
-    const int p = u * 8;
-    const Turn *t = turn + row * half + p;
-    if (p + 8 <= half) {
-      const int at0 = a.interleaved ? 2 * p : p, at1 = a.interleaved ? 2 * p + 8 : p + half;
-      float v[2][8];
-      load8<D>(a.x, from + at0, v[0]);
-      load8<D>(a.x, from + at1, v[1]);
+  for (;;) {
 #pragma unroll
-      for (int j = 0; j < 8; j++) {
-        float &x1 = a.interleaved ? v[j / 4][2 * (j % 4)] : v[0][j], &x2 = a.interleaved ? v[j / 4][2 * (j % 4) + 1] : v[1][j];
-        const float y1 = x1 * t[j].c - x2 * t[j].s, y2 = x2 * t[j].c + x1 * t[j].s;
-        x1 = y1, x2 = y2;
+    for (int j = 0; j < B; j++) {
+      if (row[j] >= nr || head[j] < 0) continue;
+      const int64_t to = (r0 + row[j]) * a.ldo + (int64_t)(h0 + head[j]) * a.hd;
+      const Turn *t = turn + row[j] * half + first;
+      if (turns) {
+#pragma unroll
+        for (int p = 0; p < P; p++) {
+          float &x1 = INTER ? v[j][0][2 * p % 8] : v[j][0][p], &x2 = INTER ? v[j][0][(2 * p + 1) % 8] : v[j][L - 1][p];
+          const Turn w = t[min(p, half - 1 - first)];  // (past the last pair: of no value)
+          const float y1 = x1 * w.c - x2 * w.s, y2 = x2 * w.c + x1 * w.s;
+          x1 = y1, x2 = y2;
+        }
       }
-      store8<O>(a.out, to + at0, v[0]);
-      store8<O>(a.out, to + at1, v[1]);
-    } else {
-      for (int j = 0; p + j < half; j++) {
-        const int i1 = a.interleaved ? 2 * (p + j) : p + j, i2 = a.interleaved ? i1 + 1 : i1 + half;
-        const float x1 = mx_load(D, a.x, from + i1), x2 = mx_load(D, a.x, from + i2);
-        mx_store(O, a.out, to + i1, x1 * t[j].c - x2 * t[j].s);
-        mx_store(O, a.out, to + i2, x2 * t[j].c + x1 * t[j].s);
+      if (whole) {
+        store8<O>(a.out, to + at0, v[j][0]);
+        if (L == 2 && turns) store8<O>(a.out, to + at1, v[j][L - 1]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+          if (e < count) {
+            mx_store(O, a.out, to + at0 + e, v[j][0][e]);
+            if (L == 2 && turns) mx_store(O, a.out, to + at1 + e, v[j][L - 1][e]);
+          }
       }
     }
+    if (next_row >= nr) break;
+    load();
   }
 }
 
 }  // namespace
 
 hipError_t launch_rope(const RopeArgs &a, hipStream_t st) {
-  const int rows = a.rot / 2 >= kT / 2 ? 1 : kT / (a.rot / 2);
+  // rows a block, while there are blocks for the chip; the heads of few rows over several blocks
+  const int rows = std::max(1, std::min({kT / (a.rot / 2), 8, a.n / 1024}));
   const int64_t blocks = (a.n + rows - 1) / rows;
-  // a few rows' heads over several blocks, as many as fill the chip
-  int parts = (int)(512 / blocks);
+  int parts = (int)(1024 / blocks);
   parts = parts < 1 ? 1 : parts > a.heads ? a.heads : parts;
   const int heads = (a.heads + parts - 1) / parts;
   const dim3 grid((unsigned)blocks, (unsigned)((a.heads + heads - 1) / heads));
   for_type(a.dtype, [&](auto d) {
     for_type(a.out_dtype, [&](auto o) {
-      hipLaunchKernelGGL((rope_kernel<decltype(d)::value, decltype(o)::value>), grid, dim3(kT), 0, st, a, rows, heads);
+      constexpr int D = decltype(d)::value, O = decltype(o)::value;
+      if (a.interleaved) hipLaunchKernelGGL((rope_kernel<D, O, true>), grid, dim3(kT), 0, st, a, rows, heads);
+      else hipLaunchKernelGGL((rope_kernel<D, O, false>), grid, dim3(kT), 0, st, a, rows, heads);
     });
   });
   return hipGetLastError();
