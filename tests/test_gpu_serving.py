@@ -432,6 +432,18 @@ def test_prompt_strides(hip, dev, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+def test_prompt_parts(hip, dev, dtype):
+    """Few queries over many keys: tiles whose keys are cut into parts, some of them past a short sequence's end."""
+    rng = np.random.default_rng(16)
+    for heads, kv, hd, lengths in ((4, 2, 64, ((130, 4500),)), (3, 1, 80, ((40, 2100), (200, 4300))), (2, 1, 128, ((1, 7000),)),
+                                   (8, 1, 128, ((33, 90), (128, 9000))), (2, 2, 256, ((70, 3000),)), (1, 1, 8, ((300, 6000), (9, 4)))):
+        for causal in (True, False):
+            _prompt_check(hip, dev, rng, dtype, heads, kv, hd, lengths, causal)
+    _prompt_check(hip, dev, rng, dtype, 2, 1, 64, ((150, 4500), (130, 90)), True, hidden=True)
+    _prompt_check(hip, dev, rng, dtype, 2, 1, 80, ((20, 400), (5, 5)), True, hidden=True)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_prompt_hidden_values(hip, dev, dtype):
     """Infinities and NaN in keys and values: queries that do not see them are not touched by them."""
     rng = np.random.default_rng(11)
@@ -507,6 +519,56 @@ def test_captured_and_concurrent_attention(hip, dev):
         for st in streams:
             rt.hipStreamDestroy(st)
         c.close()
+
+
+@pytest.mark.parametrize("dtype,n,keys", [(W.F32, 19, 449), (W.BF16, 130, 6000)])
+def test_captured_and_concurrent_prompts(hip, dev, dtype, n, keys):
+    """Prompts whose keys are cut into parts: two graphs captured on two streams and eager calls on a third, all in flight
+    together, with eager work between the replays."""
+    rng = np.random.default_rng(17)
+    heads, hd, rt = 4, 64, dev.rt
+    qo, ko = dev.put(np.array([0, n], np.int32)), dev.put(np.array([0, keys], np.int32))
+    xs = [[_rows(rng, dev, dtype, m, heads * hd)[0] for m in (n, keys, keys)] for _ in range(3)]
+    bits = bits_dtype(dtype)
+    y = [dev.put(np.zeros((n, heads * hd), bits)) for _ in range(4)]
+    streams, execs = [C.c_void_p() for _ in range(3)], []
+
+    def call(i, out, stream=0):
+        q, k, v = xs[i]
+        hip.attention(dtype, q, heads * hd, heads, k, heads * hd, v, heads * hd, heads, hd, 0.125, True, qo, ko, 1, n, keys, out,
+                      heads * hd, stream)
+
+    try:
+        for st in streams:
+            assert rt.hipStreamCreateWithFlags(C.byref(st), 1) == 0
+        for i in range(2):
+            graph, ex = C.c_void_p(), C.c_void_p()
+            assert rt.hipStreamBeginCapture(streams[i], 0) == 0
+            call(i, y[i], streams[i].value)
+            call(i, y[i], streams[i].value)
+            assert rt.hipStreamEndCapture(streams[i], C.byref(graph)) == 0
+            assert rt.hipGraphInstantiate(C.byref(ex), graph, None, None, C.c_size_t(0)) == 0
+            rt.hipGraphDestroy(graph)
+            execs.append(ex)
+        want = []
+        for i in range(3):
+            call(i, y[3])
+            want.append(dev.get(y[3], (n, heads * hd), bits).copy())
+        assert all(x.any() for x in want)
+        for _ in range(3):
+            for i in range(3):
+                dev.fill(y[i], np.zeros((n, heads * hd), bits))
+            for _ in range(4):
+                for i in range(2):
+                    assert rt.hipGraphLaunch(execs[i], streams[i]) == 0
+                call(2, y[2], streams[2].value)
+            for i in range(3):
+                assert np.array_equal(dev.get(y[i], (n, heads * hd), bits), want[i]), i
+    finally:
+        for ex in execs:
+            rt.hipGraphExecDestroy(ex)
+        for st in streams:
+            rt.hipStreamDestroy(st)
 
 
 @pytest.mark.parametrize("cache,dtype", [(W.F16, W.F32), (W.Q8_0, W.F32), (W.BF16, W.BF16), (W.F32, W.F32)])

@@ -82,7 +82,9 @@ struct PromptArgs {
   void *out;
   int64_t ldo;
 };
-hipError_t launch_prompt(const PromptArgs &a, hipStream_t st);
+// Bytes of scratch (0: none) that launch_prompt takes.
+size_t prompt_scratch(const PromptArgs &a);
+hipError_t launch_prompt(const PromptArgs &a, void *scratch, hipStream_t st);
 
 // Rows of heads turned by their positions.
 struct RopeArgs {
@@ -148,6 +150,11 @@ __device__ __forceinline__ int k_place(int r, int c) {
   else if constexpr (C % 4 == 0) return c ^ ((r >> 2) & 3);
   else return c ^ ((r >> 3) & 1);
 }
+// (rows of ten chunks: four rows in a row are kept two apart instead, v_row)
+template <int C>
+__device__ __forceinline__ int v_row(int r) { return C == 10 ? (r & ~7) | (r & 3) << 1 | ((r >> 2) & 1) : r; }
+template <int C>
+__device__ __forceinline__ int v_key(int r) { return C == 10 ? (r & ~7) | ((r >> 1) & 3) | (r & 1) << 2 : r; }  // its inverse
 template <int C>
 __device__ __forceinline__ int v_place(int r, int c) {
   if constexpr (C % 16 == 0) return c ^ ((r & 3) << 2 | ((r >> 2) & 3));
@@ -155,6 +162,11 @@ __device__ __forceinline__ int v_place(int r, int c) {
   else return c;
 }
 
+// The value of lane l % 32.
+__device__ __forceinline__ float lower_half(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]);
+}
 // Over lanes l and l ^ 32, and (quarters) l, l ^ 16, l ^ 32 and l ^ 48.
 __device__ __forceinline__ float halves_max(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);

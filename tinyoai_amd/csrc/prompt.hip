@@ -118,6 +118,19 @@ __device__ __forceinline__ Where find(const PromptArgs &a, int tile) {
   return Where{-1, 0, 0, 0, 0};
 }
 
+// Blocks go over the XCDs in turn: an XCD takes the same heads of every tile, so
+// the blocks it runs share their keys in its L2.
+__device__ __forceinline__ void tile_of(const PromptArgs &a, int block, int &head, int &tile) {
+  if (a.heads % 8 == 0) {
+    const int j = block / 8;
+    head = block % 8 * (a.heads / 8) + j % (a.heads / 8);
+    tile = j / (a.heads / 8);
+  } else {
+    head = block % a.heads;
+    tile = block / a.heads;
+  }
+}
+
 // The chunk that place `p` of a tile's plane holds: C chunks a row, a row's
 // chunks exchanged by k_place or v_place (both are their own inverse).
 template <int D, int C, bool VT>
@@ -139,7 +152,11 @@ struct Prompt {
   static constexpr int DT = (HD + 31) / 32;          // 32-dim tiles of O^T
   static constexpr int PLANE = KEYS * C;             // chunks of a tile's K or V
   static constexpr int QS = F32 ? 2 * KS : KS;       // operands of a query
-  static constexpr int SPAN = DT * 32 / V - C;       // chunks past a row that its last transposed read may touch
+  // Dims past a row's end in the last tile: chunks that an fp32 read may touch
+  // there; of 16-bit values a column of ones takes the first of them, which
+  // makes the matrix cores add up the softmax weights.
+  static constexpr int SPAN = DT * 32 / V - C;
+  static constexpr bool ONES = !F32 && SPAN > 0;
   static constexpr int JOIN = KG > 1 ? QG * KG * (DT * 16 + 2) * 16 : 0;  // chunks that the groups' sums take
   static constexpr int TILES = STAGES * KG * 2 * PLANE + SPAN;
   static constexpr int LDS = TILES > JOIN ? TILES : JOIN;
@@ -147,29 +164,30 @@ struct Prompt {
   typedef std::conditional_t<F32, float, uint16_t> Value;
 };
 
+// With `split` parts, block y takes the y-th of that many equal runs of its
+// tile's keys and leaves unnormalised records for prompt_join_kernel.
+struct Parts {
+  int split;
+  float2 *stats;   // [tile][head][part][query] {reference, sum}
+  float *values;   // [tile][head][part][query][hd]
+};
+
 template <int D, int KS, int QG, int KG, int KEYS, int STAGES, bool DMA>
 __global__ __launch_bounds__(64 * QG * KG) __attribute__((amdgpu_waves_per_eu(D != FMT_F32 && KS <= 8 ? 2 : 1)))
-void prompt_kernel(PromptArgs a) {
+void prompt_kernel(PromptArgs a, Parts parts) {
   using P = Prompt<D, KS, QG, KG, KEYS, STAGES, DMA>;
   using Value = typename P::Value;
   constexpr bool F32 = P::F32;
   constexpr int V = P::V, C = P::C, DT = P::DT, PLANE = P::PLANE, QS = P::QS, HALVES = KEYS / 32;
   constexpr float kLeap = 8.f;            // the reference moves only when a score exceeds it by 2^8
   __shared__ __align__(16) uint4 lds[P::LDS];
+  uint16_t *ones = reinterpret_cast<uint16_t *>(lds + P::TILES - P::SPAN);  // 1, 0, 0, 0; 0, 0, 0, 0
+  if (P::ONES && threadIdx.x < 8) ones[threadIdx.x] = threadIdx.x ? 0 : D == FMT_F16 ? 0x3c00 : 0x3f80;
 
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), qg = wave % QG, kg = wave / QG;
-  // Blocks go over the XCDs in turn: an XCD takes the same heads of every tile,
-  // so the blocks it runs share their keys in its L2.
   int head, tile;
-  if (a.heads % 8 == 0) {
-    const int j = blockIdx.x / 8;
-    head = blockIdx.x % 8 * (a.heads / 8) + j % (a.heads / 8);
-    tile = j / (a.heads / 8);
-  } else {
-    head = blockIdx.x % a.heads;
-    tile = blockIdx.x / a.heads;
-  }
+  tile_of(a, blockIdx.x, head, tile);
   const Where w = find<P::QB>(a, tile);
   if (w.tile < 0) return;
   const int kvh = head / (a.heads / a.kv_heads);
@@ -221,7 +239,7 @@ void prompt_kernel(PromptArgs a) {
 #pragma unroll
   for (int j = 0; j < NS; j++) {
     const bool vt = QG == 1 ? j >= N : second;
-    const int e = (part * N + j % N) * 64 + lane, r = e / C, c = vt ? chunk_at<D, C, true>(r, e % C) : chunk_at<D, C, false>(r, e % C);
+    const int e = (part * N + j % N) * 64 + lane, r = vt && !F32 ? v_key<C>(e / C) : e / C, c = vt ? chunk_at<D, C, true>(r, e % C) : chunk_at<D, C, false>(r, e % C);
     const int64_t ld = vt ? a.ldv : a.ldk;
     voff[j] = c * V < a.hd ? (uint32_t)((r * ld + c * V) * (int)sizeof(Value)) : kNone;
   }
@@ -232,7 +250,7 @@ void prompt_kernel(PromptArgs a) {
       const Value *at = base + (int64_t)t0 * ld;
       const uint32_t bytes = left ? (uint32_t)(((left - 1) * ld + a.hd) * (int)sizeof(Value)) : 0u;
       if constexpr (DMA) {
-        const __amdgpu_buffer_rsrc_t rsrc = plane_rsrc(reinterpret_cast<const uint8_t *>(at), bytes);
+        const __amdgpu_buffer_rsrc_t rsrc = plane_rsrc(uniform_ptr(reinterpret_cast<const uint8_t *>(at)), __builtin_amdgcn_readfirstlane((int)bytes));
         const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint4 *)(lds) +
                             (((stage * KG + kg) * 2 + vt) * PLANE + part * N * 64) * 16;
 #pragma unroll
@@ -263,14 +281,21 @@ void prompt_kernel(PromptArgs a) {
     }
   };
 
-  const int rounds = last_block < 0 ? 0 : (last_block / KEYS + KG) / KG;
+  // this block's rounds of KG tiles
+  int round = 0, rounds = last_block < 0 ? 0 : (last_block / KEYS + KG) / KG;
+  if (parts.split > 1) {
+    const int each = (rounds + parts.split - 1) / parts.split;
+    round = min((int)blockIdx.y * each, rounds);
+    rounds = min(round + each, rounds);
+  }
+  const int round0 = round;
   bool bad = false;
-  if (rounds) {
-    load(kg * KEYS, 0);
+  if (round < rounds) {
+    load((round * KG + kg) * KEYS, 0);
     if constexpr (!DMA) store(0);
   }
-  for (int round = 0; round < rounds; round++) {
-    const int t0 = (round * KG + kg) * KEYS, stage = STAGES == 2 ? round & 1 : 0;
+  for (; round < rounds; round++) {
+    const int t0 = (round * KG + kg) * KEYS, stage = STAGES == 2 ? (round - round0) & 1 : 0;
     if constexpr (DMA) wait_vmcnt<0>();
     __syncthreads();
     const bool more = round + 1 < rounds;
@@ -355,15 +380,15 @@ void prompt_kernel(PromptArgs a) {
             pw.y = pack2<D>(s[h][8 * st + 2], s[h][8 * st + 3]);
             pw.z = pack2<D>(s[h][8 * st + 4], s[h][8 * st + 5]);
             pw.w = pack2<D>(s[h][8 * st + 6], s[h][8 * st + 7]);
-            sum = plus2<D>(pw.x, plus2<D>(pw.y, plus2<D>(pw.z, plus2<D>(pw.w, sum))));
+            if constexpr (!P::ONES) sum = plus2<D>(pw.x, plus2<D>(pw.y, plus2<D>(pw.z, plus2<D>(pw.w, sum))));
             const int r0 = h * 32 + st * 16 + g * 4 + (lane & 15) / 4;
 #pragma unroll
             for (int t = 0; t < DT; t++) {
               const int d = t * 32 + (lane >> 4 & 1) * 16 + (lane & 3) * 4;
               auto read = [&](int r) {
-                const uint4 *chunk = vs + (r * C + v_place<C>(r, d / 8));
-                return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    (lds_s16x4 *)(reinterpret_cast<const uint16_t *>(chunk) + d % 8)));
+                const uint16_t *at = reinterpret_cast<const uint16_t *>(vs + (v_row<C>(r) * C + v_place<C>(r, d / 8))) + d % 8;
+                if (P::ONES && t == DT - 1 && (lane & 16)) at = ones + ((lane & 3) ? 4 : 0);
+                return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)at));
               };
               const uint2 lo = read(r0), hi = read(r0 + 8);
               o[t] = mfma<D>(make_uint4(lo.x, lo.y, hi.x, hi.y), pw, o[t]);
@@ -384,8 +409,12 @@ void prompt_kernel(PromptArgs a) {
     }
   }
   bad = __syncthreads_or(bad);
-  sum = halves_sum(sum);
+  if constexpr (P::ONES) sum = lower_half(o[DT - 1][8]);  // row 16 of the last tile: lanes 0 .. 31's value 8
+  else sum = halves_sum(sum);
   Value *out = static_cast<Value *>(a.out) + (w.q0 + mine) * a.ldo + (int64_t)head * a.hd;
+  // Of a part: this lane's query in the records.
+  const int64_t record = (((int64_t)tile * a.heads + head) * parts.split + blockIdx.y) * P::QB + qg * 32 + col;
+  const int fixed0 = max(first_block / (KG * KEYS), round0) * (KG * KEYS), fixed1 = min(last, rounds * KG * KEYS - 1);
   auto finish = [&](int t, f32x16 x, float inv) {
     if (mine >= w.nq) return;
 #pragma unroll
@@ -396,17 +425,24 @@ void prompt_kernel(PromptArgs a) {
 #pragma unroll
       for (int i = 0; i < 4; i++) y[i] = x[4 * j + i] * inv;
       if (bad)
-        for (int r = max(first_block / (KG * KEYS), 0) * (KG * KEYS); r <= last; r++)
+        for (int r = fixed0; r <= fixed1; r++)
           for (int i = 0; i < 4; i++) {
             const float u = mx_load(D, vp, r * a.ldv + d + i);
             if ((__float_as_uint(u) & 0x7f800000u) == 0x7f800000u) y[i] += u;
           }
-      if constexpr (F32) *reinterpret_cast<f32x4_any *>(out + d) = f32x4_any{y[0], y[1], y[2], y[3]};
+      if (parts.split > 1) *reinterpret_cast<f32x4_any *>(parts.values + record * a.hd + d) = f32x4_any{y[0], y[1], y[2], y[3]};
+      else if constexpr (F32) *reinterpret_cast<f32x4_any *>(out + d) = f32x4_any{y[0], y[1], y[2], y[3]};
       else *reinterpret_cast<u32x2_any *>(out + d) = u32x2_any{pack2<D>(y[0], y[1]), pack2<D>(y[2], y[3])};
     }
   };
+  // what the sums are multiplied by, and a part's reference and sum
+  auto ending = [&](float top, float all, bool leader) {
+    if (parts.split == 1) return all == 0.f ? 0.f : 1.f / all;
+    if (leader && g == 0 && mine < w.nq) parts.stats[record] = make_float2(top, all);
+    return 1.f;
+  };
   if constexpr (KG == 1) {
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const float inv = ending(ref, sum, true);
 #pragma unroll
     for (int t = 0; t < DT; t++) finish(t, o[t], inv);
   } else {
@@ -428,7 +464,7 @@ void prompt_kernel(PromptArgs a) {
       fade[i] = top == -INFINITY ? 0.f : exp2_hw(f[(i * QG + qg) * W] - top);
       all += fade[i] * f[(i * QG + qg) * W + 64];
     }
-    const float inv = all == 0.f ? 0.f : 1.f / all;
+    const float inv = ending(top, all, kg == 0);
     for (int t = kg; t < DT; t += KG) {
       f32x16 x;
 #pragma unroll
@@ -446,34 +482,94 @@ void prompt_kernel(PromptArgs a) {
 
 namespace {
 
+// The parts of a query, joined in order; four dims a thread.
+template <int QB>
+__global__ __launch_bounds__(256) void prompt_join_kernel(PromptArgs a, Parts p) {
+  int head, tile;
+  tile_of(a, blockIdx.x, head, tile);
+  const Where w = find<QB>(a, tile);
+  if (w.tile < 0) return;
+  const int wide = a.hd / 4;
+  for (int i = blockIdx.y * 256 + threadIdx.x; i < QB * wide; i += gridDim.y * 256) {
+    const int row = i / wide, d = i % wide * 4, mine = w.tile * QB + row;
+    if (mine >= w.nq) return;
+    const int64_t first = ((int64_t)tile * a.heads + head) * p.split * QB + row;
+    float top = -INFINITY, sum = 0.f;
+    for (int s = 0; s < p.split; s++) top = fmaxf(top, p.stats[first + s * QB].x);
+    float o[4] = {};
+#pragma unroll 4
+    for (int s = 0; s < p.split; s++) {
+      const float2 x = p.stats[first + s * QB];
+      const f32x4_any v = *reinterpret_cast<const f32x4_any *>(p.values + (first + s * QB) * a.hd + d);
+      const float fade = top == -INFINITY ? 0.f : exp2_hw(x.x - top);
+      sum += fade * x.y;
+#pragma unroll
+      for (int j = 0; j < 4; j++) o[j] += fade * v[j];
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    for (int j = 0; j < 4; j++) mx_store(a.dtype, a.out, (w.q0 + mine) * a.ldo + (int64_t)head * a.hd + d + j, o[j] * inv);
+  }
+}
+
+// How a call is run: query groups, key groups of a block, parts of the keys.
+struct Shape {
+  int qg, kg, split;
+};
+int64_t tiles_of(const PromptArgs &a, int qb) {  // at most: every sequence's last tile may be a part
+  return a.nq / qb + std::min<int64_t>(a.sequences, a.nq);
+}
+Shape shape_of(const PromptArgs &a) {
+  Shape s{4, 1, 1};
+  const int64_t blocks = tiles_of(a, 128) * a.heads, keys = a.nk / std::max(1, std::min(a.sequences, a.nk));
+  if (blocks >= 256) return s;
+  if (a.dtype == FMT_F32) {
+    s = Shape{1, a.hd > 128 ? 2 : 4, 1};
+    const int64_t few = tiles_of(a, 32) * a.heads;
+    s.split = (int)std::min(512 / few, keys / (32 * s.kg));
+  } else if (keys >= 2048 && blocks <= 256) {
+    s.split = (int)std::min(512 / blocks, keys / 1024);
+  } else if (a.nq <= 32) {
+    s = Shape{1, 4, 1};
+  } else if (a.hd <= 128) {
+    s = Shape{2, 4, 1};
+  }
+  if (s.split < 1) s.split = 1;
+  return s;
+}
+
 template <int D, int KS, int QG, int KG, int KEYS, int STAGES>
-void launch(const PromptArgs &a, bool dma, hipStream_t st) {
-  constexpr int QB = 32 * QG;
-  // at most: every sequence's last tile may be a part
-  const int64_t tiles = a.nq / QB + std::min<int64_t>(a.sequences, a.nq);
-  const dim3 grid((unsigned)(tiles * a.heads)), block(64 * QG * KG);
-  if (dma) hipLaunchKernelGGL((prompt_kernel<D, KS, QG, KG, KEYS, STAGES, true>), grid, block, 0, st, a);
-  else hipLaunchKernelGGL((prompt_kernel<D, KS, QG, KG, KEYS, STAGES, false>), grid, block, 0, st, a);
+void launch(const PromptArgs &a, const Parts &p, bool dma, hipStream_t st) {
+  const dim3 grid((unsigned)(tiles_of(a, 32 * QG) * a.heads), (unsigned)p.split), block(64 * QG * KG);
+  if (dma) hipLaunchKernelGGL((prompt_kernel<D, KS, QG, KG, KEYS, STAGES, true>), grid, block, 0, st, a, p);
+  else hipLaunchKernelGGL((prompt_kernel<D, KS, QG, KG, KEYS, STAGES, false>), grid, block, 0, st, a, p);
 }
 
 bool aligned16(const void *p, int64_t ld, int width) { return (reinterpret_cast<uintptr_t>(p) | (uintptr_t)(ld * width)) % 16 == 0; }
 
 }  // namespace
 
-hipError_t launch_prompt(const PromptArgs &a, hipStream_t st) {
+size_t prompt_scratch(const PromptArgs &a) {
+  const Shape s = shape_of(a);
+  return s.split == 1 ? 0 : (size_t)tiles_of(a, 32 * s.qg) * a.heads * s.split * 32 * s.qg * (a.hd + 2) * 4;
+}
+
+hipError_t launch_prompt(const PromptArgs &a, void *scratch, hipStream_t st) {
   const int width = (int)mx_width(a.dtype);
   const bool dma = aligned16(a.k, a.ldk, width) && aligned16(a.v, a.ldv, width);
-  const int64_t blocks = (a.nq / 128 + std::min<int64_t>(a.sequences, a.nq)) * a.heads;
+  const Shape s = shape_of(a);
+  Parts p{s.split, nullptr, static_cast<float *>(scratch)};
+  const int64_t tiles = tiles_of(a, 32 * s.qg);
+  if (s.split > 1) p.stats = reinterpret_cast<float2 *>(p.values + tiles * a.heads * s.split * 32 * s.qg * a.hd);
   auto go = [&](auto d, auto k) {
     constexpr int D = decltype(d)::value, KS = decltype(k)::value;
+    constexpr bool wide = KS > 8;
     if constexpr (D == FMT_F32) {
-      constexpr bool wide = KS > 8;
-      if (blocks < 256) launch<D, KS, 1, wide ? 2 : 4, 32, KS <= 4 ? 2 : 1>(a, dma, st);
-      else launch<D, KS, 4, 1, 32, wide ? 1 : 2>(a, dma, st);
+      if (s.qg == 1) launch<D, KS, 1, wide ? 2 : 4, 32, KS <= 4 ? 2 : 1>(a, p, dma, st);
+      else launch<D, KS, 4, 1, 32, wide ? 1 : 2>(a, p, dma, st);
     } else {
-      if (blocks < 256 && a.nq <= 32) launch<D, KS, 1, 4, 32, KS <= 8 ? 2 : 1>(a, dma, st);
-      else if (blocks < 256 && KS <= 8) launch<D, KS, KS <= 8 ? 2 : 4, KS <= 8 ? 4 : 1, 32, 2>(a, dma, st);
-      else launch<D, KS, 4, 1, KS <= 8 ? 64 : 32, 2>(a, dma, st);
+      if (s.qg == 1) launch<D, KS, 1, 4, 32, wide ? 1 : 2>(a, p, dma, st);
+      else if (s.qg == 2) launch<D, KS, wide ? 4 : 2, wide ? 1 : 4, 32, 2>(a, p, dma, st);
+      else launch<D, KS, 4, 1, wide ? 32 : 64, 2>(a, p, dma, st);
     }
   };
   for_type(a.dtype, [&](auto d) {
@@ -484,5 +580,10 @@ hipError_t launch_prompt(const PromptArgs &a, hipStream_t st) {
     else if (a.hd <= 128) go(d, std::integral_constant<int, 8>());
     else go(d, std::integral_constant<int, 16>());
   });
+  if (p.split > 1) {
+    const dim3 grid((unsigned)(tiles * a.heads), (unsigned)(s.qg == 1 ? 2 : 4));
+    if (s.qg == 1) hipLaunchKernelGGL((prompt_join_kernel<32>), grid, dim3(256), 0, st, a, p);
+    else hipLaunchKernelGGL((prompt_join_kernel<128>), grid, dim3(256), 0, st, a, p);
+  }
   return hipGetLastError();
 }

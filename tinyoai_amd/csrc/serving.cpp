@@ -2,7 +2,9 @@
 // paged key-value cache, attention over its pages and of packed prompts.
 #include <cmath>
 #include <exception>
+#include <map>
 #include <memory>
+#include <mutex>
 #include <vector>
 
 #include "attend.h"
@@ -119,6 +121,19 @@ int kv_rows(tinyoai_kv_pages *c, int32_t layer, int32_t dtype, const void *k, in
   const KVRowsArgs a{layer_pages(*c, layer), dtype, const_cast<void *>(k), const_cast<void *>(v), ldk, ldv, slots, n};
   const hipError_t e = launch(a, stream ? (hipStream_t)stream : c->stream);
   return e == hipSuccess ? TINYOAI_OK : hip_fail(e, "paged cache rows");
+}
+
+// Scratch of the calls without a handle on the current device; kept until the
+// process ends (no destructor, which might run after the runtime's).
+StreamScratch &attention_scratch() {
+  static std::mutex mu;
+  static std::map<int, StreamScratch *> *scratch = new std::map<int, StreamScratch *>;
+  int device = 0;
+  (void)hipGetDevice(&device);
+  std::lock_guard<std::mutex> lock(mu);
+  StreamScratch *&s = (*scratch)[device];
+  if (!s) s = new StreamScratch;
+  return *s;
 }
 
 }  // namespace
@@ -264,7 +279,7 @@ int tinyoai_kv_pages_close(tinyoai_kv_pages *c) {
 int tinyoai_attention_device(int32_t dtype, const void *q_dev, int64_t ldq, int32_t heads, const void *k_dev, int64_t ldk,
                              const void *v_dev, int64_t ldv, int32_t kv_heads, int32_t head_dim, float scale, int32_t causal,
                              const int32_t *q_offsets_dev, const int32_t *k_offsets_dev, int32_t sequences, int32_t nq,
-                             int32_t nk, void *out_dev, int64_t ldo, void *stream) {
+                             int32_t nk, void *out_dev, int64_t ldo, void *stream) try {
   if (!head_width(head_dim)) return fail(TINYOAI_EINVAL, "unsupported head width %d", head_dim);
   if (kv_heads <= 0 || heads <= 0 || heads % kv_heads || (int64_t)heads * head_dim > kRowValues)
     return fail(TINYOAI_EINVAL, "%d query heads over %d key heads", heads, kv_heads);
@@ -278,10 +293,15 @@ int tinyoai_attention_device(int32_t dtype, const void *q_dev, int64_t ldq, int3
   if (((int64_t)nq / 128 + std::min(sequences, nq)) * heads >= 1 << 24)
     return fail(TINYOAI_EINVAL, "%d queries of %d sequences by %d heads exceed what one call takes", nq, sequences, heads);
   if (!nq) return TINYOAI_OK;
-  const hipError_t e = launch_prompt(PromptArgs{dtype, q_dev, k_dev, v_dev, ldq, ldk, ldv, heads, kv_heads, head_dim, scale,
-                                                causal, q_offsets_dev, k_offsets_dev, sequences, nq, nk, out_dev, ldo},
-                                     (hipStream_t)stream);
+  const PromptArgs a{dtype, q_dev, k_dev, v_dev, ldq, ldk, ldv, heads, kv_heads, head_dim, scale, causal, q_offsets_dev,
+                     k_offsets_dev, sequences, nq, nk, out_dev, ldo};
+  const size_t bytes = prompt_scratch(a);
+  hipStream_t st = (hipStream_t)stream;
+  if (bytes) return attention_scratch().run(st, bytes, [&](void *scratch) { return launch_prompt(a, scratch, st); });
+  const hipError_t e = launch_prompt(a, nullptr, st);
   return e == hipSuccess ? TINYOAI_OK : hip_fail(e, "attention");
+} catch (const std::exception &e) {
+  return fail(TINYOAI_ENOMEM, "attention: %s", e.what());
 }
 
 }  // extern "C"
