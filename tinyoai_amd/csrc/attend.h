@@ -167,6 +167,23 @@ __device__ __forceinline__ float lower_half(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return __uint_as_float(r[0]);
 }
+// As lds_dma16 and lds_dma4 (or from an address per lane), for a descriptor or a
+// place in LDS that a lane read has just put into scalar registers: the
+// hardware wants five wait states between that and the load, and the compiler,
+// which sees to it elsewhere, does not look into inline assembly.
+__device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, uint32_t voff, uint32_t lds_byte) {
+  asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(r), "{m0}"(lds_byte) : "memory");
+}
+__device__ __forceinline__ void dma4(__amdgpu_buffer_rsrc_t r, uint32_t voff, uint32_t lds_byte) {
+  asm volatile("s_nop 4\n\tbuffer_load_dword %0, %1, 0 offen lds" ::"v"(voff), "s"(r), "{m0}"(lds_byte) : "memory");
+}
+__device__ __forceinline__ void dma16_at(const void *p, uint32_t lds_byte) {
+  asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "{m0}"(lds_byte) : "memory");
+}
+__device__ __forceinline__ void dma4_at(const void *p, uint32_t lds_byte) {
+  asm volatile("s_nop 4\n\tglobal_load_lds_dword %0, off" ::"v"(p), "{m0}"(lds_byte) : "memory");
+}
+
 // Over lanes l and l ^ 32, and (quarters) l, l ^ 16, l ^ 32 and l ^ 48.
 __device__ __forceinline__ float halves_max(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);

@@ -58,14 +58,6 @@ __device__ __forceinline__ void store4(int dtype, void *p, int64_t i, f32x4 v) {
   }
 }
 
-// 16 bytes, or 4, of an address per lane straight into LDS, as lds_dma16.
-__device__ __forceinline__ void lds_dma16_at(const void *p, uint32_t lds_byte) {
-  asm volatile("global_load_lds_dwordx4 %0, off" ::"v"(p), "{m0}"(lds_byte) : "memory");
-}
-__device__ __forceinline__ void lds_dma4_at(const void *p, uint32_t lds_byte) {
-  asm volatile("global_load_lds_dword %0, off" ::"v"(p), "{m0}"(lds_byte) : "memory");
-}
-
 constexpr int kUnit = 32;  // positions: what the work is dealt out by
 
 struct Plan {
@@ -287,11 +279,11 @@ void attend_kernel(AttendArgs a, Plan plan) {
       const int64_t row = kv_row(a.c, (count ? page : 0) << lg | (t0 & ((1 << lg) - 1)), kvh);
       const __amdgpu_buffer_rsrc_t rows = plane_rsrc(uniform_ptr(base + row * a.c.pitch), count * a.c.pitch);
 #pragma unroll
-      for (int j = 0; j < N; j++) lds_dma16(rows, off[j], __builtin_amdgcn_readfirstlane(to + j * 1024));
+      for (int j = 0; j < N; j++) dma16(rows, off[j], __builtin_amdgcn_readfirstlane(to + j * 1024));
       if constexpr (Q8) {
         const __amdgpu_buffer_rsrc_t sc = plane_rsrc(uniform_ptr(reinterpret_cast<const uint8_t *>(scales + row * NB)), count * NB * 2);
 #pragma unroll
-        for (int j = 0; j < A::NSC; j++) lds_dma4(sc, (j * 64 + lane) * 4, __builtin_amdgcn_readfirstlane(to + N * 1024 + j * 256));
+        for (int j = 0; j < A::NSC; j++) dma4(sc, (j * 64 + lane) * 4, __builtin_amdgcn_readfirstlane(to + N * 1024 + j * 256));
       }
       return count >= 32 ? 0xffffffffu : (1u << count) - 1u;
     }
@@ -305,7 +297,7 @@ void attend_kernel(AttendArgs a, Plan plan) {
     for (int j = 0; j < N; j++) {
       bool ok;
       const int64_t row = row_of((j * 64 + lane) / C, ok) * a.c.pitch;
-      lds_dma16_at(ok && off[j] != kNone ? base + row + off[j] : a.c.zeros, __builtin_amdgcn_readfirstlane(to + j * 1024));
+      dma16_at(ok && off[j] != kNone ? base + row + off[j] : a.c.zeros, __builtin_amdgcn_readfirstlane(to + j * 1024));
     }
     if constexpr (Q8) {
 #pragma unroll
@@ -313,7 +305,7 @@ void attend_kernel(AttendArgs a, Plan plan) {
         const int e = j * 64 + lane;  // a pair of scales
         bool ok;
         const int64_t row = row_of(e * 2 / NB, ok) * NB;
-        lds_dma4_at(ok ? (const void *)(scales + row + e * 2) : a.c.zeros, __builtin_amdgcn_readfirstlane(to + N * 1024 + j * 256));
+        dma4_at(ok ? (const void *)(scales + row + e * 2) : a.c.zeros, __builtin_amdgcn_readfirstlane(to + N * 1024 + j * 256));
       }
     }
     bool ok;
