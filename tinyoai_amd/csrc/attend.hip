@@ -96,9 +96,10 @@ struct Attend {
   static_assert(LOADS < 64, "loads in flight");
 };
 
-// The planes of eight values: element by element for the fp32 instructions,
-// else packed; their sum is the value to 8 (bf16) or 11 bits a plane.
-template <int CT, int P>
+// The planes of eight values, packed; their sum is the value to 8 (bf16) or 11
+// bits a plane. WEIGHTS: never infinite (a NaN gives one in any case), which
+// spares the tests that keep an infinity from becoming one.
+template <int CT, bool WEIGHTS, int P>
 __device__ __forceinline__ void planes_of8(const float (&v)[8], uint4 (&out)[P]) {
   if constexpr (CT == FMT_F16) {
     float rest[8];
@@ -119,7 +120,18 @@ __device__ __forceinline__ void planes_of8(const float (&v)[8], uint4 (&out)[P])
   } else {
     uint32_t h[8][P];
 #pragma unroll
-    for (int j = 0; j < 8; j++) tinyoai_mx::planes_of<P>(v[j], h[j]);
+    for (int j = 0; j < 8; j++) {
+      if constexpr (WEIGHTS) {
+        float rest = v[j];
+#pragma unroll
+        for (int p = 0; p < P; p++) {
+          h[j][p] = __float_as_uint(rest) & 0xffff0000u;
+          rest -= __uint_as_float(h[j][p]);
+        }
+      } else {
+        tinyoai_mx::planes_of<P>(v[j], h[j]);
+      }
+    }
 #pragma unroll
     for (int p = 0; p < P; p++)
       out[p] = make_uint4(tinyoai_mx::high_halves(h[0][p], h[1][p]), tinyoai_mx::high_halves(h[2][p], h[3][p]),
@@ -380,7 +392,7 @@ void attend_kernel(AttendArgs a, Plan plan) {
         scale = ldexpf(scale, -e);
       }
 #pragma unroll
-      for (int s = 0; s < QS; s++) planes_of8<CT>(v[s], q[s]);
+      for (int s = 0; s < QS; s++) planes_of8<CT, false>(v[s], q[s]);
     }
   };
 
@@ -496,7 +508,7 @@ void attend_kernel(AttendArgs a, Plan plan) {
         scales_of(vs + N * 64, 0, dv[0]);
         scales_of(vs + N * 64, 1, dv[1]);
       } else {
-        planes_of8<CT>(w, p);
+        planes_of8<CT, true>(w, p);
       }
 #pragma unroll
       for (int t = 0; t < DT; t++) {
@@ -506,7 +518,7 @@ void attend_kernel(AttendArgs a, Plan plan) {
             float x[8];
 #pragma unroll
             for (int j = 0; j < 8; j++) x[j] = w[j] * dv[j >> 2][(j & 3) * NB + t / 2];
-            planes_of8<CT>(x, p);
+            planes_of8<CT, true>(x, p);
           }
           const int k = (lane & 15) >> 1, r = (k >> 2) * 16 + g * 4 + (k & 3);
           const uint2 *chunk = reinterpret_cast<const uint2 *>(vs + r * C + v_place<C>(r, t)) + (lane & 1);
@@ -575,6 +587,12 @@ __global__ __launch_bounds__(kJoin) void attend_join_kernel(AttendArgs a, Plan p
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
   for (int i0 = 0; i0 < pieces; i0 += kJoin) {
     const float2 x = i0 + tid < pieces ? p.stats[piece(i0 + tid)] : make_float2(-INFINITY, 0.f);
+    const int end = min(pieces - i0, kJoin);
+    constexpr int B = 4;  // rows that come together with the factors
+    f32x4 rows[B];
+#pragma unroll
+    for (int j = 0; j < B; j++)
+      rows[j] = d < hd && side + j * sides < end ? *reinterpret_cast<const f32x4 *>(p.values + piece(i0 + side + j * sides) * hd + d) : f32x4{0.f, 0.f, 0.f, 0.f};
     const float w = wave_max(x.x);
     if ((tid & 63) == 0) red[0][wave] = w;
     __syncthreads();
@@ -588,9 +606,11 @@ __global__ __launch_bounds__(kJoin) void attend_join_kernel(AttendArgs a, Plan p
     sum = sum * fade + ((red[1][0] + red[1][1]) + (red[1][2] + red[1][3]));
     o *= fade;
     if (d < hd) {
-      const int end = min(pieces - i0, kJoin);
+#pragma unroll
+      for (int j = 0; j < B; j++)
+        if (side + j * sides < end) o += fades[side + j * sides] * rows[j];
 #pragma unroll 4
-      for (int i = side; i < end; i += sides) o += fades[i] * *reinterpret_cast<const f32x4 *>(p.values + piece(i0 + i) * hd + d);
+      for (int i = side + B * sides; i < end; i += sides) o += fades[i] * *reinterpret_cast<const f32x4 *>(p.values + piece(i0 + i) * hd + d);
     }
     __syncthreads();
   }

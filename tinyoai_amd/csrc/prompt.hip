@@ -649,7 +649,7 @@ Shape shape_of(const PromptArgs &a) {
   if (a.dtype == FMT_F32) {
     s = Shape{1, a.hd > 128 ? 2 : 4, 1};
     const int64_t few = tiles_of(a, 32) * a.heads;
-    s.split = (int)std::min(512 / few, keys / (32 * s.kg));
+    s.split = (int)std::min(512 / few, (keys + 32 * s.kg - 1) / (32 * s.kg));
   } else if (keys >= 2048 && blocks <= 256) {
     s.split = (int)std::min(512 / blocks, keys / 1024);
   } else if (a.nq <= 32) {
