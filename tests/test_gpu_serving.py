@@ -296,7 +296,7 @@ def _weights_rounded(cache, dtype):
 
 ATTEND = [(1, 1, 8, 1, (1,)), (8, 4, 8, 16, (1, 0, 5, 160)), (4, 4, 80, 64, (700, 1, 63, 64, 65)), (8, 2, 64, 16, (17, 0, 300, 15)),
           (6, 2, 72, 32, (130, 31, 33)), (16, 1, 128, 128, (129, 257, 1)), (12, 4, 256, 8, (40, 9, 8)), (5, 1, 96, 4, (3, 100)),
-          (20, 1, 64, 64, (90, 64)), (34, 2, 40, 16, (50,))]
+          (20, 1, 64, 64, (90, 64)), (34, 2, 40, 16, (50,)), (3, 1, 160, 16, (70, 33)), (2, 2, 200, 32, (64,))]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -408,7 +408,7 @@ def _prompt_check(hip, dev, rng, dtype, heads, kv, hd, lengths, causal, pad=0, s
 
 PROMPTS = [(1, 1, 8, ((1, 1),)), (8, 4, 8, ((5, 5), (0, 0), (64, 64), (1, 1))), (4, 4, 80, ((19, 449), (130, 130))),
            (8, 2, 64, ((33, 33), (200, 77), (7, 0), (129, 300))), (4, 1, 72, ((65, 65), (3, 190))), (16, 2, 128, ((150, 150), (1, 257))),
-           (2, 1, 256, ((70, 131), (128, 128))), (3, 3, 96, ((31, 32), (140, 63))), (6, 2, 40, ((90, 90),)), (1, 1, 160, ((50, 99),))]
+           (2, 1, 256, ((70, 131), (128, 128))), (3, 3, 96, ((31, 32), (140, 63))), (6, 2, 40, ((90, 90),)), (1, 1, 160, ((50, 99),)), (2, 1, 200, ((33, 40),))]
 
 
 @pytest.mark.parametrize("causal", [True, False])
@@ -465,6 +465,84 @@ def test_prompt_offsets(hip, dev):
         for q0, q1, k0, k1 in ((0, 5, 0, 4), (5, 9, 8, 8), (9, 18, 8, 20)):
             want, mag, load = _attention(q[q0:q1], q[k0:k1], q[k0:k1], 0.125)
             assert np.all(np.abs(got[q0:q1] - want) <= _tolerance(want, mag, load, 20, 64, dtype, 0 if dtype == W.F32 else EPS[dtype]))
+
+
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 7.0])
+def test_scales(hip, dev, scale):
+    """Scales of any sign, and zero: the mean of the values."""
+    rng = np.random.default_rng(18)
+    for dtype in TYPES:
+        hd, n, keys = 64, 40, 70
+        (pq, _, q), (pk, _, k), (pv, _, v) = (_rows(rng, dev, dtype, m, hd) for m in (n, keys, keys))
+        out = _empty(dev, dtype, n, hd)
+        hip.attention(dtype, pq, hd, 1, pk, hd, pv, hd, 1, hd, scale, False, dev.put(np.array([0, n], np.int32)),
+                      dev.put(np.array([0, keys], np.int32)), 1, n, keys, out, hd)
+        s = q @ k.T * scale
+        p = np.exp(s - s.max(-1, keepdims=True))
+        p /= p.sum(-1, keepdims=True)
+        want, mag, load = p @ v, p @ np.abs(v), (np.abs(q) @ np.abs(k).T * abs(scale)).max(-1, keepdims=True)
+        tol = _tolerance(want, mag, load, keys, hd, dtype, 0 if dtype == W.F32 else EPS[dtype])
+        assert np.all(np.abs(decode(dtype, dev.get(out, (n, hd), bits_dtype(dtype))) - want) <= tol)
+        for cache in CACHES:
+            c = hip.KVPages(cache, 1, 1, hd, 16, 5)
+            c.write(0, dtype, pk, hd, pv, hd, dev.put(np.arange(keys, dtype=np.int32)), keys)
+            c.attend(0, dtype, pq, hd, 1, scale, dev.put(np.tile(np.arange(5, dtype=np.int32), n)), 5,
+                     dev.put(np.full(n, keys, np.int32)), n, out, hd)
+            kc, vc = _held(cache, k, hd), _held(cache, v, hd)
+            s = q @ kc.T * scale
+            p = np.exp(s - s.max(-1, keepdims=True))
+            p /= p.sum(-1, keepdims=True)
+            want, mag, load = p @ vc, p @ np.abs(vc), (np.abs(q) @ np.abs(kc).T * abs(scale)).max(-1, keepdims=True)
+            tol = _tolerance(want, mag, load, keys, hd, dtype, _weights_rounded(cache, dtype))
+            assert np.all(np.abs(decode(dtype, dev.get(out, (n, hd), bits_dtype(dtype))) - want) <= tol), cache
+            c.close()
+
+
+@pytest.mark.parametrize("cache,page", [(W.F32, 1024), (W.F16, 8)])
+def test_pool_past_32_bits(hip, dev, cache, page):
+    """A pool whose planes pass 4 GiB: rows at both ends."""
+    rng = np.random.default_rng(19)
+    heads, hd = 8, 256
+    pages = (5 << 30) // (page * heads * hd * (4 if cache == W.F32 else 2))
+    c = hip.KVPages(cache, 1, heads, hd, page, pages)
+    table = np.array([[pages - 1, 0, pages - 2]], np.int32)
+    length = 2 * page + 5
+    t = np.arange(length)
+    slots = (table[0, t // page] * page + t % page).astype(np.int32)
+    (pk, ld, k), (pv, _, v), (pq, _, q) = (_rows(rng, dev, W.F32, n, heads * hd) for n in (length, length, 1))
+    ps = dev.put(slots)
+    c.write(0, W.F32, pk, ld, pv, ld, ps, length)
+    ko, vo, out = (_empty(dev, W.F32, n, heads * hd) for n in (length, length, 1))
+    c.read(0, W.F32, ko, ld, vo, ld, ps, length)
+    k, v = _held(cache, k, hd), _held(cache, v, hd)
+    assert np.array_equal(dev.get(ko, k.shape), k) and np.array_equal(dev.get(vo, v.shape), v)
+    c.attend(0, W.F32, pq, ld, heads, 0.0625, dev.put(table), 3, dev.put(np.array([length], np.int32)), 1, out, ld)
+    got = dev.get(out, (heads, hd))
+    for h in range(heads):
+        g = slice(h * hd, h * hd + hd)
+        want, mag, load = _attention(q[:, g], k[:, g], v[:, g], 0.0625)
+        assert np.all(np.abs(got[h] - want[0]) <= _tolerance(want, mag, load, length, hd, W.F32, 0)[0])
+    c.close()
+
+
+def test_prompt_past_32_bits(hip, dev):
+    """Rows of keys and values 8 MiB apart, 5.6 GiB of them."""
+    rng = np.random.default_rng(20)
+    hd, n, keys, ld = 64, 50, 700, 1 << 22
+    buf = dev.room((keys * ld + 2 * hd) * 2)
+    (kb, k), (vb, v) = (encode(W.F16, rng.standard_normal((keys, hd))) for _ in range(2))
+    both = np.concatenate([kb, vb], 1)
+    for r in range(keys):
+        row = np.ascontiguousarray(both[r])
+        assert dev.rt.hipMemcpy(buf + r * ld * 2, row.ctypes.data, row.nbytes, 1) == 0
+    pq, _, q = _rows(rng, dev, W.F16, n, hd)
+    out = _empty(dev, W.F16, n, hd)
+    hip.attention(W.F16, pq, hd, 1, buf, ld, buf + 2 * hd, ld, 1, hd, 0.125, True, dev.put(np.array([0, n], np.int32)),
+                  dev.put(np.array([0, keys], np.int32)), 1, n, keys, out, hd)
+    seen = np.arange(keys) <= np.arange(n)[:, None] + keys - n
+    want, mag, load = _attention(q, k, v, 0.125, seen)
+    tol = _tolerance(want, mag, load, keys, hd, W.F16, EPS[W.F16])
+    assert np.all(np.abs(decode(W.F16, dev.get(out, (n, hd), np.uint16)) - want) <= tol)
 
 
 # ---------------------------------------------------------------- streams, graphs, threads
