@@ -291,7 +291,9 @@ def _attend_check(hip, dev, rng, cache, dtype, heads, kv, hd, page, lengths, pad
 
 
 def _weights_rounded(cache, dtype):
-    return 0.0
+    """New tokens' weights: fp32 in all their bits, or for 16-bit results two planes of eight bits, the second cut short
+    (what a plane leaves is below 2^-7 of what it was)."""
+    return 0.0 if dtype == W.F32 or cache == W.F32 else 2.0 ** -14
 
 
 ATTEND = [(1, 1, 8, 1, (1,)), (8, 4, 8, 16, (1, 0, 5, 160)), (4, 4, 80, 64, (700, 1, 63, 64, 65)), (8, 2, 64, 16, (17, 0, 300, 15)),

@@ -39,12 +39,13 @@ def hipcc() -> str:
     raise RuntimeError("hipcc not found")
 
 
-# Per-source additions: the Q8_0 wide-tile and the fp32-accurate kernels keep
-# their matrix-core results in ordinary vector registers (each K step's
-# products are rescaled or added on the vector unit, which cannot read the
-# accumulation registers); the BF16 kernels keep theirs in the accumulation registers.
+# Per-source additions: the Q8_0 wide-tile, the fp32-accurate and the prompts'
+# attention kernels keep their matrix-core results in ordinary vector registers
+# (each K step's products are rescaled or added on the vector unit, which cannot
+# read the accumulation registers); the BF16 kernels keep theirs in the accumulation registers.
 EXTRA = {"gemm_q8.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
-         "gemm_exact.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+         "gemm_exact.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+         "prompt.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 
 
 def _compile(src: str) -> str:

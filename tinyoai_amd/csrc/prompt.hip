@@ -178,7 +178,7 @@ struct Parts {
 };
 
 template <int D, int KS, int QN, int QG, int KG, int KEYS, int STAGES, bool DMA>
-__global__ __launch_bounds__(64 * QG * KG) __attribute__((amdgpu_waves_per_eu(D == FMT_F32 || KS > 8 ? 1 : KS == 5 && QG == 4 && DMA ? 3 : 2)))
+__global__ __launch_bounds__(64 * QG * KG) __attribute__((amdgpu_waves_per_eu(KS > 8 ? 1 : D != FMT_F32 && KS == 5 && QG == 4 && DMA ? 3 : 2)))
 void prompt_kernel(PromptArgs a, Parts parts) {
   using P = Prompt<D, KS, QN, QG, KG, KEYS, STAGES, DMA>;
   static_assert(QN == 1 || KG == 1, "one or the other");
@@ -471,9 +471,8 @@ void prompt_kernel(PromptArgs a, Parts parts) {
             x[t] = make_uint4(lo.x, lo.y, hi.x, hi.y);
           }
         };
-        // (heads of 80: a third wave a SIMD, which the registers then hold, is worth more)
-        constexpr bool PIPE = KS != 5;
-        if constexpr (!PIPE) {
+        // (KS 5: in turn, which leaves registers for a third wave a SIMD: 1620 against 1680 us for 16381 tokens of 32 heads of 80)
+        if constexpr (KS == 5) {
 #pragma unroll
           for (int i = 0; i < STEPS; i++) {
             uint4 x[DT];
@@ -483,32 +482,32 @@ void prompt_kernel(PromptArgs a, Parts parts) {
             for (int t = 0; t < DT; t++) o[0][t] = mfma<D>(x[t], p, o[0][t]);
           }
         } else {
-        uint4 x[2][DT], p[2][QN];
-        operands(0, x[0]);
+          uint4 x[2][DT], p[2][QN];
+          operands(0, x[0]);
 #pragma unroll
-        for (int n = 0; n < QN; n++) p[0][n] = weights(n, 0);
+          for (int n = 0; n < QN; n++) p[0][n] = weights(n, 0);
 #pragma unroll
-        for (int i = 0; i < STEPS; i++) {
-          __builtin_amdgcn_sched_barrier(0);
-          if (i + 1 < STEPS) {
-            operands(i + 1, x[(i + 1) & 1]);
+          for (int i = 0; i < STEPS; i++) {
+            __builtin_amdgcn_sched_barrier(0);
+            if (i + 1 < STEPS) {
+              operands(i + 1, x[(i + 1) & 1]);
 #pragma unroll
-            for (int n = 0; n < QN; n++) p[(i + 1) & 1][n] = weights(n, i + 1);
-          }
+              for (int n = 0; n < QN; n++) p[(i + 1) & 1][n] = weights(n, i + 1);
+            }
 #pragma unroll
-          for (int t = 0; t < DT; t++)
+            for (int t = 0; t < DT; t++)
 #pragma unroll
-            for (int n = 0; n < QN; n++) o[n][t] = mfma<D>(x[i & 1][t], p[i & 1][n], o[n][t]);
-          if (i + 1 < STEPS) {
-            __builtin_amdgcn_sched_group_barrier(kReads, 2 * DT, 0);
+              for (int n = 0; n < QN; n++) o[n][t] = mfma<D>(x[i & 1][t], p[i & 1][n], o[n][t]);
+            if (i + 1 < STEPS) {
+              __builtin_amdgcn_sched_group_barrier(kReads, 2 * DT, 0);
 #pragma unroll
-            for (int t = 0; t < DT * QN; t++) {
-              __builtin_amdgcn_sched_group_barrier(kProducts, 1, 0);
-              __builtin_amdgcn_sched_group_barrier(kVector, 16 / DT, 0);
-              __builtin_amdgcn_sched_group_barrier(kExponents, 8 / DT, 0);
+              for (int t = 0; t < DT * QN; t++) {
+                __builtin_amdgcn_sched_group_barrier(kProducts, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(kVector, 16 / DT, 0);
+                __builtin_amdgcn_sched_group_barrier(kExponents, 8 / DT, 0);
+              }
             }
           }
-        }
         }
       }
     }
