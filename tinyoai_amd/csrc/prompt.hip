@@ -15,6 +15,18 @@
 // by transposed LDS reads (each 16 lanes read 4 keys x 16 dims, and a lane gets
 // its dim of the four keys). fp32 values: 32x32x2 products, each value of S^T a
 // step, V read as it lies.
+//
+// What bounds it: at length the power the card gives. 8192 queries and keys, 32
+// over 8 bf16 heads of 128, all seen: 1.07 ms, 1028 TFLOP/s; 16381 fp16 tokens of
+// 32 heads of 80, causal: 1.51 ms, 910 (a library product of 8192^3: 1160 to
+// 1207). There the clock falls to 1.6 to 1.9 GHz, and fewer cycles (products
+// scheduled between their operands' reads and the weights) do not change the
+// time, fewer bytes do: 64 queries a wave for heads up to 64 (829 -> 882). At few
+// thousand queries it is the longest block's chain of tiles, 1.3 to 2 us each
+// (64 keys by 128 queries). Few queries over many keys: the keys are cut into
+// parts whose sums a second kernel joins (296 queries over 12000 keys 81 -> 58
+// us), or over groups of waves in a block (19 over 449 in fp32 61 -> 16).
+// fp32: 140 TFLOP/s at heads of 128 (a library product: 154).
 #include <type_traits>
 
 #include "attend.h"
@@ -121,16 +133,12 @@ __device__ __forceinline__ Where find(const PromptArgs &a, int tile) {
 // Which block does what. Blocks go over the eight XCDs in turn, and an XCD takes
 // the same heads of every tile, so that the blocks that it runs share their keys
 // in its L2 (all heads of some tiles to an XCD: 8192 queries and keys, 32 over 8
-// heads of 128, 1100 instead of 1060 us). Tiles come longest first; where two
-// blocks a CU take all there are, the second ones shortest first.
+// heads of 128, 1100 instead of 1060 us). Tiles come longest first.
 struct Order {
   int tiles, split;
 };
 __device__ __forceinline__ void block_of(const PromptArgs &a, const Order &o, int block, int &head, int &tile, int &part) {
-  const int ways = a.heads % 8 == 0 ? 8 : 1, heads = a.heads / ways;
-  const int all = o.tiles * o.split * heads, once = 256 / ways;  // blocks of an XCD, and what they are one a CU
-  int j = block / ways;
-  if (all <= 2 * once && j >= once) j = once + all - 1 - j;
+  const int ways = a.heads % 8 == 0 ? 8 : 1, heads = a.heads / ways, j = block / ways;
   head = block % ways * heads + j % heads;
   tile = j / heads / o.split;
   part = j / heads % o.split;
@@ -640,6 +648,9 @@ struct Shape {
 int64_t tiles_of(const PromptArgs &a, int qb) {  // at most: every sequence's last tile may be a part
   return a.nq / qb + std::min<int64_t>(a.sequences, a.nq);
 }
+// Two blocks of 128 queries a CU are 512. Fewer than 256 leave CUs idle: there
+// the keys are cut, into parts of 1024 at least where they are long (a join costs
+// 7 us), else over a block's waves (512 queries of 32 heads of 80: 10.7 us).
 Shape shape_of(const PromptArgs &a) {
   Shape s{4, 1, 1};
   const int64_t blocks = tiles_of(a, 128) * a.heads, keys = a.nk / std::max(1, std::min(a.sequences, a.nk));
