@@ -401,7 +401,8 @@ int tinyoai_experts_free(tinyoai_experts *e);
  * TINYOAI_BF16. A buffer's row holds its heads one after another and rows are
  * `ld` values apart (at most 2^22); a buffer starts at a multiple of its type's
  * size. Heads have a multiple of 8 values, at most 256. A call with no rows
- * (n, nq = 0) does nothing. Handles may be used by several threads at once;
+ * (n, nq = 0) does nothing. What a call writes may not overlap its other buffers
+ * but where it says so. Handles may be used by several threads at once;
  * what is still enqueued must have ended before a close. */
 
 #define TINYOAI_ROPE_HALF 0        /* value i of a head turns with i + rot / 2 */
@@ -476,7 +477,9 @@ int tinyoai_kv_pages_close(tinyoai_kv_pages *c);
  * they are. Offsets that leave [0, nq] or [0, nk] count as the nearest that do
  * not; they must not fall (rows of such sequences may be left out; nothing
  * outside `out` is touched). nq and nk are at most 2^30, and (nq / 128 +
- * sequences) * heads must stay below 2^24. */
+ * sequences) * heads must stay below 2^24. Few queries: the keys are cut into parts whose sums are joined in order, in
+ * scratch as tinyoai_weight_mul_device's, kept for each device until the process
+ * ends; the buffers and the stream must be the current device's. */
 int tinyoai_attention_device(int32_t dtype, const void *q_dev, int64_t ldq, int32_t heads, const void *k_dev, int64_t ldk,
                              const void *v_dev, int64_t ldv, int32_t kv_heads, int32_t head_dim, float scale, int32_t causal,
                              const int32_t *q_offsets_dev, const int32_t *k_offsets_dev, int32_t sequences, int32_t nq,

@@ -361,6 +361,21 @@ def test_attend_entries(hip, dev):
     c.close()
 
 
+def test_attend_full_tables(hip, dev):
+    """64 sequences that each fill the longest table (its entries all one page): 2^31 units of 32 positions, one
+    more than 31 bits count. Equal scores and small whole values, so that every sum is exact: multiples of 32
+    up to 2^30 times at most 8."""
+    hd, page, width, n = 8, 1024, 1 << 20, 64
+    c = hip.KVPages(W.BF16, 1, 1, hd, page, 1)
+    k, v = encode(W.BF16, np.zeros((page, hd)))[0], encode(W.BF16, np.tile(np.arange(1.0, 9.0), (page, 1)))[0]
+    c.write(0, W.BF16, dev.put(k), hd, dev.put(v), hd, dev.put(np.arange(page, dtype=np.int32)), page)
+    out = _empty(dev, W.F32, n, hd)
+    c.attend(0, W.F32, dev.put(np.ones((n, hd), np.float32)), hd, 1, 1.0, dev.put(np.zeros((n, width), np.int32)), width,
+             dev.put(np.full(n, 2**31 - 1, np.int32)), n, out, hd)
+    assert np.array_equal(dev.get(out, (n, hd)), np.tile(np.arange(1.0, 9.0, dtype=np.float32), (n, 1)))
+    c.close()
+
+
 # ---------------------------------------------------------------- packed prompts
 def _prompt_check(hip, dev, rng, dtype, heads, kv, hd, lengths, causal, pad=0, shift=0, spread=1.0, hidden=False):
     """Sequences of (queries, keys); two rows more than theirs in every buffer. `hidden`: values that are not finite in keys

@@ -193,15 +193,16 @@ void attend_kernel(AttendArgs a, Plan plan) {
 
   // The units of a sequence; a lane each of 64 sequences at a time.
   const int per = a.c.kv_heads * plan.qtiles;
-  int first = 0, len = 0, upto = 0;  // the window's first sequence; of the lane's: its length, the units up to its end
+  int first = 0, len = 0;  // the window's first sequence; of the lane's: its length
+  uint32_t upto = 0;       // and the units up to its end (64 of the longest: 2^31)
   auto units_of = [&](int length) { return max((length + kUnit - 1) / kUnit, 1); };  // (one to write zeros)
   auto length_of = [&](int s) { return s < a.n ? (int)min((int64_t)max(a.lengths[s], 0), most) : -1; };
   auto window = [&]() {
     len = length_of(first + lane);
-    upto = len < 0 ? 0 : units_of(len);
+    upto = len < 0 ? 0u : (uint32_t)units_of(len);
 #pragma unroll
     for (int off = 1; off < 64; off *= 2) {
-      const int x = __shfl_up(upto, off);
+      const uint32_t x = __shfl_up(upto, off);
       if (lane >= off) upto += x;
     }
   };
@@ -209,7 +210,8 @@ void attend_kernel(AttendArgs a, Plan plan) {
     return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)x));
   };
   window();
-  int64_t all_units = __builtin_amdgcn_readlane(upto, 63);
+  auto upto_of = [&](int l) { return (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)upto, l); };
+  int64_t all_units = upto_of(63);
   if (a.n > 64) {
     double sum = 0;  // (exact: below 2^53)
     for (int s = 64 + lane; s < a.n; s += 64) sum += units_of(length_of(s));
@@ -227,12 +229,11 @@ void attend_kernel(AttendArgs a, Plan plan) {
   {
     const int64_t at_units = uniform(u / per);
     int64_t before = 0;  // units before the window
-    int total;
-    while (at_units >= before + (total = __builtin_amdgcn_readlane(upto, 63))) before += total, first += 64, window();
+    while (at_units >= before + upto_of(63)) before += upto_of(63), first += 64, window();
     at = __builtin_amdgcn_readfirstlane(__builtin_ctzll(__ballot(before + upto > at_units)));
     length = __builtin_amdgcn_readlane(len, at);
     units = units_of(length);
-    const int64_t local = uniform(u - (before + __builtin_amdgcn_readlane(upto, at) - units) * per);
+    const int64_t local = uniform(u - (before + upto_of(at) - units) * per);
     pair = __builtin_amdgcn_readfirstlane((int)(local / units));
     unit = __builtin_amdgcn_readfirstlane((int)(local % units));
   }
