@@ -290,7 +290,8 @@ int tinyoai_weight_mul(tinyoai_weight *w, const float *x, int32_t n, float *out)
  * (a hipStream_t; NULL = the weight's own stream) without synchronizing.
  * Operand planes and K-split partials live in a buffer per stream that the
  * weight keeps (hipStreamPerThread: per thread; streams past eight share one
- * buffer, their calls one after another), so calls in flight on several
+ * buffer, their calls one after another, and those on hipStreamPerThread then
+ * return when their work has ended), so calls in flight on several
  * streams do not meet. A call on a capturing stream takes a buffer of its
  * capture's own, allocated then, which the graph and the executable graphs
  * made from it hold until they are destroyed; the replays of one executable

@@ -29,7 +29,7 @@ class StreamScratch {
     if (int rc = take(st, bytes, &lease)) return rc;
     hipError_t e = launch(lease.ptr);
     if (lease.shared) {  // also after a launch that failed: an earlier one of the call may run
-      const hipError_t r = hipEventRecord(shared_done_, st);
+      const hipError_t r = give_back(st);
       if (e == hipSuccess) e = r;
     }
     return e == hipSuccess ? TINYOAI_OK : hip_fail(e, "product launch");
@@ -37,9 +37,10 @@ class StreamScratch {
 
  private:
   int take(hipStream_t st, size_t bytes, ScratchPool::Lease *lease);
+  hipError_t give_back(hipStream_t st);  // the shared buffer, after what `st` holds
   std::mutex mu_;
   ScratchPool pool_;
-  hipEvent_t shared_done_ = nullptr;  // after the shared buffer's last call
+  hipEvent_t shared_done_ = nullptr;  // after the shared buffer's last call but those that were waited for
 };
 
 }  // namespace tinyoai
