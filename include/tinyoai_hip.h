@@ -309,7 +309,8 @@ int tinyoai_weight_mul_device(tinyoai_weight *w, const float *x_dev, int32_t n, 
  * the previous one left there, so the library orders them: `stream` NULL
  * runs the call on one library stream per GPU (not the weight's own
  * stream), and a caller's stream first waits for the previous call on
- * that GPU, on whatever stream it ran. Under HIP stream capture no such
+ * that GPU, on whatever stream it ran (a call on hipStreamPerThread returns
+ * when its work has ended). Under HIP stream capture no such
  * wait is recorded: captured calls that overlap on one GPU race for the
  * array. */
 int tinyoai_weight_mul_device_noalloc(tinyoai_weight *w, const float *x_dev, int32_t n, float *out_dev, void *stream);

@@ -818,6 +818,47 @@ def test_threads_share_a_buffer_in_turn():
         products.test_products_in_flight_on_many_streams(W.F16, 70)
 
 
+def test_threads_share_the_library_array_in_turn(hip, dev):
+    """No-allocation products of threads that end with their work enqueued, behind those of four streams."""
+    import threading
+    rng = np.random.default_rng(33)
+    rows, cols, sizes = 900, 1536, (70, 73, 76, 79)
+    w = hip.Weight(W.Tensor(W.F16, rows, cols, encode(W.F16, rng.standard_normal((rows, cols)))[0].reshape(-1).view(np.uint8)))
+    x = [dev.put(rng.standard_normal((sizes[-1], cols)).astype(np.float32)) for _ in range(6)]
+    y = [[_empty(dev, W.F32, m, rows) for m in sizes] for _ in x]
+    streams = [C.c_void_p() for _ in range(4)]
+    for st in streams:
+        assert dev.rt.hipStreamCreateWithFlags(C.byref(st), 1) == 0
+
+    def run(i, stream):
+        dev.rt.hipSetDevice(0)
+        for k, m in enumerate(sizes):
+            w.mul_device_noalloc(x[i], m, y[i][k], stream)
+
+    want = []
+    for i in range(6):
+        run(i, streams[0].value)
+        want.append([dev.get(y[i][k], (m, rows)) for k, m in enumerate(sizes)])
+    for _ in range(60):
+        clear = np.full((sizes[-1], rows), np.nan, np.float32)
+        for i in range(6):
+            for k, m in enumerate(sizes):
+                assert dev.rt.hipMemcpy(y[i][k], clear.ctypes.data, m * rows * 4, 1) == 0
+        for i in range(4):
+            run(i, streams[i].value)
+        threads = [threading.Thread(target=run, args=(i, 2)) for i in (4, 5)]  # hipStreamPerThread
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        for i in range(6):
+            for k, m in enumerate(sizes):
+                assert np.array_equal(dev.get(y[i][k], (m, rows)), want[i][k]), (i, m)
+    for st in streams:
+        dev.rt.hipStreamDestroy(st)
+    w.close()
+
+
 def test_refusals_of_handles(hip, dev):
     """Refusals that need an open handle; none of them reaches the device."""
     r, c = hip.Rope(64, 64), hip.KVPages(W.Q8_0, 2, 4, 64, 16, 4)

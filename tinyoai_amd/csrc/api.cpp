@@ -2581,7 +2581,13 @@ int tinyoai_weight_mul_device_noalloc(tinyoai_weight *w, const float *x_dev, int
                 sizeof(scratch));
   if (order && (e = hipStreamWaitEvent(st, d->done, 0)) != hipSuccess) return hip_fail(e, "no-allocation ordering");
   e = mx ? launch_mx_product(mp, d->ptr, st) : product_launch(p, m, x_dev, n, out_dev, d->ptr, st);
-  if (e == hipSuccess && order) e = hipEventRecord(d->done, st);
+  // (a thread's own stream: once the thread has ended, events do not wait for what it left there)
+  if (order && st == hipStreamPerThread) {
+    const hipError_t s = hipStreamSynchronize(st);
+    if (e == hipSuccess) e = s;
+  } else if (e == hipSuccess && order) {
+    e = hipEventRecord(d->done, st);
+  }
   return e == hipSuccess ? TINYOAI_OK : hip_fail(e, "product launch");
 }
 
