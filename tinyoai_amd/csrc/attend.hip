@@ -84,10 +84,15 @@ struct Plan {
   float *values;
 };
 
-// CT: the cache's type; KS: steps of 32 dims; PL: planes of the queries.
+// CT: the cache's type; KS: steps of 32 dims; PL: planes of the queries (3: fp32, 1:
+// as the matrix cores take them, 2: the other 16-bit type; fp32 caches: any type).
 template <int CT, int KS, int PL>
 struct Attend {
   static constexpr bool F32 = CT == FMT_F32, Q8 = CT == FMT_Q8_0, F16 = CT == FMT_F16;
+  // The queries' type. It is the instance's: with a branch on the argument where
+  // they are read, the compiler left their address undefined behind one of its
+  // sides, and a wave's next pairs read theirs from there.
+  static constexpr int QT = PL == 3 ? FMT_F32 : PL == 1 ? (Q8 ? FMT_BF16 : CT) : F16 ? FMT_BF16 : FMT_F16;
   static constexpr int WAVES = KS == 8 ? 2 : 4;
   static constexpr int ROWS = F32 ? 16 : 32;                // positions of a tile
   static constexpr int C = KS * (F32 ? 8 : Q8 ? 2 : 4);     // chunks of a row in LDS
@@ -278,6 +283,7 @@ void attend_kernel(AttendArgs a, Plan plan) {
   };
   Piece now, next;
   if (!next_piece(now)) return;
+  next = now;
 
   // Table entries of the piece whose loads are started: a lane each from page `wb` on.
   int wb = 0, entry = -1;
@@ -382,11 +388,7 @@ void attend_kernel(AttendArgs a, Plan plan) {
         const int d = s * 32 + g * 8;
 #pragma unroll
         for (int j = 0; j < 8; j++) v[s][j] = 0.f;
-        if (live && d < hd) {
-          if (a.dtype == FMT_F32) load8<FMT_F32>(a.q, from + d, v[s]);
-          else if (a.dtype == FMT_F16) load8<FMT_F16>(a.q, from + d, v[s]);
-          else load8<FMT_BF16>(a.q, from + d, v[s]);
-        }
+        if (live && d < hd) load8<A::QT>(a.q, from + d, v[s]);
 #pragma unroll
         for (int j = 0; j < 8; j++) big = fmaxf(big, fabsf(v[s][j]));
       }
