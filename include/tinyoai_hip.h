@@ -460,7 +460,7 @@ int tinyoai_kv_pages_read_device(tinyoai_kv_pages *c, int32_t layer, int32_t dty
  * outside [0, pages) are left out, entries past the length are not read, and
  * a sequence without positions gets zeros. The new token's own key and value are
  * written first (they count as any other). Scores, softmax and sums are fp32, of
- * the values that the cache stands for; the result is rounded once. n * heads is
+ * the values that the cache stands for (infinities too); the result is rounded once. n * heads is
  * at most 2^22. Long sequences are cut into ranges whose sums are joined in
  * order, in scratch as tinyoai_weight_mul_device's. */
 int tinyoai_kv_pages_attend_device(tinyoai_kv_pages *c, int32_t layer, int32_t dtype, const void *q_dev, int64_t ldq,

@@ -1,5 +1,5 @@
 """Rotary positions, the paged cache and the attention operators on the GPU where they may go wrong: the kernels' forms for
-large calls."""
+large calls, and values that are not finite."""
 import numpy as np
 import pytest
 
@@ -66,3 +66,99 @@ def test_attend_many_pairs(hip, dev, cache, dtype):
                 assert np.all(np.abs(got[i, g] - want) <= tol), (heads, kv, hd, i, g, x)
         c.close()
         dev.close()
+
+
+# ---------------------------------------------------------------- values that are not finite
+def _softmax_sums(q, k, v, scale, seen=None):
+    """The attention's formula in float64 with IEEE rules for infinities and NaN, of queries [m, hd]: (outputs, and of the
+    finite values alone the sums of weight times magnitude and the largest sums of scale |q| |k|)."""
+    with np.errstate(invalid="ignore", over="ignore"):
+        s = (q[:, None] * k).sum(-1) * scale
+        if seen is not None:
+            s = np.where(seen, s, -np.inf)
+        top = s.max(-1, keepdims=True)
+        p = np.exp(s - top)
+        p = p / p.sum(-1, keepdims=True)
+        terms = p[..., None] * v
+        if seen is not None:  # what is not seen has no effect, whatever it holds
+            terms = np.where(seen[..., None], terms, 0)
+        out = terms.sum(1)
+    mag = np.where(np.isfinite(terms), np.abs(terms), 0).sum(1)
+    load = np.where(np.isfinite(k), np.abs(q[:, None] * k), 0).sum(-1).max(-1, initial=0)[:, None] * abs(scale)
+    if seen is not None:
+        out[~seen.any(-1)] = 0
+    return out, mag, load
+
+
+def _same(got, want, tol):
+    """Where the formula's result is finite within the tolerance, else that result."""
+    assert np.array_equal(np.isnan(got), np.isnan(want)), (np.isnan(got).sum(), np.isnan(want).sum())
+    at = np.isfinite(want)
+    assert np.array_equal(got[~at], want[~at], equal_nan=True)
+    assert np.all(np.abs(got[at] - want[at]) <= np.broadcast_to(tol, want.shape)[at])
+
+
+def _infinite_attend(hip, dev, rng, cache, dtype, heads, kv, hd, page, lengths, spoil):
+    """New tokens over pages whose rows `spoil(i, k, v, q)` has changed, [length, kv, hd] of sequence i (q [heads, hd])."""
+    n, width = len(lengths), -(-max(lengths) // page)
+    pages, rows = n * width, n * width * page
+    table = rng.permutation(pages).astype(np.int32).reshape(n, width)
+    qb, q = encode(dtype, rng.standard_normal((n, heads * hd)))
+    k, v = (rng.standard_normal((rows, kv, hd)).astype(np.float32) for _ in range(2))
+    slots = [table[i, np.arange(x) // page] * page + np.arange(x) % page for i, x in enumerate(lengths)]
+    for i, s in enumerate(slots):
+        ks, vs = k[s], v[s]
+        spoil(i, ks, vs, q[i].reshape(heads, hd))
+        k[s], v[s] = ks, vs
+    c = hip.KVPages(cache, 1, kv, hd, page, pages)
+    c.write(0, W.F32, dev.put(k), kv * hd, dev.put(v), kv * hd, dev.put(np.arange(rows, dtype=np.int32)), rows)
+    out = _empty(dev, dtype, n, heads * hd)
+    scale = hd ** -0.5
+    c.attend(0, dtype, dev.put(qb), heads * hd, heads, scale, dev.put(table), width, dev.put(np.asarray(lengths, np.int32)), n, out,
+             heads * hd)
+    got = decode(dtype, dev.get(out, (n, heads * hd), bits_dtype(dtype))).reshape(n, heads, hd)
+    c.close()
+    with np.errstate(invalid="ignore", over="ignore"):
+        k, v = (_held(cache, x.reshape(rows, -1).astype(np.float64), hd).reshape(rows, kv, hd) for x in (k, v))
+    for i, s in enumerate(slots):
+        for h in range(heads):
+            g = h // (heads // kv)
+            want, mag, load = _softmax_sums(q[i].reshape(heads, hd)[h:h + 1], k[s, g], v[s, g], scale)
+            with np.errstate(invalid="ignore"):
+                tol = _tolerance(np.where(np.isfinite(want), want, 0), mag, load, lengths[i], hd, dtype, _weights_rounded(cache, dtype))
+            _same(got[i, h], want[0], tol[0])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cache", TYPES)
+def test_attend_infinities(hip, dev, cache, dtype):
+    """Infinities that are seen count as fp32 sums of products have them: one in the values makes its outputs infinite, both
+    signs NaN; one in the keys weighs nothing where the score falls to -inf and makes NaN where it rises to +inf."""
+    rng = np.random.default_rng(41)
+
+    def values(i, k, v, q):
+        v[rng.integers(0, len(v), 5), :, rng.integers(0, v.shape[2], 5)] = np.inf
+        v[rng.integers(0, len(v), 5), :, rng.integers(0, v.shape[2], 5)] = -np.inf
+
+    def one_value(i, k, v, q):  # its weight is exactly 1
+        v[0, :, ::3] = np.inf
+
+    def keys(i, k, v, q):  # a score of -inf for the first head of each key head
+        group = len(q) // k.shape[1]
+        for g in range(k.shape[1]):
+            for t in rng.integers(0, len(k), 3):
+                d = rng.integers(0, k.shape[2])
+                k[t, g, d] = -np.inf * np.sign(q[g * group, d])
+
+    def both(i, k, v, q):
+        if i == 0:
+            values(i, k, v, q)
+        if i == 1:
+            keys(i, k, v, q)
+
+    for heads, kv, hd, page, lengths, spoil in ((4, 2, 64, 16, (40, 3, 200), values), (4, 2, 64, 16, (1, 2), one_value),
+                                                (2, 2, 80, 8, (33, 150), values), (3, 1, 128, 64, (65, 7), keys),
+                                                (2, 2, 96, 32, (31, 100), keys), (20, 1, 40, 4, (50, 9), both),
+                                                (2, 1, 256, 16, (70, 20), both), (1, 1, 8, 1, (9, 40), values),
+                                                (4, 4, 128, 16, (3000, 2500, 1000), both), (2, 1, 64, 64, (6000, 5000), both)):
+        _infinite_attend(hip, dev, rng, cache, dtype, heads, kv, hd, page, lengths, spoil)
