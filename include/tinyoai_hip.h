@@ -475,7 +475,8 @@ int tinyoai_kv_pages_close(tinyoai_kv_pages *c);
  * chunk of a prompt behind what is cached of it), else all of them; one that
  * sees none gets zeros. Masked keys and values have no effect, whatever they
  * hold. q, k, v and out have one type; sums are fp32, and for 16-bit types the
- * softmax weights are rounded to that type. Rows outside the sequences stay as
+ * softmax weights are rounded to that type (in fp16 those below 2^-36 of the
+ * largest count as none). Rows outside the sequences stay as
  * they are. Offsets that leave [0, nq] or [0, nk] count as the nearest that do
  * not; they must not fall (rows of such sequences may be left out; nothing
  * outside `out` is touched). nq and nk are at most 2^30, and (nq / 128 +

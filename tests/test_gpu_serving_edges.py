@@ -1,10 +1,10 @@
 """Rotary positions, the paged cache and the attention operators on the GPU where they may go wrong: the kernels' forms for
-large calls, and values that are not finite."""
+large calls, values that are not finite, weights that are small."""
 import numpy as np
 import pytest
 
 from experts_fixture import EPS, Device, bits_dtype, decode, encode
-from test_gpu_serving import CACHES, TYPES, _attention, _empty, _held, _tolerance, _weights_rounded
+from test_gpu_serving import CACHES, TYPES, U, _attention, _empty, _held, _tolerance, _weights_rounded
 from tinyoai_amd import weights as W
 
 pytestmark = pytest.mark.gpu
@@ -162,3 +162,39 @@ def test_attend_infinities(hip, dev, cache, dtype):
                                                 (2, 1, 256, 16, (70, 20), both), (1, 1, 8, 1, (9, 40), values),
                                                 (4, 4, 128, 16, (3000, 2500, 1000), both), (2, 1, 64, 64, (6000, 5000), both)):
         _infinite_attend(hip, dev, rng, cache, dtype, heads, kv, hd, page, lengths, spoil)
+
+
+# ---------------------------------------------------------------- small weights
+@pytest.mark.parametrize("dtype", [W.F16, W.BF16])
+@pytest.mark.parametrize("heads,hd,nq,nk,causal", [(1, 64, 1, 131072, False), (1, 128, 1, 1 << 20, False), (2, 80, 130, 20000, True),
+                                                   (1, 64, 19, 1500, False), (2, 96, 50, 1500, True), (16, 128, 2048, 2048, True),
+                                                   (64, 64, 2048, 2048, True), (8, 256, 4096, 4096, False)])
+def test_prompt_small_weights(hip, dev, dtype, heads, hd, nq, nk, causal):
+    """One key far above all others, whose weights count together: 17.4 nats below it each, or spread over 25 nats."""
+    rng = np.random.default_rng(51)
+    for scores in (np.full(nk, -17.4), -25 * rng.random(nk)):
+        scores[0] = 0  # (the causal queries all see it)
+        k = np.zeros((nk, hd))
+        k[:, 0] = scores
+        v = rng.random((nk, hd))
+        v[0, ::2] = 0
+        kb, k = encode(dtype, k)
+        vb, v = encode(dtype, v)
+        q = np.zeros((nq, heads, hd), np.float32)
+        q[..., 0] = 1
+        qb = encode(dtype, q.reshape(nq, -1))[0]
+        out = _empty(dev, dtype, nq, heads * hd)
+        hip.attention(dtype, dev.put(qb), heads * hd, heads, dev.put(kb), hd, dev.put(vb), hd, 1, hd, 1.0, causal,
+                      dev.put(np.array([0, nq], np.int32)), dev.put(np.array([0, nk], np.int32)), 1, nq, nk, out, heads * hd)
+        got = decode(dtype, dev.get(out, (nq, heads * hd), bits_dtype(dtype))).reshape(nq, heads, hd)
+        p = np.exp(k[:, 0])
+        last = np.arange(nq) + nk - nq if causal else np.full(nq, nk - 1)
+        top, total, keys = np.cumsum(p[:, None] * v, 0)[last], np.cumsum(p)[last][:, None], last[:, None] + 1
+        want = top / total
+        # a weight, of at most 1, rounds by half a step (and its score by 25 U, its power by 2 U); fp16's are multiples of
+        # 2^-35 of the largest at least, and then off by 2^-36 each; the sums have chains of keys / 4 terms
+        tiny = keys * (2.0 ** -36 if dtype == W.F16 else 0)
+        off = EPS[dtype] + 30 * U + 2 * (keys / 4 + 64) * U
+        tol = 1.01 * (2 * off * want + (1 + want) * tiny / total) + EPS[dtype] * want + (2.0 ** -25 if dtype == W.F16 else 0)
+        assert np.all(np.abs(got - want[:, None]) <= tol[:, None]), (np.abs(got - want[:, None]) / tol[:, None]).max()
+        dev.close()

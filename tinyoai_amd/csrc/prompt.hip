@@ -193,7 +193,12 @@ void prompt_kernel(PromptArgs a, Parts parts) {
   using Value = typename P::Value;
   constexpr bool F32 = P::F32;
   constexpr int V = P::V, C = P::C, DT = P::DT, PLANE = P::PLANE, QS = P::QS, HALVES = KEYS / 32;
-  constexpr float kLeap = 8.f;            // the reference moves only when a score exceeds it by 2^8
+  // The reference moves only when a score exceeds it by kLeap (in powers of two).
+  // Weights lie higher by 2^kLift: in fp16 the largest is 2^15, and those below
+  // 2^-36 of it (24.9 nats), the half of its smallest, vanish. Without that, 131071
+  // keys 17.4 nats below one lost all of their 0.36%. The lift cancels in the division.
+  constexpr bool HALF = D == FMT_F16;
+  constexpr float kLeap = HALF ? 4.f : 8.f, kLift = HALF ? 11.f : 0.f;
   __shared__ __align__(16) uint4 lds[P::LDS];
   uint16_t *ones = reinterpret_cast<uint16_t *>(lds + P::TILES - P::SPAN);  // 1, 0, 0, 0; 0, 0, 0, 0
   if (P::ONES && threadIdx.x < 8) ones[threadIdx.x] = threadIdx.x ? 0 : D == FMT_F16 ? 0x3c00 : 0x3f80;
@@ -435,7 +440,7 @@ void prompt_kernel(PromptArgs a, Parts parts) {
       }
       float base[QN];
 #pragma unroll
-      for (int n = 0; n < QN; n++) base[n] = ref[n] == -INFINITY ? 0.f : -ref[n];
+      for (int n = 0; n < QN; n++) base[n] = ref[n] == -INFINITY ? 0.f : kLift - ref[n];
       if constexpr (F32) {
 #pragma unroll
         for (int h = 0; h < HALVES; h++)
