@@ -289,9 +289,9 @@ int tinyoai_weight_mul(tinyoai_weight *w, const float *x, int32_t n, float *out)
 /* The same product on device-resident buffers, enqueued on `stream`
  * (a hipStream_t; NULL = the weight's own stream) without synchronizing.
  * Operand planes and K-split partials live in a buffer per stream that the
- * weight keeps (hipStreamPerThread: per thread; streams past eight share one
- * buffer, their calls one after another, and those on hipStreamPerThread then
- * return when their work has ended), so calls in flight on several
+ * weight keeps (hipStreamPerThread: per thread, and a thread that made such
+ * calls ends when its work there has ended; streams past eight share one
+ * buffer, their calls one after another), so calls in flight on several
  * streams do not meet. A call on a capturing stream takes a buffer of its
  * capture's own, allocated then, which the graph and the executable graphs
  * made from it hold until they are destroyed; the replays of one executable
@@ -309,8 +309,8 @@ int tinyoai_weight_mul_device(tinyoai_weight *w, const float *x_dev, int32_t n, 
  * the previous one left there, so the library orders them: `stream` NULL
  * runs the call on one library stream per GPU (not the weight's own
  * stream), and a caller's stream first waits for the previous call on
- * that GPU, on whatever stream it ran (a call on hipStreamPerThread returns
- * when its work has ended). Under HIP stream capture no such
+ * that GPU, on whatever stream it ran (a thread that made calls on
+ * hipStreamPerThread ends when its work there has ended). Under HIP stream capture no such
  * wait is recorded: captured calls that overlap on one GPU race for the
  * array. */
 int tinyoai_weight_mul_device_noalloc(tinyoai_weight *w, const float *x_dev, int32_t n, float *out_dev, void *stream);

@@ -2549,7 +2549,7 @@ int scratch_device(ScratchDev **out) {
 
 extern "C" {
 
-int tinyoai_weight_mul_device_noalloc(tinyoai_weight *w, const float *x_dev, int32_t n, float *out_dev, void *stream) {
+int tinyoai_weight_mul_device_noalloc(tinyoai_weight *w, const float *x_dev, int32_t n, float *out_dev, void *stream) try {
   if (!w || !x_dev || !out_dev || n <= 0) return fail(TINYOAI_EINVAL, "invalid product arguments");
   const Matrix &m = w->m.desc;
   const int cols = (int)w->cols();
@@ -2579,16 +2579,16 @@ int tinyoai_weight_mul_device_noalloc(tinyoai_weight *w, const float *x_dev, int
   if ((mx ? mx_scratch(mp) : p.bytes()) > sizeof(scratch))
     return fail(TINYOAI_EINVAL, "product of %d x %d needs more than the no-allocation limit of %zu bytes", n, cols,
                 sizeof(scratch));
+  if (order && st == hipStreamPerThread) (void)thread_stream(dev);
   if (order && (e = hipStreamWaitEvent(st, d->done, 0)) != hipSuccess) return hip_fail(e, "no-allocation ordering");
   e = mx ? launch_mx_product(mp, d->ptr, st) : product_launch(p, m, x_dev, n, out_dev, d->ptr, st);
-  // (a thread's own stream: once the thread has ended, events do not wait for what it left there)
-  if (order && st == hipStreamPerThread) {
-    const hipError_t s = hipStreamSynchronize(st);
-    if (e == hipSuccess) e = s;
-  } else if (e == hipSuccess && order) {
-    e = hipEventRecord(d->done, st);
+  if (order) {  // also after a launch that failed: an earlier one of the call may run
+    const hipError_t r = hipEventRecord(d->done, st);
+    if (e == hipSuccess) e = r;
   }
   return e == hipSuccess ? TINYOAI_OK : hip_fail(e, "product launch");
+} catch (const std::exception &e) {
+  return fail(TINYOAI_ENOMEM, "product: %s", e.what());
 }
 
 int tinyoai_weight_mul(tinyoai_weight *w, const float *x, int32_t n, float *out) {

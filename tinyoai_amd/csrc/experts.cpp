@@ -35,13 +35,35 @@ struct RelaxedCapture {
     if (set) hipThreadExchangeStreamCaptureMode(&mode);
   }
 };
-// This thread's number, no other's before or after.
-uint64_t thread_number() {
-  static std::atomic<uint64_t> next{1};
-  thread_local const uint64_t number = next++;
-  return number;
-}
+class ThreadEnd {
+ public:
+  ThreadStream add(int device) {
+    if (!life_) life_ = std::make_shared<char>(0);
+    if (std::find(devices_.begin(), devices_.end(), device) == devices_.end()) devices_.push_back(device);
+    return ThreadStream{number_, life_};
+  }
+  ~ThreadEnd() {
+    RelaxedCapture relaxed;
+    for (int device : devices_)
+      if (hipSetDevice(device) == hipSuccess) (void)hipStreamSynchronize(hipStreamPerThread);
+  }
+
+ private:
+  static uint64_t next() {
+    static std::atomic<uint64_t> n{1};
+    return n++;
+  }
+  std::shared_ptr<char> life_;  // (released last)
+  std::vector<int> devices_;
+  const uint64_t number_ = next();
+};
 }  // namespace
+
+// (made behind the thread's first call of the runtime, so it ends before the runtime's own record of the thread)
+ThreadStream thread_stream(int device) {
+  thread_local ThreadEnd end;
+  return end.add(device);
+}
 
 StreamScratch::~StreamScratch() {
   pool_.clear([](void *p) { hipFree(p); });
@@ -79,7 +101,13 @@ int StreamScratch::take(hipStream_t st, size_t bytes, ScratchPool::Lease *lease)
       }
     }
   } else {
-    *lease = pool_.eager(st, st == hipStreamPerThread ? thread_number() : 0, bytes, alloc);
+    uint64_t thread = 0;
+    if (st == hipStreamPerThread) {
+      int device = 0;
+      if ((e = hipGetDevice(&device)) != hipSuccess) return hip_fail(e, "hipGetDevice");
+      thread = thread_stream(device).number;
+    }
+    *lease = pool_.eager(st, thread, bytes, alloc);
   }
   if (!lease->ptr) return fail(TINYOAI_ENOMEM, "product scratch of %zu bytes", bytes);
   if (lease->shared) {
@@ -93,13 +121,9 @@ int StreamScratch::take(hipStream_t st, size_t bytes, ScratchPool::Lease *lease)
   return TINYOAI_OK;
 }
 
-// Calls on hipStreamPerThread are waited for: once a thread has ended, neither an
-// event recorded on its stream nor a device synchronization waits for what it
-// left there (two threads that enqueued four products each and ended: wrong
-// sums in 3 of 300 runs, with no error).
 hipError_t StreamScratch::give_back(hipStream_t st) {
   RelaxedCapture relaxed;
-  return st == hipStreamPerThread ? hipStreamSynchronize(st) : hipEventRecord(shared_done_, st);
+  return hipEventRecord(shared_done_, st);
 }
 
 // ---------------------------------------------------------------- matrices
