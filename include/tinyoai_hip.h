@@ -290,7 +290,8 @@ int tinyoai_weight_mul(tinyoai_weight *w, const float *x, int32_t n, float *out)
  * (a hipStream_t; NULL = the weight's own stream) without synchronizing.
  * Operand planes and K-split partials live in a buffer per stream that the
  * weight keeps (hipStreamPerThread: per thread, and a thread that made such
- * calls ends when its work there has ended; streams past eight share one
+ * calls ends when its work there has ended, its buffer free for another stream;
+ * streams past eight, also ones that a program has destroyed, share one
  * buffer, their calls one after another), so calls in flight on several
  * streams do not meet. A call on a capturing stream takes a buffer of its
  * capture's own, allocated then, which the graph and the executable graphs

@@ -101,13 +101,13 @@ int StreamScratch::take(hipStream_t st, size_t bytes, ScratchPool::Lease *lease)
       }
     }
   } else {
-    uint64_t thread = 0;
+    ThreadStream thread{};
     if (st == hipStreamPerThread) {
       int device = 0;
       if ((e = hipGetDevice(&device)) != hipSuccess) return hip_fail(e, "hipGetDevice");
-      thread = thread_stream(device).number;
+      thread = thread_stream(device);
     }
-    *lease = pool_.eager(st, thread, bytes, alloc);
+    *lease = pool_.eager(st, thread.number, bytes, alloc, thread.number ? &thread.life : nullptr);
   }
   if (!lease->ptr) return fail(TINYOAI_ENOMEM, "product scratch of %zu bytes", bytes);
   if (lease->shared) {

@@ -3,11 +3,13 @@
 // code; the caller brings the allocation.
 #pragma once
 
+#include <algorithm>
 #include <atomic>
 #include <cstddef>
 #include <cstdint>
 #include <functional>
 #include <map>
+#include <memory>
 #include <utility>
 #include <vector>
 
@@ -44,12 +46,27 @@ class ScratchPool {
   // each thread, on thread `thread`'s), which runs in order there. A buffer
   // that has become too small is kept: enqueued work may still use it (each
   // is at least half as large again, so all of them are no more than three
-  // times the last).
-  Lease eager(const void *stream, uint64_t thread, size_t bytes, const Alloc &alloc) {
+  // times the last). `life`, of a thread, ends when its stream is idle for good:
+  // the buffer then goes to the next stream that has none.
+  Lease eager(const void *stream, uint64_t thread, size_t bytes, const Alloc &alloc,
+              const std::weak_ptr<const void> *life = nullptr) {
     auto it = streams_.find({stream, thread});
+    if (it == streams_.end()) {
+      const auto ended = std::find_if(streams_.begin(), streams_.end(),
+                                      [](const auto &s) { return s.second.of_thread && s.second.life.expired(); });
+      if (ended != streams_.end()) {
+        auto node = streams_.extract(ended);
+        node.key() = Key{stream, thread};
+        it = streams_.insert(std::move(node)).position;
+      }
+    }
     const bool shared = it == streams_.end() && streams_.size() >= kStreams;
     if (it == streams_.end() && !shared) it = streams_.emplace(Key{stream, thread}, Buffer{}).first;
     Buffer &b = shared ? shared_ : it->second;
+    if (!shared) {
+      b.of_thread = life != nullptr;
+      if (life) b.life = *life;
+    }
     if (b.bytes < bytes) {
       size_t want = bytes > b.bytes + b.bytes / 2 ? bytes : b.bytes + b.bytes / 2;
       kept_.reserve(kept_.size() + 1);
@@ -57,7 +74,8 @@ class ScratchPool {
       if (!p && want > bytes) p = alloc(want = bytes);
       if (!p) return Lease{};
       if (b.ptr) kept_.push_back(b.ptr);
-      b = Buffer{p, want};
+      b.ptr = p;
+      b.bytes = want;
     }
     return Lease{b.ptr, shared};
   }
@@ -115,6 +133,8 @@ class ScratchPool {
   struct Buffer {
     void *ptr = nullptr;
     size_t bytes = 0;
+    bool of_thread = false;
+    std::weak_ptr<const void> life;  // (of_thread)
   };
   struct Capture {
     uint64_t id;
