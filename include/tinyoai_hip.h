@@ -404,7 +404,8 @@ int tinyoai_experts_free(tinyoai_experts *e);
  * TINYOAI_BF16. A buffer's row holds its heads one after another and rows are
  * `ld` values apart (at most 2^22); a buffer starts at a multiple of its type's
  * size. Heads have a multiple of 8 values, at most 256. A call with no rows
- * (n, nq = 0) does nothing. What a call writes may not overlap its other buffers
+ * (n, nq = 0) does nothing; buffers of no rows (a call's then, K and V where
+ * nk = 0) may be NULL. What a call writes may not overlap its other buffers
  * but where it says so. Handles may be used by several threads at once;
  * what is still enqueued must have ended before a close. */
 

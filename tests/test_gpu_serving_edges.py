@@ -1,5 +1,5 @@
 """Rotary positions, the paged cache and the attention operators on the GPU where they may go wrong: the kernels' forms for
-large calls, values that are not finite, weights that are small."""
+large calls, values that are not finite, weights that are small, no rows."""
 import numpy as np
 import pytest
 
@@ -198,3 +198,24 @@ def test_prompt_small_weights(hip, dev, dtype, heads, hd, nq, nk, causal):
         tol = 1.01 * (2 * off * want + (1 + want) * tiny / total) + EPS[dtype] * want + (2.0 ** -25 if dtype == W.F16 else 0)
         assert np.all(np.abs(got - want[:, None]) <= tol[:, None]), (np.abs(got - want[:, None]) / tol[:, None]).max()
         dev.close()
+
+
+# ---------------------------------------------------------------- empty buffers
+def test_calls_of_nothing(hip, dev):
+    """Empty arrays have no address: calls without rows do nothing, and queries over no keys give zeros."""
+    r, c = hip.Rope(64, 64), hip.KVPages(W.F16, 1, 4, 64, 16, 4)
+    r.rotate(W.F32, 0, 256, 0, 4, 0, W.F32, 0, 256)
+    r.rotate(W.F32, 0, 256, 0, 4, 0, W.F16, 0, 256)
+    for call in (c.write, c.read):
+        call(0, W.F32, 0, 256, 0, 256, 0, 0)
+    c.attend(0, W.F32, 0, 256, 4, 0.125, 0, 0, 0, 0, 0, 256)
+    for dtype in TYPES:
+        for nq in (1, 50, 700):
+            q = dev.put(np.ones((nq, 256), bits_dtype(dtype)))
+            qo, ko = dev.put(np.array([0, nq // 2, nq], np.int32)), dev.put(np.zeros(3, np.int32))
+            for causal in (True, False):
+                out = _empty(dev, dtype, nq, 256)
+                hip.attention(dtype, q, 256, 4, 0, 256, 0, 256, 4, 64, 0.125, causal, qo, ko, 2, nq, 0, out, 256)
+                assert not dev.get(out, (nq, 256), bits_dtype(dtype)).any()
+    r.close()
+    c.close()

@@ -80,3 +80,19 @@ def test_attention_refusals():
     _refused("exceed", call, nq=1 << 30)
     _refused("exceed", call, nq=1 << 21, sequences=1 << 21)
     call(nq=0)  # nothing to do
+
+
+def test_attention_of_nothing():
+    """No queries: nothing to do, whatever is empty with them. Refusals stay."""
+    def call(q=None, k=None, v=None, qo=None, ko=None, sequences=0, nq=0, nk=0, out=None):
+        hip.attention(W.F16, q, 512, 8, k, 256, v, 256, 4, 64, 0.125, True, qo, ko, sequences, nq, nk, out, 512)
+
+    call()
+    call(nk=5)
+    call(sequences=3, qo=A, ko=A)
+    _refused("invalid offsets", call, sequences=-1)
+    _refused("invalid offsets", call, nk=-1)
+    _refused("q is null", call, nq=1, qo=A, ko=A, sequences=1)
+    _refused("out is null", call, nq=1, qo=A, ko=A, sequences=1, q=A)
+    _refused("k is null", call, nq=1, nk=1, qo=A, ko=A, sequences=1, q=A, out=A)
+    _refused("v is null", call, nq=1, nk=1, qo=A, ko=A, sequences=1, q=A, out=A, k=A)

@@ -42,10 +42,10 @@ namespace {
 
 bool plain_type(int32_t dtype) { return dtype == FMT_F32 || dtype == FMT_F16 || dtype == FMT_BF16; }
 
-// Rows of `heads` heads of a buffer, ld values apart.
-int check_heads(const char *what, int32_t dtype, const void *p, int64_t ld, int32_t heads, int32_t hd) {
+// `rows` rows of `heads` heads of a buffer (of none: null, as empty arrays are), ld values apart.
+int check_heads(const char *what, int32_t dtype, const void *p, int64_t ld, int32_t heads, int32_t hd, int32_t rows) {
   if (!plain_type(dtype)) return fail(TINYOAI_EINVAL, "unsupported %s type %d", what, dtype);
-  if (!p) return fail(TINYOAI_EINVAL, "%s is null", what);
+  if (!p && rows) return fail(TINYOAI_EINVAL, "%s is null", what);
   if (ld < (int64_t)heads * hd)
     return fail(TINYOAI_EINVAL, "%s rows of %d heads of %d are %lld apart", what, heads, hd, (long long)ld);
   if (ld > kRowValues) return fail(TINYOAI_EINVAL, "%s rows are %lld apart, more than %lld", what, (long long)ld, (long long)kRowValues);
@@ -113,9 +113,9 @@ int check_layer(const tinyoai_kv_pages *c, int32_t layer) {
 int kv_rows(tinyoai_kv_pages *c, int32_t layer, int32_t dtype, const void *k, int64_t ldk, const void *v, int64_t ldv,
             const int32_t *slots, int32_t n, void *stream, hipError_t (*launch)(const KVRowsArgs &, hipStream_t)) {
   if (!c) return fail(TINYOAI_EINVAL, "the paged cache is closed");
-  if (int rc = check_heads("k", dtype, k, ldk, c->d.kv_heads, c->d.hd)) return rc;
-  if (int rc = check_heads("v", dtype, v, ldv, c->d.kv_heads, c->d.hd)) return rc;
-  if (!slots || n < 0) return fail(TINYOAI_EINVAL, "invalid slots of %d rows", n);
+  if (int rc = check_heads("k", dtype, k, ldk, c->d.kv_heads, c->d.hd, n)) return rc;
+  if (int rc = check_heads("v", dtype, v, ldv, c->d.kv_heads, c->d.hd, n)) return rc;
+  if ((!slots && n) || n < 0) return fail(TINYOAI_EINVAL, "invalid slots of %d rows", n);
   if (int rc = check_layer(c, layer)) return rc;
   if (!n) return TINYOAI_OK;
   const KVRowsArgs a{layer_pages(*c, layer), dtype, const_cast<void *>(k), const_cast<void *>(v), ldk, ldv, slots, n};
@@ -173,10 +173,10 @@ int tinyoai_rope_device(tinyoai_rope *r, int32_t dtype, const void *x_dev, int64
   if (!r) return fail(TINYOAI_EINVAL, "the rotary positions are closed");
   if (n < 0 || heads <= 0 || (int64_t)heads * r->hd > kRowValues)
     return fail(TINYOAI_EINVAL, "invalid rotation of %d rows of %d heads", n, heads);
-  if (int rc = check_heads("x", dtype, x_dev, ldx, heads, r->hd)) return rc;
-  if (int rc = check_heads("out", out_dtype, out_dev, ldo, heads, r->hd)) return rc;
-  if (!positions_dev) return fail(TINYOAI_EINVAL, "positions are null");
-  if (x_dev == out_dev && (dtype != out_dtype || ldx != ldo))
+  if (int rc = check_heads("x", dtype, x_dev, ldx, heads, r->hd, n)) return rc;
+  if (int rc = check_heads("out", out_dtype, out_dev, ldo, heads, r->hd, n)) return rc;
+  if (!positions_dev && n) return fail(TINYOAI_EINVAL, "positions are null");
+  if (n && x_dev == out_dev && (dtype != out_dtype || ldx != ldo))
     return fail(TINYOAI_EINVAL, "rows turned in place keep their type and distance");
   if (int rc = check_device(r->device, "rotary positions")) return rc;
   if (!n) return TINYOAI_OK;
@@ -253,10 +253,10 @@ int tinyoai_kv_pages_attend_device(tinyoai_kv_pages *c, int32_t layer, int32_t d
   if (!c) return fail(TINYOAI_EINVAL, "the paged cache is closed");
   if (heads <= 0 || heads % c->d.kv_heads || (int64_t)heads * c->d.hd > kRowValues)
     return fail(TINYOAI_EINVAL, "%d query heads over %d key heads", heads, c->d.kv_heads);
-  if (int rc = check_heads("q", dtype, q_dev, ldq, heads, c->d.hd)) return rc;
-  if (int rc = check_heads("out", dtype, out_dev, ldo, heads, c->d.hd)) return rc;
+  if (int rc = check_heads("q", dtype, q_dev, ldq, heads, c->d.hd, n)) return rc;
+  if (int rc = check_heads("out", dtype, out_dev, ldo, heads, c->d.hd, n)) return rc;
   if (!std::isfinite(scale)) return fail(TINYOAI_EINVAL, "invalid scale %g", scale);
-  if (!table_dev || !lengths_dev || n < 0 || width <= 0 || ((int64_t)width << c->d.page_log2) > kPositions)
+  if (n < 0 || width < 0 || ((!table_dev || !lengths_dev || !width) && n) || ((int64_t)width << c->d.page_log2) > kPositions)
     return fail(TINYOAI_EINVAL, "invalid page table of %d rows of %d", n, width);
   if ((int64_t)n * heads > kAttendRows) return fail(TINYOAI_EINVAL, "%d rows of %d heads exceed what one call takes", n, heads);
   if (int rc = check_layer(c, layer)) return rc;
@@ -283,12 +283,12 @@ int tinyoai_attention_device(int32_t dtype, const void *q_dev, int64_t ldq, int3
   if (!head_width(head_dim)) return fail(TINYOAI_EINVAL, "unsupported head width %d", head_dim);
   if (kv_heads <= 0 || heads <= 0 || heads % kv_heads || (int64_t)heads * head_dim > kRowValues)
     return fail(TINYOAI_EINVAL, "%d query heads over %d key heads", heads, kv_heads);
-  if (int rc = check_heads("q", dtype, q_dev, ldq, heads, head_dim)) return rc;
-  if (int rc = check_heads("k", dtype, k_dev, ldk, kv_heads, head_dim)) return rc;
-  if (int rc = check_heads("v", dtype, v_dev, ldv, kv_heads, head_dim)) return rc;
-  if (int rc = check_heads("out", dtype, out_dev, ldo, heads, head_dim)) return rc;
+  if (int rc = check_heads("q", dtype, q_dev, ldq, heads, head_dim, nq)) return rc;
+  if (int rc = check_heads("k", dtype, k_dev, ldk, kv_heads, head_dim, nq ? nk : 0)) return rc;
+  if (int rc = check_heads("v", dtype, v_dev, ldv, kv_heads, head_dim, nq ? nk : 0)) return rc;
+  if (int rc = check_heads("out", dtype, out_dev, ldo, heads, head_dim, nq)) return rc;
   if (!std::isfinite(scale)) return fail(TINYOAI_EINVAL, "invalid scale %g", scale);
-  if (!q_offsets_dev || !k_offsets_dev || sequences <= 0 || nq < 0 || nk < 0 || nq > kPositions || nk > kPositions)
+  if (((!q_offsets_dev || !k_offsets_dev || !sequences) && nq) || sequences < 0 || nq < 0 || nk < 0 || nq > kPositions || nk > kPositions)
     return fail(TINYOAI_EINVAL, "invalid offsets of %d sequences of %d queries and %d keys", sequences, nq, nk);
   if (((int64_t)nq / 128 + std::min(sequences, nq)) * heads >= 1 << 24)
     return fail(TINYOAI_EINVAL, "%d queries of %d sequences by %d heads exceed what one call takes", nq, sequences, heads);
