@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 from experts_fixture import EPS, Device, bits_dtype, decode, encode
-from test_gpu_serving import CACHES, TYPES, U, _attention, _empty, _held, _tolerance, _weights_rounded
+from test_gpu_serving import CACHES, TYPES, U, _attention, _empty, _encoded, _held, _rope_check, _rows, _take, _tolerance, _weights_rounded
 from tinyoai_amd import weights as W
 
 pytestmark = pytest.mark.gpu
@@ -219,3 +219,157 @@ def test_calls_of_nothing(hip, dev):
                 assert not dev.get(out, (nq, 256), bits_dtype(dtype)).any()
     r.close()
     c.close()
+
+
+# ---------------------------------------------------------------- prompts of ordinary size
+def _form(dtype, heads, hd, nq, nk, sequences):
+    """(groups of 32 queries of a block, groups of keys, parts of the keys, sets of queries a wave) as launch_prompt chooses."""
+    def tiles(queries):
+        return nq // queries + min(sequences, nq)
+
+    blocks, keys = tiles(128) * heads, nk // max(1, min(sequences, nk))
+    sets = 2 if dtype != W.F32 and hd <= 64 and tiles(256) * heads >= 512 else 1
+    if blocks >= 256:
+        return 4, 1, 1, sets
+    if dtype == W.F32:
+        groups = 2 if hd > 128 else 4
+        return 1, groups, max(1, min(512 // (tiles(32) * heads), -(-keys // (32 * groups)))), 1
+    if keys >= 2048:
+        return 4, 1, max(1, min(512 // blocks, keys // 1024)), sets
+    return (1, 4, 1, 1) if nq <= 32 else (2, 4, 1, 1) if hd <= 128 else (4, 1, 1, sets)
+
+
+def _prompt_rows(hip, dev, rng, dtype, heads, kv, hd, lengths, causal, pad=0, shift=0, hidden=False, spread=1.0):
+    """Sequences of (queries, keys), checked at rows around the tiles' borders and some others, of three heads."""
+    nq, nk = (sum(x[i] for x in lengths) + 2 for i in range(2))
+    (pq, ldq, q), (pk, ldk, k), (pv, ldv, v) = (_rows(rng, dev, dtype, m, h * hd, pad, shift, spread) for m, h in ((nq, heads), (nk, kv), (nk, kv)))
+    if hidden:
+        for p, x in ((pk, k), (pv, v)):
+            raw = dev.get(p, (nk, kv * hd + pad), bits_dtype(dtype)).copy()
+            x[-2:] = np.nan
+            at = 0
+            for m, keys in lengths:
+                if keys > 3:
+                    x[at + keys - 1, ::3] = np.nan
+                    x[at + keys - 2, 1::3] = np.inf
+                    x[at + keys // 2, 2::7] = -np.inf
+                at += keys
+            raw[:, :kv * hd] = _encoded(dtype, x)[0]
+            dev.fill(p, raw)
+    qo, ko = (np.cumsum([0] + [x[i] for x in lengths]).astype(np.int32) for i in range(2))
+    out = _empty(dev, dtype, nq, heads * hd, pad, shift)
+    scale = hd ** -0.5
+    hip.attention(dtype, pq, ldq, heads, pk, ldk, pv, ldv, kv, hd, scale, causal, dev.put(qo), dev.put(ko), len(lengths), nq, nk, out, ldq)
+    raw = _take(dev, out, dtype, nq, heads * hd, pad)
+    assert (raw[-2:] == 7).all()
+    got = decode(dtype, raw).reshape(nq, heads, hd)
+    for (m, keys), q0, k0 in zip(lengths, qo, ko):
+        if not m:
+            continue
+        rows = np.concatenate([np.arange(0, m, 32), np.arange(31, m, 32), [m - 1], rng.integers(0, m, 12)])
+        rows = np.unique(np.concatenate([rng.permutation(rows)[:30], [0, m - 1, max(m - keys, 0), max(m - keys - 1, 0)]]))
+        rows = rows[rows < m]
+        seen = np.arange(keys) <= rows[:, None] + keys - m if causal else np.ones((len(rows), keys), bool)
+        for h in {0, heads - 1, int(rng.integers(0, heads))}:
+            g = slice(h // (heads // kv) * hd, h // (heads // kv) * hd + hd)
+            qs, ks, vs = q[q0 + rows, h * hd:h * hd + hd], k[k0:k0 + keys, g], v[k0:k0 + keys, g]
+            bad_k, bad_v = ~np.isfinite(ks).all(-1), ~np.isfinite(vs)
+            want, mag, load = _attention(qs, np.where(np.isfinite(ks), ks, 0), np.where(bad_v, 0, vs), scale, seen)
+            fine = ~((seen @ bad_k.astype(float))[:, None] + seen @ bad_v.astype(float) > 0)
+            with np.errstate(invalid="ignore"):  # (a score of -inf is a weight of zero: such a key need not show)
+                zero = (seen & (qs @ ks.T == -np.inf)).any(-1) if bad_k.any() else np.zeros(len(rows), bool)
+            part = got[q0 + rows, h]
+            assert not np.isfinite(part[~fine & ~zero[:, None]]).any()
+            tol = _tolerance(want, mag, load, keys, hd, dtype, 0 if dtype == W.F32 else EPS[dtype])
+            assert np.all((np.abs(part - want) <= tol) | ~fine), (m, keys, h)
+            if causal and m > keys:
+                assert not part[rows < m - keys].any()
+
+
+LARGE = ((1500, 1500), (37, 37), (1, 700), (0, 5), (2000, 2000), (700, 500), (300, 1500), (260, 0))
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dtype,heads,kv,hd,sets", [(t, h, kv, hd, sets) for t, shapes in (
+    (W.F16, ((32, 8, 64, 2), (32, 32, 8, 2), (32, 1, 40, 2), (8, 2, 64, 1), (8, 8, 80, 1), (8, 4, 96, 1), (8, 2, 128, 1), (8, 1, 256, 1), (8, 2, 72, 1))),
+    (W.BF16, ((32, 8, 64, 2), (32, 4, 24, 2), (32, 2, 40, 2), (8, 2, 32, 1), (8, 8, 80, 1), (8, 4, 96, 1), (8, 2, 128, 1), (8, 1, 200, 1))),
+    (W.F32, ((8, 2, 8, 1), (8, 1, 64, 1), (8, 8, 80, 1), (8, 2, 96, 1), (8, 2, 128, 1), (8, 4, 256, 1), (8, 4, 160, 1)))) for h, kv, hd, sets in shapes])
+def test_prompt_large(hip, dev, dtype, heads, kv, hd, sets, causal):
+    """Blocks of 128 or 256 queries that see all of their keys: ragged sequences, more queries than keys and none, rows at
+    16-byte distances and at odd ones, values that are not finite in what some do not see."""
+    rng = np.random.default_rng(71)
+    nq, nk = (sum(x[i] for x in LARGE) + 2 for i in range(2))
+    assert _form(dtype, heads, hd, nq, nk, len(LARGE)) == (4, 1, 1, sets)
+    odd = dict(pad=3, shift=2 if dtype != W.F32 else 4)
+    _prompt_rows(hip, dev, rng, dtype, heads, kv, hd, LARGE, causal)
+    dev.close()
+    _prompt_rows(hip, dev, rng, dtype, heads, kv, hd, LARGE, causal, **odd, hidden=causal)
+    dev.close()
+    if causal:
+        _prompt_rows(hip, dev, rng, dtype, heads, kv, hd, LARGE, True, hidden=True, spread=2.0)
+        dev.close()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_prompt_small_forms(hip, dev, dtype):
+    """The forms of few queries at the widths that other tests leave out."""
+    rng = np.random.default_rng(72)
+    for heads, kv, hd, lengths, form in ((2, 1, 96, ((20, 300),), (1, 4, 1, 1)), (2, 1, 96, ((90, 300),), (2, 4, 1, 1)),
+                                         (1, 1, 96, ((90, 5000),), (4, 1, 4, 1)), (1, 1, 32, ((130, 9000),), (4, 1, 8, 1)),
+                                         (2, 2, 160, ((100, 300),), (4, 1, 1, 1)), (2, 2, 256, ((9, 700),), (1, 4, 1, 1)),
+                                         (3, 1, 40, ((70, 1100), (5, 9)), (2, 4, 1, 1))):
+        nq, nk = (sum(x[i] for x in lengths) + 2 for i in range(2))
+        assert dtype == W.F32 or _form(dtype, heads, hd, nq, nk, len(lengths)) == form
+        for causal in (True, False):
+            _prompt_rows(hip, dev, rng, dtype, heads, kv, hd, lengths, causal)
+            _prompt_rows(hip, dev, rng, dtype, heads, kv, hd, lengths, causal, pad=1, shift=4, hidden=causal)
+        dev.close()
+
+
+# ---------------------------------------------------------------- many rows
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("dtype,odtype", [(W.F32, W.F32), (W.BF16, W.BF16), (W.F16, W.F32)])
+def test_rope_many_rows(hip, dev, dtype, odtype, layout):
+    """Blocks of several rows, the last of fewer, few heads and many, also in place."""
+    rng = np.random.default_rng(81)
+    for n, heads, hd, rot, pad, shift in ((2047, 3, 64, 64, 0, 0), (2048, 5, 80, 20, 8, 0), (3001, 2, 128, 128, 1, 4), (8195, 1, 8, 2, 0, 0),
+                                          (8195, 3, 72, 36, 3, 4), (5000, 2, 256, 250, 0, 0), (4099, 20, 64, 2, 0, 0)):
+        positions = rng.integers(0, 100000, n)
+        _rope_check(hip, dev, rng, n, heads, hd, rot, layout, dtype, odtype, positions, pad=pad, shift=shift)
+        if dtype == odtype:
+            px, ld, _ = _rows(rng, dev, dtype, n, heads * hd, pad, shift)
+            raw = dev.get(px, (n, ld), bits_dtype(dtype)).copy()
+            out, pp = dev.put(raw, shift), dev.put(positions.astype(np.int32))
+            r = hip.Rope(hd, rot, layout)
+            r.rotate(dtype, px, ld, n, heads, pp, dtype, out, ld)
+            r.rotate(dtype, px, ld, n, heads, pp, dtype, px, ld)
+            r.close()
+            got = dev.get(px, (n, ld), bits_dtype(dtype))
+            assert np.array_equal(got, dev.get(out, (n, ld), bits_dtype(dtype))) and not np.array_equal(got, raw)
+        dev.close()
+
+
+@pytest.mark.parametrize("cache,dtype", [(W.F32, W.F32), (W.F16, W.F32), (W.BF16, W.BF16), (W.Q8_0, W.F32), (W.Q8_0, W.F16)])
+def test_cache_many_rows(hip, dev, cache, dtype):
+    """Four rows a thread and a rest, side by side in a block and over two blocks: bit for bit, as in test_cache_rows."""
+    rng = np.random.default_rng(82)
+    for n, heads, hd, page, pad in ((12500, 8, 64, 16, 0), (1801, 30, 136, 64, 5), (6001, 3, 72, 1024, 1)):
+        width, pages = heads * hd, -(-(n + 9) // page) + 1
+        c = hip.KVPages(cache, 1, heads, hd, page, pages)
+        (kb, k), (vb, v) = (_encoded(dtype, rng.standard_normal((n, width + pad)) * np.exp(rng.standard_normal(width + pad))) for _ in range(2))
+        slots = rng.permutation(pages * page)[:n].astype(np.int32)
+        gone = rng.random(n) < 0.05
+        slots[gone] = rng.choice([-1, pages * page, -(1 << 31)], gone.sum())
+        ps = dev.put(slots)
+        c.write(0, dtype, dev.put(kb), width + pad, dev.put(vb), width + pad, ps, n)
+        ko, vo = _empty(dev, W.F32, n, width, pad), _empty(dev, W.F32, n, width, pad)
+        c.read(0, W.F32, ko, width + pad, vo, width + pad, ps, n)
+        for out, x in ((ko, k), (vo, v)):
+            want = np.where(gone[:, None], 0, _held(cache, x[:, :width], hd))
+            assert np.array_equal(_take(dev, out, W.F32, n, width, pad), want.astype(np.float32))
+        rest = np.setdiff1d(np.arange(pages * page), slots).astype(np.int32)
+        ko, vo = (_empty(dev, W.F32, len(rest), width) for _ in range(2))
+        c.read(0, W.F32, ko, width, vo, width, dev.put(rest), len(rest))
+        assert not dev.get(ko, (len(rest), width)).any() and not dev.get(vo, (len(rest), width)).any()
+        c.close()
+        dev.close()
