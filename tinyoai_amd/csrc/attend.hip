@@ -35,10 +35,10 @@
 // the pieces of others leave unnormalised records {m, sum, o}, two a wave at
 // most, which a second kernel joins in order.
 //
-// Two contexts of 131071 positions (8 fp16 key heads of 64): 103 us, 5.2 TB/s (a
+// Two contexts of 131071 positions (8 fp16 key heads of 64): 104 us, 5.2 TB/s (a
 // copy on this card: 4.9). 64 requests of up to 4096 (32 over 8 bf16 heads of
-// 128): 31 to 41 us with the lengths drawn, 28 the floor of their mean. 8-bit
-// pages, 32 requests of up to 2048 (22 heads of 128, fp32 queries): 28 to 34 us,
+// 128): 31 to 45 us with the lengths drawn, 28 the floor of their mean. 8-bit
+// pages, 32 requests of up to 2048 (22 heads of 128, fp32 queries): 28 to 35 us,
 // bound by the codes' and planes' vector work (660 instructions a tile). One
 // request of 700 positions (32 heads of 80): 11 us, two launches' latencies. With
 // ranges of a fixed length for each block instead of equal runs for each wave the

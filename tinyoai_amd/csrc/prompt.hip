@@ -17,9 +17,9 @@
 // step, V read as it lies.
 //
 // What bounds it: at length the power the card gives. 8192 queries and keys, 32
-// over 8 bf16 heads of 128, all seen: 1.07 ms, 1028 TFLOP/s; 16381 fp16 tokens of
-// 32 heads of 80, causal: 1.51 ms, 910 (a library product of 8192^3: 1160 to
-// 1207). There the clock falls to 1.6 to 1.9 GHz, and fewer cycles (products
+// over 8 bf16 heads of 128, all seen: 1.03 to 1.07 ms, 1028 to 1065 TFLOP/s by the
+// card; 16381 fp16 tokens of 32 heads of 80, causal: 1.50 to 1.60 ms, 860 to 915 (a
+// library product of 8192^3: 1160 to 1207). There the clock falls to 1.6 to 1.9 GHz, and fewer cycles (products
 // scheduled between their operands' reads and the weights) do not change the
 // time, fewer bytes do: 64 queries a wave for heads up to 64 (829 -> 882). At few
 // thousand queries it is the longest block's chain of tiles, 1.3 to 2 us each
@@ -27,6 +27,11 @@
 // parts whose sums a second kernel joins (296 queries over 12000 keys 81 -> 58
 // us), or over groups of waves in a block (19 over 449 in fp32 61 -> 16).
 // fp32: 140 TFLOP/s at heads of 128 (a library product: 154).
+//
+// 16-bit weights are rounded to their type before the product with V, and summed
+// as rounded. Errors against 64 bits are 1.2 to 1.4 times those of results that
+// are only rounded themselves; a second plane for the rest of the weights would
+// double the products with V.
 #include <type_traits>
 
 #include "attend.h"
