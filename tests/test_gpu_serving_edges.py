@@ -26,9 +26,9 @@ def dev():
 
 # ---------------------------------------------------------------- new tokens: more work than a launch has waves
 # (query heads, key heads, head width, page, sequences, longest): a wave's run holds several pairs or pieces of them. In the
-# first, pairs of a sequence and a key head are fewer than the waves (1024 at 256 values a head, 2048 at up to 128, 3072 at
-# up to 64, 4096 at up to 32), in the others more.
-MANY = [(16, 8, 64, 64, 12, 2100), (32, 32, 80, 16, 96, 500), (8, 4, 256, 32, 300, 200), (360, 20, 128, 8, 60, 150),
+# first, pairs of a sequence and a key head are fewer than the waves (four blocks of four a CU at up to 32 values a head,
+# three at up to 64, two at up to 128, two of two waves at 256), in the others more.
+MANY = [(16, 8, 64, 64, 12, 2100), (32, 32, 80, 16, 95, 500), (8, 4, 256, 32, 300, 200), (360, 20, 128, 8, 60, 150),
         (64, 32, 64, 64, 100, 300), (32, 32, 24, 4, 130, 90)]
 
 
